@@ -16,6 +16,7 @@ LIB_PATH = os.environ.get("DEVIS_HIP_LIB") or os.path.join(_HERE, "libdevis_hip.
 DEVIS_F32, DEVIS_BF16 = 0, 1
 LABEL_I64, LABEL_U8, LABEL_I32 = 0, 1, 2
 EVID_MAX_K = 8
+TOP_MAX_K = 128
 EVID_SCAL_FLOATS = 4 + 3 * EVID_MAX_K
 
 _STATUS = {-1: "bad argument", -2: "unsupported shape", -3: "HIP error", -4: "workspace too small",
@@ -53,6 +54,23 @@ class EvidParams(C.Structure):
                 ("lam", C.c_float), ("a_au", C.c_float), ("eps", C.c_float)]
 
 
+class DistillParams(C.Structure):
+    _fields_ = [("N", C.c_int64), ("V", C.c_int64), ("K", C.c_int64), ("k", C.c_int64),
+                ("sN", C.c_int64), ("sV", C.c_int64), ("sK", C.c_int64),
+                ("oN", C.c_int64), ("oV", C.c_int64), ("oK", C.c_int64),
+                ("values", C.c_void_p), ("indices", C.c_void_p), ("rest", C.c_void_p), ("row_mask", C.c_void_p),
+                ("temperature", C.c_float), ("dtype", C.c_int), ("values_dtype", C.c_int), ("index_dtype", C.c_int),
+                ("mean", C.c_int)]
+
+
+class VerifyParams(C.Structure):
+    _fields_ = [("B", C.c_int64), ("T", C.c_int64), ("Tp", C.c_int64), ("K", C.c_int64),
+                ("pB", C.c_int64), ("pT", C.c_int64), ("pK", C.c_int64),
+                ("qB", C.c_int64), ("qT", C.c_int64), ("qK", C.c_int64),
+                ("tokens", C.c_void_p), ("accept_u", C.c_void_p), ("sample_u", C.c_void_p), ("lengths", C.c_void_p),
+                ("dtype", C.c_int), ("token_dtype", C.c_int)]
+
+
 CRIT_DCE, CRIT_DCEU, CRIT_CE, CRIT_MSE, CRIT_KL = range(5)
 PACK_CONV, PACK_CONV_DGRAD, PACK_CONVT, PACK_CONVT_DGRAD = range(4)
 PACK_CHUNK = 1024
@@ -61,6 +79,7 @@ PACK_ROW_FLAG, PACK_ROW_MAX = 0x40000000, 8192
 _P, _I64, _I, _F, _SZ = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_size_t
 _CD, _CTD, _EP = C.POINTER(ConvDesc), C.POINTER(ConvTDesc), C.POINTER(EvidParams)
 _CS = C.POINTER(ConvStats)
+_DP, _VP = C.POINTER(DistillParams), C.POINTER(VerifyParams)
 
 # name -> (restype, argtypes); every symbol include/devis_hip.h declares
 SIGNATURES = {
@@ -116,6 +135,12 @@ SIGNATURES = {
     "devis_evid_crit_fwd": (_I, [_EP, _P, _I64, _I64, _I64, _I, _P, _P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _SZ, _P]),
     "devis_evid_crit_bwd": (_I, [_EP, _P, _I64, _I64, _I64, _I, _P, _P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P]),
     "devis_evid_infer": (_I, [_P, _I64, _I64, _I64, _I, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _I, _P]),
+    "devis_top_logits": (_I, [_P, _I64, _I64, _I64, _I, _I64, _I64, _I64, _I64, _F, _P, _P, _I, _I64, _I64, _I64, _P, _P]),
+    "devis_distill_workspace_bytes": (_SZ, [_DP]),
+    "devis_distill_stats_bytes": (_SZ, [_DP]),
+    "devis_distill_fwd": (_I, [_DP, _P, _P, _P, _P, _P, _SZ, _P]),
+    "devis_distill_bwd": (_I, [_DP, _P, _P, _P, _P, _I, _P, _I64, _I64, _I64, _P]),
+    "devis_verify_drafts": (_I, [_VP, _P, _P, _P, _P, _P]),
     "devis_att_chunks": (_I64, [_I64]),
     "devis_att_psi_bwd_chunks": (_I64, [_I64, _I64, _I]),
     "devis_att_psi_fwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _P, _P, _SZ, _P]),

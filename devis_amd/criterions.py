@@ -164,6 +164,62 @@ def dce_evidence_u_loss(p, alpha, c, current_step, lamda_step, total_step, eps, 
     return pv + (1 - a_au) * dice
 
 
+# --------------------------------------------------------------------------- distillation (no counterpart in the reference)
+class _DistillFn(torch.autograd.Function):
+    """logits -> loss (scalar, or one per row), given the teacher's top logits."""
+
+    @staticmethod
+    def forward(ctx, logits, values, indices, rest, row_mask, channels_last, temperature, reduction, grad_on):
+        rows = reduction == "none"
+        params, dev, shape, ts = ops.distill_params(logits, values, indices, rest, row_mask, channels_last, temperature,
+                                                    reduction == "mean")
+        ctx.empty = params.N * params.V == 0
+        if ctx.empty:
+            ctx.like = logits.shape, logits.dtype, dev
+            return torch.zeros(shape if rows else (), dtype=torch.float32, device=dev)
+        need = grad_on and ctx.needs_input_grad[0]
+        per_row, scal, stats = ops.distill_fwd(params, dev, shape, ts[0], rows, not rows, need)
+        ctx.save_for_backward(*ts, stats, scal)
+        ctx.params, ctx.channels_last, ctx.rows = params, channels_last, rows
+        ctx.at = tuple(None if t is None else (t.data_ptr(), t.stride()) for t in ts)
+        return per_row if rows else scal[0].clone()
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        if ctx.empty:
+            shape, dtype, dev = ctx.like
+            return (torch.zeros(shape, dtype=dtype, device=dev),) + (None,) * 8
+        *ts, stats, scal = ctx.saved_tensors
+        x, params = ts[0], ctx.params
+        if tuple(None if t is None else (t.data_ptr(), t.stride()) for t in ts) != ctx.at:      # moved by saved-tensor hooks
+            params, _, _, ts = ops.distill_params(*ts, ctx.channels_last, params.temperature, params.mean)
+            x = ts[0]
+        g = g.contiguous().float()
+        return (ops.distill_bwd(params, x.device, x, ctx.channels_last, stats, scal, g, ctx.rows),) + (None,) * 8
+
+
+def distill_top_loss(logits: Tensor, values: Tensor, indices: Tensor, rest: Optional[Tensor] = None, channels_last: bool = True,
+                     temperature: float = 1.0, row_mask: Optional[Tensor] = None, reduction: str = "mean") -> Tensor:
+    """Distillation of a student's rows from a teacher's largest logits (``ops.top_logits``), differentiable in
+    ``logits``: temperature^2 * KL(p || q) with q = softmax(logits / temperature) and p = softmax over the teacher's slots
+    ``values / temperature`` at the classes ``indices`` - and, given ``rest``, over one class more that stands for every
+    class in no slot (q's share of it is their sum); without ``rest`` the slots alone are normalised.
+
+    ``logits`` (..., K), or (N, K, ...) with ``channels_last=False``, float32 or bfloat16, any strides; ``values`` (float32
+    or bfloat16) and ``indices`` (uint8, int32 or int64) with k <= 128 in the place of K; ``rest`` float32, one per row, at
+    the same temperature.  A slot whose value is -inf is empty.  Rows with ``row_mask`` (bool or uint8) 0, and rows without
+    a filled slot, have loss and gradient 0 whatever they hold.  A filled slot whose class is not in [0, K) makes its row
+    NaN.  A class in two slots is aimed at by both.
+    ``reduction``: "mean" over the counted rows (0 if there is none), "sum", or "none" (fp32, one per row)."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError("reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
+    if values.requires_grad or (rest is not None and rest.requires_grad):
+        raise ValueError("distill_top_loss does not differentiate in the teacher: detach values and rest")
+    return _DistillFn.apply(logits, values, indices, rest, row_mask, bool(channels_last), float(temperature), reduction,
+                            torch.is_grad_enabled())
+
+
 # --------------------------------------------------------------------------- API-compat shims (torch ops)
 def get_soft_label(input_tensor: Tensor, num_class: int) -> Tensor:
     """criterions.py:353-370: (N,1,...) integer labels -> (N,...,K) float one-hot."""

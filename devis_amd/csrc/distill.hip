@@ -1,0 +1,368 @@
+// Distillation from a teacher's top logits (toplogits.hip makes them), loss and gradient.
+//
+//   teacher: k slots (t_j, class i_j), t_j = -inf for an empty one, and optionally rest = log sum of exp(t / T) over
+//   every other class;  p = softmax over {t_j / T} and rest,  q = softmax(z / T) of the student's row,
+//   q_rest = the sum of q over the classes in no slot
+//   L      = T^2 [ sum_j p_j (log p_j - log q_{i_j}) + p_rest (log p_rest - log q_rest) ]
+//   dL/dz_c = T [ q_c - sum_{j: i_j = c} p_j ],  and T [ q_c - p_rest q_c / q_rest ] for a class in no slot.
+//
+// Without rest, p_rest = 0 and the top is renormalised.  Both passes are bound by memory: the forward reads the row
+// once with a running maximum and sum per thread, keeping the classes in no slot apart (a bit per class in LDS tells
+// them); the backward reads it once more and writes the gradient: for a class in no slot it is one exponential times a
+// factor of the row, W = 1/s - p_rest/s_rest; the k listed classes are put right afterwards.
+#include "rows.h"
+
+namespace devis {
+
+constexpr int DIS_MAX_K = DEVIS_TOP_MAX_K;
+constexpr int DIS_SEG = 131072;               // classes whose slot bits are in LDS at a time (16 KB)
+constexpr int DIS_MAX_BLOCKS = 2048;          // 8 blocks of 256 threads on each of 256 CUs
+
+// what the backward needs of a row
+struct RowStats { float ref, w, m, inv_s; };  // gradient of a class in no slot: exp((z - ref)/T) w;  q = exp((z - m)/T) inv_s
+
+struct Teacher {
+  const void* values; const void* indices; const float* rest; const uint8_t* mask;
+  RowShape o;                                 // strides of values / indices, K = number of slots
+  int value_kind, index_kind;
+};
+
+__device__ __forceinline__ int class_at(const void* idx, int kind, int64_t at) {
+  if (kind == DEVIS_LABEL_U8) return ((const uint8_t*)idx)[at];
+  if (kind == DEVIS_LABEL_I32) return ((const int32_t*)idx)[at];
+  const int64_t c = ((const int64_t*)idx)[at];
+  return c < 0 || c > 0x7ffffffe ? -1 : (int)c;
+}
+
+struct SlotShared {
+  float p[DIS_MAX_K];          // share of each slot
+  int c[DIS_MAX_K];            // its class
+  double p_rest, log_p_rest;
+  int state;                   // 0 row not counted (masked, or every slot empty), 1 counted, 2 a slot names no class
+};
+
+// The teacher's softmax of one row, by the first wave; log p_j stay in registers (lane l: slots l and l + 64).  Shares
+// come from fp32 exponentials of fp64 differences; the normaliser and every logarithm are fp64, because the loss is
+// the difference of near-equal logarithms once the student is near the teacher.
+__device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int K, double inv_t, SlotShared& sh, double (&logp)[2],
+                                            int (&cls)[2]) {
+  const int lane = threadIdx.x;
+  const int k = t.o.K;
+  const int64_t at = row_offset(t.o, r);
+  double y[2];
+  bool bad = false, any = false;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int j = lane + 64 * u;
+    y[u] = -__builtin_inf();
+    cls[u] = 0;
+    if (j < k) {
+      const int64_t i = at + j * t.o.sK;
+      const float v = t.value_kind == DEVIS_F32 ? ((const float*)t.values)[i] : (float)((const bf16*)t.values)[i];
+      if (v != neg_inf()) {
+        any = true;
+        y[u] = (double)v * inv_t;
+        cls[u] = class_at(t.indices, t.index_kind, i);
+        if (cls[u] < 0 || cls[u] >= K) { bad = true; cls[u] = 0; }
+      }
+    }
+  }
+  const int state = !__any(any) ? 0 : __any(bad) ? 2 : 1;
+  const double yr = t.rest ? (double)t.rest[r] : -__builtin_inf();
+  double hi = fmax(fmax(y[0], y[1]), yr);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) hi = fmax(hi, __shfl_xor(hi, o, 64));
+  const float e0 = expf((float)(y[0] - hi)), e1 = expf((float)(y[1] - hi)), er = expf((float)(yr - hi));
+  const double sum = wave_sum((double)e0 + (double)e1) + (double)er;
+  const double ls = log(sum);
+  logp[0] = y[0] - hi - ls;
+  logp[1] = y[1] - hi - ls;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int j = lane + 64 * u;
+    if (j < k) {
+      sh.p[j] = (float)((double)(u ? e1 : e0) / sum);
+      // an empty slot takes part in nothing
+      sh.c[j] = y[u] == -__builtin_inf() ? -1 : cls[u];
+    }
+  }
+  if (lane == 0) {
+    sh.p_rest = (double)er / sum;
+    sh.log_p_rest = yr - hi - ls;
+    sh.state = state;
+  }
+}
+
+__device__ __forceinline__ bool row_masked(const Teacher& t, int64_t r) { return t.mask && t.mask[r] == 0; }
+
+template <typename T, bool UNIT, bool REST, int BS>
+__global__ void __launch_bounds__(BS)
+k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, double t2, RowStats* __restrict__ stats,
+              float* __restrict__ per_row, double* __restrict__ partial) {
+  __shared__ SlotShared sh;
+  __shared__ uint32_t s_bits[REST ? DIS_SEG / 32 : 1];
+  __shared__ double s_red[BS / 64];
+  __shared__ float s_max[BS / 64];
+  const int tid = threadIdx.x, K = s.K;
+  const int64_t NV = s.N * s.V;
+  double loss_sum = 0.;
+  int64_t count = 0;
+  for (int64_t r = blockIdx.x; r < NV; r += gridDim.x) {
+    const T* p = z + row_offset(s, r);
+    double logp[2];
+    int cls[2];
+    if (row_masked(t, r)) {
+      if (tid == 0) sh.state = 0;
+    } else if (tid < 64) {
+      teacher_row(t, r, K, inv_t, sh, logp, cls);
+    }
+    __syncthreads();
+    const int state = sh.state;
+    if (state != 1) {
+      const float v = state == 2 ? __builtin_nanf("") : 0.f;
+      if (tid == 0) {
+        if (per_row) per_row[r] = v;
+        if (stats) stats[r] = RowStats{0.f, v, 0.f, v};
+        if (state == 2) { loss_sum += (double)v; ++count; }
+      }
+      __syncthreads();
+      continue;
+    }
+    // running maximum and sum of the classes in no slot (all classes without REST)
+    float m = neg_inf(), acc = 0.f;
+    for (int lo = 0; lo < K; lo += DIS_SEG) {
+      const int hi = K - lo < DIS_SEG ? K : lo + DIS_SEG;
+      if constexpr (REST) {
+        for (int i = tid; i < (hi - lo + 31) / 32; i += BS) s_bits[i] = 0;
+        __syncthreads();
+        for (int j = tid; j < t.o.K; j += BS) {
+          const int c = sh.c[j];
+          if (c >= lo && c < hi) atomicOr(&s_bits[(c - lo) >> 5], 1u << ((c - lo) & 31));
+        }
+        __syncthreads();
+      }
+      each_class<T, UNIT, BS>(p, s.sK, lo, hi, [&](auto& x, int c) {
+        constexpr int N = sizeof(x) / sizeof(float);
+        if constexpr (REST) {
+          const uint32_t b = s_bits[(c - lo) >> 5] >> ((c - lo) & 31);
+          if (b & ((1u << N) - 1u)) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = (b >> i) & 1u ? neg_inf() : x[i];
+          }
+        }
+        const float mx = max_of(x);
+        if (mx > m) { acc *= exp2_f((m - mx) * scale); m = mx; }
+        const float ref = m == neg_inf() ? 0.f : m;
+        float e[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = exp2_f((x[i] - ref) * scale);
+        acc += sum_of(e);
+      });
+      if constexpr (REST) __syncthreads();
+    }
+    const float m_rest = block_max<BS>(m, s_max);
+    const float ref = m_rest == neg_inf() ? 0.f : m_rest;
+    double sum_rest = block_sum<BS>(m == neg_inf() ? (double)acc : (double)acc * (double)exp2_f((m - ref) * scale), s_red);
+    if (tid < 64) {
+      // the listed classes' logits; a class in two slots counts once in the student's sum (its first slot)
+      float x[2];
+      bool first[2];
+      float m_all = m_rest;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int j = tid + 64 * u;
+        x[u] = neg_inf();
+        first[u] = false;
+        if (j < t.o.K && sh.c[j] >= 0) {
+          x[u] = (float)p[(int64_t)cls[u] * s.sK];
+          if constexpr (REST) {
+            first[u] = true;
+            for (int i = 0; i < j; ++i) first[u] = first[u] && sh.c[i] != cls[u];
+          }
+        }
+      }
+      double sum = sum_rest;
+      if constexpr (REST) {
+        m_all = fmaxf(m_rest, wave_max(fmaxf(x[0], x[1])));
+        const float ra = m_all == neg_inf() ? 0.f : m_all;
+        double mine = 0.;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) if (first[u]) mine += (double)exp2_f((x[u] - ra) * scale);
+        sum = wave_sum(mine) + (m_rest == neg_inf() ? sum_rest : sum_rest * exp2(((double)m_rest - (double)ra) * (double)inv_t * 1.4426950408889634));
+      }
+      const double m_d = m_all == neg_inf() ? 0. : (double)m_all;
+      const double ls = log(sum);             // log q = (x - m)/T - ls: the large part cancels first
+      double kl = 0.;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int j = tid + 64 * u;
+        if (j < t.o.K && sh.c[j] >= 0) {
+          const double pj = (double)sh.p[j];
+          const double logq = x[u] == neg_inf() ? -__builtin_inf() : ((double)x[u] - m_d) * inv_t - ls;
+          if (!(pj == 0.)) kl += pj * (logp[u] - logq);
+        }
+      }
+      kl = wave_sum(kl);
+      if (tid == 0) {
+        const double pr = sh.p_rest;
+        double inv = sum > 0. ? 1. / sum : sum == 0. ? 0. : sum;
+        double w = inv;
+        if constexpr (REST) {
+          const double log_q_rest = sum_rest == 0. ? -__builtin_inf() : ((double)ref - m_d) * inv_t + log(sum_rest) - ls;
+          if (!(pr == 0.)) kl += pr * (sh.log_p_rest - log_q_rest);
+          // q = exp((z - m_rest)/T) * w before the teacher's share of the rest is taken off
+          w = m_rest == neg_inf() ? 0. : inv * exp2(((double)m_rest - m_d) * inv_t * 1.4426950408889634) - pr / sum_rest;
+        }
+        const double loss = t2 * kl;
+        if (per_row) per_row[r] = (float)loss;
+        if (stats) stats[r] = RowStats{ref, (float)w, (float)m_d, (float)inv};
+        loss_sum += loss;
+        ++count;
+      }
+    }
+    __syncthreads();
+  }
+  if (partial && tid == 0) {
+    partial[2 * blockIdx.x] = loss_sum;
+    partial[2 * blockIdx.x + 1] = (double)count;
+  }
+}
+
+// scal[0] = sum or mean of the counted rows' losses, scal[1] = what a row's gradient is multiplied by, scal[2] = rows counted
+__global__ void __launch_bounds__(256)
+k_distill_finalize(const double* __restrict__ partial, int n, int mean, float* __restrict__ scal) {
+  __shared__ double s_red[4];
+  double loss = 0., count = 0.;
+  for (int i = threadIdx.x; i < n; i += 256) { loss += partial[2 * i]; count += partial[2 * i + 1]; }
+  loss = block_sum<256>(loss, s_red);
+  count = block_sum<256>(count, s_red);
+  if (threadIdx.x == 0) {
+    const double f = mean ? 1. / (count > 0. ? count : 1.) : 1.;
+    scal[0] = (float)(loss * f);
+    scal[1] = (float)f;
+    scal[2] = (float)count;
+  }
+}
+
+template <typename T, bool UNIT, bool REST, int BS>
+__global__ void __launch_bounds__(BS)
+k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
+              const RowStats* __restrict__ stats, const float* __restrict__ scal, const float* __restrict__ grad, int grad_rows,
+              T* __restrict__ dz, RowShape d) {
+  __shared__ SlotShared sh;
+  const int tid = threadIdx.x, K = s.K;
+  const int64_t NV = s.N * s.V;
+  for (int64_t r = blockIdx.x; r < NV; r += gridDim.x) {
+    const T* p = z + row_offset(s, r);
+    T* q = dz + row_offset(d, r);
+    double logp[2];
+    int cls[2];
+    if (row_masked(t, r)) {
+      if (tid == 0) sh.state = 0;
+    } else if (tid < 64) {
+      teacher_row(t, r, K, inv_t, sh, logp, cls);
+    }
+    __syncthreads();
+    const bool live = sh.state != 0;
+    const float g = grad_rows ? grad[r] : grad[0] * scal[1];
+    const float f = g * temperature;
+    RowStats st = {0.f, 0.f, 0.f, 0.f};
+    if (live) st = stats[r];
+    const float w = f * st.w;
+    if (!live) {
+      for (int c = tid; c < K; c += BS) q[(int64_t)c * d.sK] = (T)0.f;
+    } else {
+      each_class<T, UNIT, BS>(p, s.sK, 0, K, [&](auto& x, int c) {
+        constexpr int N = sizeof(x) / sizeof(float);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = exp2_f((x[i] - st.ref) * scale) * w;
+        store_vec(q + (int64_t)c * (UNIT ? 1 : d.sK), x);
+      });
+      __syncthreads();                       // the listed classes are written again, by other threads
+      for (int j = tid; j < t.o.K; j += BS) {
+        const int c = sh.c[j];
+        if (c < 0 || sh.state == 2) continue;
+        float share = 0.f;
+        for (int i = 0; i < t.o.K; ++i) share += sh.c[i] == c ? sh.p[i] : 0.f;
+        const float x = (float)p[(int64_t)c * s.sK];
+        const float qc = x == neg_inf() ? 0.f : exp2_f((x - st.m) * scale) * st.inv_s;
+        q[(int64_t)c * d.sK] = (T)(f * (qc - share));
+      }
+    }
+    __syncthreads();
+  }
+}
+
+static int distill_blocks(int64_t NV) { return (int)(NV < DIS_MAX_BLOCKS ? NV : DIS_MAX_BLOCKS); }
+
+static bool distill_args_ok(const devis_distill_params* a, const void* logits) {
+  if (!a || !logits || !a->values || !a->indices) return false;
+  if (!rows_ok(a->sN, a->sV, a->sK, a->N, a->V, a->K) || !rows_ok(a->oN, a->oV, a->oK, a->N, a->V, a->K)) return false;
+  if (a->k < 1 || a->k > a->K || a->k > DIS_MAX_K || a->index_dtype < 0 || a->index_dtype > 2) return false;
+  if (!(a->temperature > 0x1p-100f) || !(a->temperature < 0x1p100f)) return false;
+  if (a->values_dtype != DEVIS_F32 && a->values_dtype != DEVIS_BF16) return false;
+  return a->dtype == DEVIS_F32 || a->dtype == DEVIS_BF16;
+}
+
+}  // namespace devis
+
+using namespace devis;
+
+#define DISTILL_DISPATCH(KERNEL, ...)                                                                             \
+  DEVIS_DISPATCH_DTYPE(a->dtype, {                                                                                \
+    if (a->K <= 1024) {                                                                                           \
+      if (unit) { if (a->rest) KERNEL(true, true, 64); else KERNEL(true, false, 64); }                            \
+      else { if (a->rest) KERNEL(false, true, 64); else KERNEL(false, false, 64); }                               \
+    } else {                                                                                                      \
+      if (unit) { if (a->rest) KERNEL(true, true, 256); else KERNEL(true, false, 256); }                          \
+      else { if (a->rest) KERNEL(false, true, 256); else KERNEL(false, false, 256); }                             \
+    }                                                                                                             \
+  })
+
+extern "C" {
+
+size_t devis_distill_workspace_bytes(const devis_distill_params* a) {
+  return a ? (size_t)DIS_MAX_BLOCKS * 2 * sizeof(double) : 0;
+}
+
+size_t devis_distill_stats_bytes(const devis_distill_params* a) {
+  return a && a->N > 0 && a->V > 0 ? (size_t)a->N * (size_t)a->V * sizeof(RowStats) : 0;
+}
+
+int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* per_row, float* scal, void* stats, void* ws,
+                      size_t ws_bytes, void* stream) {
+  if (!distill_args_ok(a, logits) || (!per_row && !scal) || (scal && !ws)) return DEVIS_ERR_BAD_ARG;
+  if (scal && ws_bytes < devis_distill_workspace_bytes(a)) return DEVIS_ERR_WORKSPACE;
+  const RowShape s = {a->sN, a->sV, a->sK, a->N, a->V, (int)a->K};
+  const Teacher t = {a->values, a->indices, a->rest, a->row_mask, {a->oN, a->oV, a->oK, a->N, a->V, (int)a->k}, a->values_dtype, a->index_dtype};
+  const double inv_t = 1.0 / (double)a->temperature, t2 = (double)a->temperature * (double)a->temperature;
+  const float scale = (float)(1.4426950408889634 * inv_t);
+  const bool unit = a->sK == 1;
+  const int blocks = distill_blocks(a->N * a->V);
+  double* part = scal ? (double*)ws : nullptr;
+#define LAUNCH_DISTILL_FWD(UNIT, REST, BS) hipLaunchKernelGGL((k_distill_fwd<T, UNIT, REST, BS>), dim3(blocks), dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, t2, (RowStats*)stats, per_row, part)
+  DISTILL_DISPATCH(LAUNCH_DISTILL_FWD);
+#undef LAUNCH_DISTILL_FWD
+  const int rc = launch_status();
+  if (rc || !scal) return rc;
+  hipLaunchKernelGGL(k_distill_finalize, dim3(1), dim3(256), 0, (hipStream_t)stream, (const double*)ws, blocks, a->mean, scal);
+  return launch_status();
+}
+
+int devis_distill_bwd(const devis_distill_params* a, const void* logits, const void* stats, const float* scal, const float* grad,
+                      int grad_rows, void* dlogits, int64_t dN, int64_t dV, int64_t dK, void* stream) {
+  if (!distill_args_ok(a, logits) || !stats || !grad || !dlogits || (!grad_rows && !scal)) return DEVIS_ERR_BAD_ARG;
+  if (!rows_ok(dN, dV, dK, a->N, a->V, a->K)) return DEVIS_ERR_BAD_ARG;
+  const RowShape s = {a->sN, a->sV, a->sK, a->N, a->V, (int)a->K}, d = {dN, dV, dK, a->N, a->V, (int)a->K};
+  const Teacher t = {a->values, a->indices, a->rest, a->row_mask, {a->oN, a->oV, a->oK, a->N, a->V, (int)a->k}, a->values_dtype, a->index_dtype};
+  const double inv_t = 1.0 / (double)a->temperature;
+  const float scale = (float)(1.4426950408889634 * inv_t);
+  const bool unit = a->sK == 1 && dK == 1;
+  const int blocks = distill_blocks(a->N * a->V);
+#define LAUNCH_DISTILL_BWD(UNIT, REST, BS) hipLaunchKernelGGL((k_distill_bwd<T, UNIT, REST, BS>), dim3(blocks), dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, (const RowStats*)stats, scal, grad, grad_rows, (T*)dlogits, d)
+  DISTILL_DISPATCH(LAUNCH_DISTILL_BWD);
+#undef LAUNCH_DISTILL_BWD
+  return launch_status();
+}
+
+}  // extern "C"

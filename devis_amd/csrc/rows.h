@@ -1,0 +1,143 @@
+// Rows of class values: what the kernels over two models' class distributions share (toplogits.hip, distill.hip,
+// verify.hip).  A row is one voxel's or one token's K class values; row r = (n, v) starts at n*sN + v*sV and its
+// classes are sK apart, so one kernel takes channels-last voxels, channels-first volumes (sK = V) and vocabulary rows.
+#pragma once
+#include "common.h"
+
+namespace devis {
+
+struct RowShape { int64_t sN, sV, sK, N, V; int K; };
+
+__device__ __forceinline__ int64_t row_offset(const RowShape& s, int64_t r) {
+  if (s.V == 1) return r * s.sN;
+  const int64_t n = r / s.V;
+  return n * s.sN + (r - n * s.V) * s.sV;
+}
+
+__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+__device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 16 bytes of consecutive classes.  A row of an odd vocabulary starts at any multiple of the element size: the copies
+// below compile to one 16-byte access that the hardware takes at any address.
+template <typename T> constexpr int vec_of() { return 16 / (int)sizeof(T); }
+
+struct Raw16 { uint32_t w[4]; };
+
+template <typename T> __device__ __forceinline__ Raw16 load16(const T* p) {
+  Raw16 r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+__device__ __forceinline__ void unpack(const Raw16& r, float (&x)[8]) {      // bf16
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __builtin_bit_cast(float, r.w[i] << 16);
+    x[2 * i + 1] = __builtin_bit_cast(float, r.w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack(const Raw16& r, float (&x)[4]) {      // fp32
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = __builtin_bit_cast(float, r.w[i]);
+}
+__device__ __forceinline__ void store_vec(bf16* p, const float (&x)[8]) {
+  Raw16 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+  __builtin_memcpy(p, &r, 16);
+}
+__device__ __forceinline__ void store_vec(float* p, const float (&x)[4]) { __builtin_memcpy(p, x, 16); }
+template <typename T> __device__ __forceinline__ void store_vec(T* p, const float (&x)[1]) { *p = (T)x[0]; }
+
+// f(x, c): x = the values of classes c, c + 1, .. (VEC of them, or one at a time behind the last whole vector), over
+// the classes [lo, hi) of one row, dealt to the BS threads of a block vector by vector.  UNIT: the classes are
+// adjacent in memory (sK = 1) and travel 16 bytes at a time, four loads in flight; otherwise one by one.
+template <typename T, bool UNIT, int BS, typename F>
+__device__ __forceinline__ void each_class(const T* __restrict__ p, int64_t sK, int lo, int hi, F f) {
+  const int tid = threadIdx.x;
+  if constexpr (UNIT) {
+    constexpr int VEC = vec_of<T>();
+    const int full = (hi - lo) / VEC;
+    const T* q = p + lo;
+    int v = tid;
+    for (; v + 3 * BS < full; v += 4 * BS) {
+      Raw16 r[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) r[u] = load16(q + (int64_t)(v + u * BS) * VEC);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float x[VEC];
+        unpack(r[u], x);
+        f(x, lo + (v + u * BS) * VEC);
+      }
+    }
+    for (; v < full; v += BS) {
+      float x[VEC];
+      unpack(load16(q + (int64_t)v * VEC), x);
+      f(x, lo + v * VEC);
+    }
+    const int c = lo + full * VEC + tid;
+    if (c < hi) {
+      float x[1] = {(float)p[c]};
+      f(x, c);
+    }
+  } else {
+    for (int c = lo + tid; c < hi; c += BS) {
+      float x[1] = {(float)p[(int64_t)c * sK]};
+      f(x, c);
+    }
+  }
+}
+
+template <int N> __device__ __forceinline__ float max_of(const float (&x)[N]) {
+  float m = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
+  return m;
+}
+template <int N> __device__ __forceinline__ float sum_of(const float (&x)[N]) {
+  if constexpr (N == 1) return x[0];
+  else {
+    float y[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) y[i] = x[2 * i] + x[2 * i + 1];
+    return sum_of(y);
+  }
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// block-wide reductions, the result in every thread; `s` holds BS/64 entries and is free again on return
+template <int BS> __device__ __forceinline__ float block_max(float v, float* s) {
+  v = wave_max(v);
+  if constexpr (BS > 64) {
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = s[0];
+#pragma unroll
+    for (int i = 1; i < BS / 64; ++i) v = fmaxf(v, s[i]);
+    __syncthreads();
+  }
+  return v;
+}
+template <int BS> __device__ __forceinline__ double block_sum(double v, double* s) {
+  v = wave_sum(v);
+  if constexpr (BS > 64) {
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = s[0];
+#pragma unroll
+    for (int i = 1; i < BS / 64; ++i) v += s[i];
+    __syncthreads();
+  }
+  return v;
+}
+
+inline bool rows_ok(int64_t sN, int64_t sV, int64_t sK, int64_t N, int64_t V, int64_t K) {
+  return N > 0 && V > 0 && K > 0 && K < 0x7fffffff && sN >= 0 && sV >= 0 && sK > 0 && N <= INT64_MAX / V;
+}
+
+}  // namespace devis

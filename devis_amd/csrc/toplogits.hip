@@ -1,0 +1,201 @@
+// The k largest logits of every row and the log-sum-exp of what is left: a teacher's row reduced to what
+// distillation (distill.hip) learns from.
+//
+//   order the classes by (value descending, class ascending); values / indices = the first k;
+//   rest = log sum over the classes not among them of exp(z_c / T).
+//
+// Selection in two passes over the row.  A class is its 64-bit key (value as an ordered integer, class counted
+// downwards), so keys differ and every tie falls to the lowest class.  Pass 1: each thread's largest key; the k-th
+// largest of these BS keys, tau, has at least k keys at or above it, and rarely many more (73 expected for k = 64 of
+// 256 threads).  Pass 2: keys >= tau go to a list in LDS, everything else into the sum of exponentials; the list is
+// ranked by counting.  Memory is read once from HBM; pass 2 finds the row in L2 / Infinity Cache.
+#include "rows.h"
+
+namespace devis {
+
+constexpr int TOP_MAX_K = DEVIS_TOP_MAX_K;
+constexpr int TOP_CAP = 1024;                 // list entries; >= 8 * TOP_MAX_K, see the refinement below
+
+__device__ __forceinline__ float nan_high(float x) { return x != x ? __builtin_inff() : x; }
+
+__device__ __forceinline__ uint64_t top_key(float x, int c) {
+  uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);        // -0 orders as 0
+  b ^= (uint32_t)((int32_t)b >> 31) | 0x80000000u;
+  return ((uint64_t)b << 32) | (uint32_t)~c;
+}
+__device__ __forceinline__ int key_class(uint64_t key) { return (int)~(uint32_t)key; }
+__device__ __forceinline__ float key_value(uint64_t key) {
+  uint32_t b = (uint32_t)(key >> 32);
+  b ^= (b >> 31) ? 0x80000000u : 0xffffffffu;
+  return __builtin_bit_cast(float, b);
+}
+
+template <typename T, typename I, bool UNIT, int BS>
+__global__ void __launch_bounds__(BS)
+k_top_rows(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t, T* __restrict__ values,
+           I* __restrict__ indices, RowShape o, float* __restrict__ rest) {
+  __shared__ uint64_t s_group[BS];
+  __shared__ uint64_t s_list[TOP_CAP];
+  __shared__ uint64_t s_tau, s_kth;
+  __shared__ int s_n;
+  __shared__ double s_red[BS / 64];
+  __shared__ float s_max[BS / 64];
+  const int tid = threadIdx.x, K = s.K;
+  const int64_t NV = s.N * s.V;
+  for (int64_t r = blockIdx.x; r < NV; r += gridDim.x) {
+    const T* p = z + row_offset(s, r);
+    // pass 1: this thread's largest key (the vector first, then the class within it)
+    float best = neg_inf();
+    int at = -1;
+    each_class<T, UNIT, BS>(p, s.sK, 0, K, [&](auto& x, int c) {
+      constexpr int N = sizeof(x) / sizeof(float);
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = nan_high(x[i]);
+      const float m = max_of(x);
+      if (m > best || at < 0) { best = m; at = c; }
+    });
+    uint64_t mine = 0;
+    if (at >= 0) {
+      int c = at;
+      while (nan_high((float)p[(int64_t)c * s.sK]) != best) ++c;       // ends inside the vector that gave `best`
+      mine = top_key(best, c);
+    }
+    s_group[tid] = mine;
+    if (tid == 0) { s_tau = 0; s_n = 0; }
+    __syncthreads();
+    {
+      int above = 0;
+#pragma unroll 8
+      for (int j = 0; j < BS; ++j) above += s_group[j] > mine ? 1 : 0;
+      if (mine != 0 && above == k - 1) s_tau = mine;       // fewer than k threads hold a class: tau stays 0, all are listed
+    }
+    __syncthreads();
+    uint64_t tau = s_tau;
+    float floor_v, base;
+    double sum;
+    int n;
+    uint64_t below = ~0ull;                                // some key no class reaches
+    for (;;) {
+      floor_v = tau ? key_value(tau) : neg_inf();
+      base = floor_v == neg_inf() ? 0.f : floor_v;
+      float acc = 0.f;
+      each_class<T, UNIT, BS>(p, s.sK, 0, K, [&](auto& x, int c) {
+        constexpr int N = sizeof(x) / sizeof(float);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = nan_high(x[i]);
+        if (max_of(x) >= floor_v) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const uint64_t key = top_key(x[i], c + i);
+            if (key >= tau) {
+              const int at_n = atomicAdd(&s_n, 1);
+              if (at_n < TOP_CAP) s_list[at_n] = key;
+              x[i] = neg_inf();
+            }
+          }
+        }
+        float e[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = exp2_f((x[i] - base) * scale);
+        acc += sum_of(e);
+      });
+      __syncthreads();
+      n = s_n;
+      sum = (double)acc;
+      if (n <= TOP_CAP) break;
+      // More keys than the list holds (many large classes dealt to few threads).  Halve the interval [tau, below) until
+      // between k and TOP_CAP keys are left: keys differ, so the count takes every value in between.
+      __syncthreads();
+      for (;;) {
+        const uint64_t mid = tau + (below - tau) / 2;
+        int cnt = 0;
+        each_class<T, UNIT, BS>(p, s.sK, 0, K, [&](auto& x, int c) {
+          constexpr int N = sizeof(x) / sizeof(float);
+#pragma unroll
+          for (int i = 0; i < N; ++i) cnt += top_key(nan_high(x[i]), c + i) >= mid ? 1 : 0;
+        });
+        const int total = (int)block_sum<BS>((double)cnt, s_red);
+        if (total < k) below = mid;
+        else tau = mid;
+        if (total >= k && total <= TOP_CAP) break;
+      }
+      if (tid == 0) s_n = 0;
+      __syncthreads();
+    }
+    // rank the list; what does not make the first k joins the rest
+    for (int i = tid; i < n; i += BS) {
+      const uint64_t key = s_list[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += s_list[j] > key ? 1 : 0;
+      if (rank < k) {
+        const int64_t at_o = row_offset(o, r) + rank * o.sK;
+        const int c = key_class(key);
+        values[at_o] = p[(int64_t)c * s.sK];
+        indices[at_o] = (I)c;
+        if (rank == k - 1) s_kth = key;
+      } else {
+        sum += (double)exp2_f((key_value(key) - base) * scale);
+      }
+    }
+    if (rest) {
+      sum = block_sum<BS>(sum, s_red);
+      __syncthreads();
+      float ref = base;
+      // the rest lies far below the listed classes (or they are infinite): take its own largest value as reference
+      if (!(sum > 0x1p-60) || !(ref < __builtin_inff())) {
+        const uint64_t kth = s_kth;
+        float m = neg_inf();
+        each_class<T, UNIT, BS>(p, s.sK, 0, K, [&](auto& x, int c) {
+          constexpr int N = sizeof(x) / sizeof(float);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const float y = nan_high(x[i]);
+            if (top_key(y, c + i) < kth) m = fmaxf(m, y);
+          }
+        });
+        ref = block_max<BS>(m, s_max);
+        float acc = 0.f;
+        each_class<T, UNIT, BS>(p, s.sK, 0, K, [&](auto& x, int c) {
+          constexpr int N = sizeof(x) / sizeof(float);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const float y = nan_high(x[i]);
+            if (top_key(y, c + i) < kth && y > neg_inf()) acc += exp2_f((y - ref) * scale);
+          }
+        });
+        sum = block_sum<BS>((double)acc, s_red);
+      }
+      if (tid == 0) {
+        const bool unbounded = !(fabsf(ref) < __builtin_inff());       // nothing is left (-inf), or infinities are
+        rest[r] = unbounded ? ref : (float)((double)ref * inv_t + log(sum));
+      }
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace devis
+
+using namespace devis;
+
+extern "C" int devis_top_logits(const void* logits, int64_t sN, int64_t sV, int64_t sK, int dtype, int64_t N, int64_t V,
+                                int64_t K, int64_t k, float temperature, void* values, void* indices, int index_dtype,
+                                int64_t oN, int64_t oV, int64_t oK, float* rest, void* stream) {
+  if (!logits || !values || !indices || !rows_ok(sN, sV, sK, N, V, K) || !rows_ok(oN, oV, oK, N, V, K)) return DEVIS_ERR_BAD_ARG;
+  if (k < 1 || k > K || k > TOP_MAX_K || !(temperature > 0x1p-100f) || !(temperature < 0x1p100f)) return DEVIS_ERR_BAD_ARG;
+  if (index_dtype != DEVIS_LABEL_I32 && !(index_dtype == DEVIS_LABEL_U8 && K <= 256)) return DEVIS_ERR_BAD_ARG;
+  const RowShape s = {sN, sV, sK, N, V, (int)K}, o = {oN, oV, oK, N, V, (int)k};
+  const int64_t NV = N * V;
+  const double inv_t = 1.0 / (double)temperature;
+  const float scale = (float)(1.4426950408889634 * inv_t);
+  const hipStream_t st = (hipStream_t)stream;
+  const unsigned blocks = (unsigned)(NV < (1 << 20) ? NV : (1 << 20));
+#define LAUNCH_TOP(I, UNIT, BS) hipLaunchKernelGGL((k_top_rows<T, I, UNIT, BS>), dim3(blocks), dim3(BS), 0, st, (const T*)logits, s, (int)k, scale, inv_t, (T*)values, (I*)indices, o, rest)
+#define LAUNCH_TOP_U(I, BS) do { if (sK == 1) LAUNCH_TOP(I, true, BS); else LAUNCH_TOP(I, false, BS); } while (0)
+#define LAUNCH_TOP_B(I) do { if (K <= TOP_CAP) LAUNCH_TOP_U(I, 64); else LAUNCH_TOP_U(I, 256); } while (0)
+  DEVIS_DISPATCH_DTYPE(dtype, { if (index_dtype == DEVIS_LABEL_U8) LAUNCH_TOP_B(uint8_t); else LAUNCH_TOP_B(int32_t); });
+#undef LAUNCH_TOP_B
+#undef LAUNCH_TOP_U
+#undef LAUNCH_TOP
+  return launch_status();
+}

@@ -8,6 +8,7 @@ functions is differentiable by autograd - the manual backward lives in
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import threading
 from typing import Optional, Sequence, Tuple
@@ -936,3 +937,208 @@ def softplus_bwd(z: Tensor, g: Tensor) -> Tensor:
     dz = torch.empty_like(z)
     check(_lib.load().devis_softplus_bwd(_p(z), _p(g), _p(dz), z.numel(), _stream()), "softplus_bwd")
     return dz
+
+
+# ------------------------------------------------------------ two models' class distributions
+def class_rows(x: Tensor, channels_last: bool):
+    """``x`` (copied only if its strides are not regular) as rows of classes: (x, N, V, K, sN, sV, sK) with N the first
+    dimension and V the product of the others; row (n, v) starts at n*sN + v*sV, its classes are sK apart."""
+    if x.dim() < (1 if channels_last else 2):
+        raise _lib.DevisError("expected %s, got %d dimensions" % ("(..., K)" if channels_last else "(N, K, ...)", x.dim()))
+    kd = x.dim() - 1 if channels_last else 1
+    lead = [d for d in range(x.dim()) if d != kd]
+    n = x.shape[lead[0]] if lead else 1
+    v = 1
+    for d in lead[1:]:
+        v *= x.shape[d]
+
+    def strides(t):
+        st, size = None, 1
+        for d in reversed(lead[1:]):
+            if t.shape[d] == 1:
+                continue
+            if st is None:
+                st = t.stride(d)
+            elif t.stride(d) != st * size:
+                return None
+            size *= t.shape[d]
+        sk = t.stride(kd) if t.shape[kd] > 1 else 1
+        if sk <= 0:
+            return None
+        return (t.stride(lead[0]) if lead and t.shape[lead[0]] > 1 else 0), st or 0, sk
+
+    s = strides(x)
+    if s is None:
+        x = x.contiguous()
+        s = strides(x)
+    return (x, n, v, x.shape[kd]) + s
+
+
+def _same_device(what: str, *ts: Optional[Tensor]) -> torch.device:
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _lib.DevisError("devis_amd kernels need GPU tensors (got a %s tensor); there is no CPU fallback" % t.device)
+        if dev is not None and t.device != dev:
+            raise _lib.DevisError("%s: tensors on %s and %s" % (what, dev, t.device))
+        dev = t.device
+    return dev
+
+
+def _on_device(dev: torch.device):
+    """Kernels launch on the current device: make it the tensors' own where it is another."""
+    if dev.index == torch._C._cuda_getDevice():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def top_logits(logits: Tensor, k: int, channels_last: bool = True, temperature: float = 1.0, want_rest: bool = True):
+    """The k largest logits of every row and the mass of what is left, as ``criterions.distill_top_loss`` takes them.
+
+    ``logits``: (..., K) or, with ``channels_last=False``, (N, K, ...); float32 or bfloat16, any strides.
+    -> dict(values, indices, rest).  ``values`` (the logits' type) and ``indices`` (uint8 for K <= 256, else int32) have
+    the logits' shape with k in the place of K, largest first, the lowest class first among equals; a NaN counts as
+    +inf.  ``rest`` (fp32, one per row; None without ``want_rest``) = log of the sum over the other classes of
+    exp(z / temperature), -inf if none is left.  1 <= k <= min(K, 128).  Not differentiable."""
+    code = dt_code(logits.dtype)
+    x, n, v, kk, sn, sv, sk = class_rows(logits.detach(), channels_last)
+    k, temperature = int(k), float(temperature)
+    if not 1 <= k <= min(kk, _lib.TOP_MAX_K):
+        raise _lib.DevisError("top_logits: k must be in [1, min(K, %d)] = [1, %d], got %d" % (_lib.TOP_MAX_K, min(kk, _lib.TOP_MAX_K), k))
+    _check_temperature(temperature)
+    dev = _same_device("top_logits", x)
+    shape = tuple(x.shape[:-1]) if channels_last else (x.shape[0],) + tuple(x.shape[2:])
+    oshape = shape + (k,) if channels_last else (x.shape[0], k) + tuple(x.shape[2:])
+    idt = torch.uint8 if kk <= 256 else torch.int32
+    with _on_device(dev):
+        values = torch.empty(oshape, dtype=x.dtype, device=dev)
+        indices = torch.empty(oshape, dtype=idt, device=dev)
+        rest = torch.empty(shape, dtype=torch.float32, device=dev) if want_rest else None
+        if n * v:
+            on, ov, ok = class_rows(values, channels_last)[4:]
+            check(_lib.load().devis_top_logits(_p(x), sn, sv, sk, code, n, v, kk, k, temperature, _p(values), _p(indices),
+                                               _label_code(indices), on, ov, ok, _p(rest), _stream()), "top_logits")
+    return dict(values=values, indices=indices, rest=rest)
+
+
+def _check_temperature(t: float) -> None:
+    if not 2.0 ** -100 < t < 2.0 ** 100:
+        raise _lib.DevisError("temperature must be a positive finite number, got %r" % t)
+
+
+def distill_params(logits: Tensor, values: Tensor, indices: Tensor, rest: Optional[Tensor], row_mask: Optional[Tensor],
+                   channels_last: bool, temperature: float, mean: bool):
+    """-> (params, tensors the params point into).  All shapes, types and devices are checked here."""
+    x, n, v, kk, sn, sv, sk = class_rows(logits, channels_last)
+    shape = tuple(x.shape[:-1]) if channels_last else (x.shape[0],) + tuple(x.shape[2:])
+    t, tn, tv, k, on, ov, ok = class_rows(values, channels_last)
+    lead = tuple(t.shape[:-1]) if channels_last else (t.shape[0],) + tuple(t.shape[2:])
+    if lead != shape or t.dim() != x.dim():
+        raise _lib.DevisError("distill: values %s do not go with logits %s" % (tuple(values.shape), tuple(logits.shape)))
+    if indices.shape != values.shape:
+        raise _lib.DevisError("distill: values %s and indices %s differ in shape" % (tuple(values.shape), tuple(indices.shape)))
+    if not 1 <= k <= min(kk, _lib.TOP_MAX_K):
+        raise _lib.DevisError("distill: 1 to min(K, %d) = %d slots a row, got %d" % (_lib.TOP_MAX_K, min(kk, _lib.TOP_MAX_K), k))
+    i, _, _, _, *io = class_rows(indices, channels_last)
+    if tuple(io) != (on, ov, ok):
+        t, i = t.contiguous(), i.contiguous()
+        on, ov, ok = class_rows(t, channels_last)[4:]
+    _check_temperature(temperature)
+    if rest is not None:
+        if rest.dtype != torch.float32 or tuple(rest.shape) != shape:
+            raise _lib.DevisError("distill: rest must be float32 of shape %s, got %s %s" % (shape, rest.dtype, tuple(rest.shape)))
+        rest = rest.contiguous()
+    if row_mask is not None:
+        if row_mask.dtype not in (torch.bool, torch.uint8) or tuple(row_mask.shape) != shape:
+            raise _lib.DevisError("distill: row_mask must be bool or uint8 of shape %s, got %s %s" % (shape, row_mask.dtype, tuple(row_mask.shape)))
+        row_mask = row_mask.contiguous()
+    codes = dt_code(x.dtype), dt_code(t.dtype), _label_code(i)
+    dev = _same_device("distill", x, t, i, rest, row_mask)
+    p = _lib.DistillParams(n, v, kk, k, sn, sv, sk, on, ov, ok, _p(t), _p(i), _p(rest), _p(row_mask), temperature, *codes,
+                           1 if mean else 0)
+    return p, dev, shape, (x, t, i, rest, row_mask)
+
+
+def distill_fwd(params, dev: torch.device, shape, x: Tensor, want_rows: bool, want_scal: bool, want_stats: bool):
+    """-> (per_row fp32 | None, scal (3,) fp32 | None, stats | None)"""
+    lib = _lib.load()
+    with _on_device(dev):
+        f = dict(dtype=torch.float32, device=dev)
+        per_row = torch.empty(shape, **f) if want_rows else None
+        scal = torch.empty((3,), **f) if want_scal else None
+        stats = torch.empty((lib.devis_distill_stats_bytes(C.byref(params)),), dtype=torch.uint8, device=dev) if want_stats else None
+        # the workspace is the call's own (not `workspace`): a captured graph keeps what it allocates to itself, so two
+        # graphs replayed side by side do not meet in it
+        nb = lib.devis_distill_workspace_bytes(C.byref(params)) if want_scal else 0
+        ws = torch.empty((nb,), dtype=torch.uint8, device=dev) if want_scal else None
+        check(lib.devis_distill_fwd(C.byref(params), _p(x), _p(per_row), _p(scal), _p(stats), _p(ws), nb, _stream()), "distill_fwd")
+    return per_row, scal, stats
+
+
+def distill_bwd(params, dev: torch.device, x: Tensor, channels_last: bool, stats: Tensor, scal: Optional[Tensor],
+                grad: Tensor, grad_rows: bool) -> Tensor:
+    with _on_device(dev):
+        dx = torch.empty_like(x)
+        y, _, _, _, dn, dv, dk = class_rows(dx, channels_last)
+        if y is not dx:                                    # strides the kernel does not take
+            dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+            dn, dv, dk = class_rows(dx, channels_last)[4:]
+        check(_lib.load().devis_distill_bwd(C.byref(params), _p(x), _p(stats), _p(scal), _p(grad), 1 if grad_rows else 0,
+                                            _p(dx), dn, dv, dk, _stream()), "distill_bwd")
+    return dx
+
+
+def verify_drafts(tokens: Tensor, target_probs: Tensor, draft_probs: Optional[Tensor], accept_u: Tensor, sample_u: Tensor,
+                  lengths: Optional[Tensor] = None):
+    """Drafted classes verified against a target model's probabilities, so that what comes out is distributed as the
+    target's own draws.
+
+    ``tokens`` (B, T) int64 or int32; ``target_probs`` (B, T, K), or (B, T + 1, K) with a row behind the last draft;
+    ``draft_probs`` (B, T, K), or None for drafts that come without (a lookup, an arg max); both float32 or both
+    bfloat16, any strides.  ``accept_u`` (B, T) and ``sample_u`` (B,) are uniform in [0, 1), float32.  ``lengths`` (B,):
+    drafts of each sequence (clamped to [0, T]), T without.  Draft t is accepted while ``accept_u * draft < target`` at
+    its class; one class more is drawn from max(target - draft, 0) at the first refused place, or from the row behind the
+    last draft if all were accepted and there is one.
+    -> dict(tokens (B, target_probs.shape[1]): accepted, drawn, then -1; accepted (B,)), both of the tokens' type.
+    A label map is B = voxels, T = 1.  Not differentiable."""
+    if tokens.dim() != 2 or target_probs.dim() != 3:
+        raise _lib.DevisError("verify_drafts: tokens must be (B, T) and target_probs (B, T or T + 1, K)")
+    b, t = tokens.shape
+    tp, k = target_probs.shape[1:]
+    if tokens.dtype not in (torch.int64, torch.int32):
+        raise _lib.DevisError("verify_drafts: tokens must be int64 or int32")
+    if target_probs.shape[0] != b or tp not in (t, t + 1) or tp < 1 or k < 1:
+        raise _lib.DevisError("verify_drafts: target_probs %s do not go with tokens %s" % (tuple(target_probs.shape), (b, t)))
+    if draft_probs is not None and (tuple(draft_probs.shape) != (b, t, k) or draft_probs.dtype != target_probs.dtype):
+        raise _lib.DevisError("verify_drafts: draft_probs must be %s %s, got %s %s" %
+                              ((b, t, k), target_probs.dtype, tuple(draft_probs.shape), draft_probs.dtype))
+    for name, u, shape in (("accept_u", accept_u, (b, t)), ("sample_u", sample_u, (b,))):
+        if u.dtype != torch.float32 or tuple(u.shape) != shape:
+            raise _lib.DevisError("verify_drafts: %s must be float32 %s, got %s %s" % (name, shape, u.dtype, tuple(u.shape)))
+    if lengths is not None:
+        if lengths.dtype not in (torch.int64, torch.int32) or tuple(lengths.shape) != (b,):
+            raise _lib.DevisError("verify_drafts: lengths must be int64 or int32 (B,)")
+    code = dt_code(target_probs.dtype)
+    dev = _same_device("verify_drafts", tokens, target_probs, draft_probs, accept_u, sample_u, lengths)
+    if lengths is not None:
+        lengths = lengths.to(tokens.dtype).contiguous()
+    tokens, accept_u, sample_u = tokens.contiguous(), accept_u.contiguous(), sample_u.contiguous()
+
+    def regular(x):
+        x = x.detach()
+        return x if k == 1 or x.stride(2) > 0 else x.contiguous()
+    target = regular(target_probs)
+    draft = regular(draft_probs) if draft_probs is not None and t > 0 else None
+    ps = target.stride()
+    qs = draft.stride() if draft is not None else (0, 0, 1)
+    with _on_device(dev):
+        out = torch.empty((b, tp), dtype=tokens.dtype, device=dev)
+        accepted = torch.empty((b,), dtype=tokens.dtype, device=dev)
+        if b:
+            p = _lib.VerifyParams(b, t, tp, k, ps[0], ps[1], ps[2], qs[0], qs[1], qs[2], _p(tokens), _p(accept_u), _p(sample_u),
+                                  _p(lengths), code, _label_code(tokens))
+            check(_lib.load().devis_verify_drafts(C.byref(p), _p(target), _p(draft), _p(out), _p(accepted), _stream()),
+                  "verify_drafts")
+    return dict(tokens=out, accepted=accepted)

@@ -379,6 +379,73 @@ int devis_evid_infer(const void* logits, int64_t sN, int64_t sV, int64_t sK, int
  * when the evidence is consumed outside the fused loss. */
 int devis_softplus_bwd(const float* z, const float* g, float* dz, int64_t n, void* stream);
 
+/* ------------------------------------------- two models' class distributions -- */
+/* No counterpart in the reference.  A row is one voxel's or one token's K class values; row (n, v) of `logits` starts at
+ * n*sN + v*sV and its classes are sK apart (elements), as in devis_evid_loss_fwd; K has no upper bound below 2^31 - 1.
+ *
+ * devis_top_logits: the k <= DEVIS_TOP_MAX_K largest logits of every row.  Classes are ordered by (value descending,
+ * class ascending), a NaN as +inf; values (dtype of the logits) and indices (index_dtype: DEVIS_LABEL_I32, or
+ * DEVIS_LABEL_U8 for K <= 256) hold the first k in that order, slot j of row (n, v) at n*oN + v*oV + j*oK;
+ * rest (optional, [N*V] fp32) = log of the sum over all other classes of exp(z / temperature), -inf if none is left. */
+#define DEVIS_TOP_MAX_K 128
+int devis_top_logits(const void* logits, int64_t sN, int64_t sV, int64_t sK, int dtype, int64_t N, int64_t V,
+                     int64_t K, int64_t k, float temperature, void* values, void* indices, int index_dtype,
+                     int64_t oN, int64_t oV, int64_t oK, float* rest, void* stream);
+
+/* Distillation of a student's rows from a teacher's k top logits (slots; a value of -inf is an empty slot):
+ *   p = softmax over {values / temperature} and rest (no rest: the slots alone),  q = softmax(logits / temperature),
+ *   q_rest = the sum of q over the classes in no slot,
+ *   loss of a row = temperature^2 [ sum_j p_j (log p_j - log q_{i_j}) + p_rest (log p_rest - log q_rest) ].
+ * A row with row_mask[r] = 0 (r = n*V + v) or without a filled slot has loss and gradient 0 and is not counted.  A
+ * filled slot whose class is outside [0, K) makes its row's loss and gradient NaN; nothing is read there.
+ * fwd: per_row (optional, [N*V] fp32) the rows' losses; scal (optional, 3 fp32, with workspace)
+ *   [0] their sum, or mean over the counted rows (mean = 1; 0 if none is)  [1] 1 or 1/counted  [2] counted;
+ *   stats (devis_distill_stats_bytes, optional: needed by the backward).
+ * bwd: dlogits (dtype of the logits; strides dN, dV, dK) = gradient, times grad[0] * scal[1], or times grad[r] with
+ *   grad_rows = 1.  Results do not depend on the order in which blocks run. */
+typedef struct devis_distill_params {
+  int64_t N, V, K, k;
+  int64_t sN, sV, sK;   /* logits */
+  int64_t oN, oV, oK;   /* values and indices */
+  const void* values;   /* values_dtype */
+  const void* indices;  /* index_dtype: a devis_label_dtype */
+  const float* rest;    /* [N*V], optional */
+  const uint8_t* row_mask; /* [N*V], optional */
+  float temperature;
+  int dtype;            /* of logits and dlogits */
+  int values_dtype, index_dtype, mean;
+} devis_distill_params;
+size_t devis_distill_workspace_bytes(const devis_distill_params* p);
+size_t devis_distill_stats_bytes(const devis_distill_params* p);
+int devis_distill_fwd(const devis_distill_params* p, const void* logits, float* per_row, float* scal, void* stats,
+                      void* workspace, size_t workspace_bytes, void* stream);
+int devis_distill_bwd(const devis_distill_params* p, const void* logits, const void* stats, const float* scal,
+                      const float* grad, int grad_rows, void* dlogits, int64_t dN, int64_t dV, int64_t dK, void* stream);
+
+/* Drafted classes verified against a target model's probabilities, random numbers given.  Sequence b has
+ * n = lengths[b] (T without lengths; clamped to [0, T]) drafted classes tokens[b*T + t], the target's rows
+ * target[b*pB + t*pT + c*pK], t < Tp (Tp = T, or T + 1: a row behind the last draft), and optionally the drafter's rows
+ * draft[b*qB + t*qT + c*qK], t < T; both of `dtype`.  Draft t is accepted while
+ *   accept_u[b*T + t] * draft[b][t][token] < target[b][t][token]   (draft = NULL: accept_u < target),
+ * a token outside [0, K) never is.  With a = drafts accepted before the first that is not, one class is drawn from
+ *   a < n: max(target[b][a] - draft[b][a], 0), or target[b][a] if nothing is left (draft = NULL: target[b][a] without
+ *          the refused token);   a = n < Tp: target[b][n]
+ * as the first c whose cumulated weight exceeds sample_u[b] times the whole (all in fp64; weights that are not > 0
+ * count as 0).  out_tokens[b*Tp + t] = the accepted tokens, the drawn class, -1 behind them (-1 also for the drawn
+ * class if no class has weight); out_accepted[b] = a.  tokens, lengths and both outputs are of token_dtype
+ * (DEVIS_LABEL_I64 or DEVIS_LABEL_I32). */
+typedef struct devis_verify_params {
+  int64_t B, T, Tp, K;
+  int64_t pB, pT, pK, qB, qT, qK;
+  const void* tokens;
+  const float* accept_u;
+  const float* sample_u;
+  const void* lengths; /* optional */
+  int dtype, token_dtype;
+} devis_verify_params;
+int devis_verify_drafts(const devis_verify_params* p, const void* target, const void* draft, void* out_tokens,
+                        void* out_accepted, void* stream);
+
 /* ---------------------------------------------------------- attention gate -- */
 /* Attention_block of the 3-D attention U-Net (UNet3DZoo.py:69-100) behind its 1x1 convs W_g / W_x:
  *   a = relu(BN_g(g1) + BN_x(x1));  s = psi_conv(a) (one channel, fp32 [N][V]);  out = skip * sigmoid(BN_psi(s)).
