@@ -293,6 +293,191 @@ k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
   }
 }
 
+// ---- few classes: one thread a row, everything in registers, nothing kept for the backward.  Exponentials and logarithms
+// are fp32 here (fp64 ones would cost more than the memory at this many rows); a row's loss is put together from
+//   T (log p_j - log q_j) = (t_j - t_max) - (z_j - z_max) + T log(S_student / S_teacher),
+// where the large parts have cancelled before anything is rounded.  Sums over rows are fp64.
+__device__ __forceinline__ float log2_f(float x) { return __builtin_amdgcn_logf(x); }
+__device__ __forceinline__ float rcp_f(float x) { return __builtin_amdgcn_rcpf(x); }
+
+template <int KT>
+__device__ __forceinline__ float pick_class(const float (&x)[KT], int c) {
+  float v = x[0];
+#pragma unroll
+  for (int i = 1; i < KT; ++i) v = c == i ? x[i] : v;
+  return v;
+}
+
+template <int KT> struct FewRow {
+  float x[KT], e[KT];          // logits; exponentials, of a class in a slot against the row's maximum, else against m_rest
+  float a[KT], p[KT];          // slots: logit below the largest, share
+  int c[KT];
+  unsigned listed;
+  float m, sum, inv;           // student: maximum, sum of exponentials against it, 1 / sum
+  float sum_rest, to_m;        // classes in no slot: sum against m_rest, exp((m_rest - m)/T)
+  float d_rest, a_rest, p_rest;
+  float off;                   // log2(S_student / S_teacher), both against their own maxima
+};
+
+// -> state as SlotShared::state
+template <typename T, int KT, bool FULL, bool REST>
+__device__ __forceinline__ int few_row(const T* __restrict__ p, int64_t sK, int K, const Teacher& t, int64_t at, int64_t r,
+                                       float scale, double inv_t, FewRow<KT>& w) {
+  const int k = t.o.K;
+  load_row<T, KT, FULL>(p, sK, K, w.x);
+  float hi = neg_inf();
+  bool bad = false;
+  w.listed = 0;
+#pragma unroll
+  for (int j = 0; j < KT; ++j) {
+    w.a[j] = neg_inf();
+    w.c[j] = -1;
+    if (j < k) {
+      const int64_t i = at + j * t.o.sK;
+      w.a[j] = t.value_kind == DEVIS_F32 ? ((const float*)t.values)[i] : (float)((const bf16*)t.values)[i];
+      w.c[j] = class_at(t.indices, t.index_kind, i);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < KT; ++j) {
+    const bool filled = w.a[j] != neg_inf();
+    bad = bad || (filled && (unsigned)w.c[j] >= (unsigned)K);
+    w.c[j] = filled ? w.c[j] & (FEW_CLASSES - 1) : -1;
+    w.listed |= filled ? 1u << w.c[j] : 0u;
+    hi = fmaxf(hi, w.a[j]);
+  }
+  if (w.listed == 0) return 0;
+  if (bad) return 2;
+  // teacher, in base 2 against its largest logarithm
+  w.a_rest = neg_inf();
+  float shift = 0.f;
+  if constexpr (REST) {
+    w.a_rest = (float)(((double)t.rest[r] - (double)hi * inv_t) * 1.4426950408889634);
+    shift = fmaxf(w.a_rest, 0.f);
+    w.a_rest -= shift;
+  }
+  float sum_t = REST ? exp2_f(w.a_rest) : 0.f;
+  w.p_rest = sum_t;
+#pragma unroll
+  for (int j = 0; j < KT; ++j) {
+    w.a[j] -= hi;
+    w.p[j] = exp2_f(fmaf(w.a[j], scale, -shift));
+    sum_t += w.p[j];
+  }
+  const float inv_sum_t = rcp_f(sum_t);
+#pragma unroll
+  for (int j = 0; j < KT; ++j) w.p[j] *= inv_sum_t;
+  w.p_rest *= inv_sum_t;
+  // student
+  w.m = max_of(w.x);
+  const float m = w.m == neg_inf() ? 0.f : w.m;
+  if constexpr (REST) {
+    float m_rest = neg_inf();
+#pragma unroll
+    for (int c = 0; c < KT; ++c) m_rest = fmaxf(m_rest, (w.listed >> c) & 1u ? neg_inf() : w.x[c]);
+    w.d_rest = m_rest == neg_inf() ? 0.f : (m_rest - m) * scale;
+    const float ref = m_rest == neg_inf() ? 0.f : m_rest;
+    w.to_m = exp2_f(w.d_rest);
+    float in = 0.f;
+    w.sum_rest = 0.f;
+#pragma unroll
+    for (int c = 0; c < KT; ++c) {
+      const bool l = (w.listed >> c) & 1u;
+      w.e[c] = exp2_f((w.x[c] - (l ? m : ref)) * scale);
+      in += l ? w.e[c] : 0.f;
+      w.sum_rest += l ? 0.f : w.e[c];
+    }
+    w.sum = fmaf(w.sum_rest, w.to_m, in);
+  } else {
+#pragma unroll
+    for (int c = 0; c < KT; ++c) w.e[c] = exp2_f((w.x[c] - m) * scale);
+    w.sum = sum_of(w.e);
+  }
+  w.inv = w.sum == 0.f ? 0.f : rcp_f(w.sum);
+  w.off = log2_f(w.sum * inv_sum_t) - shift;
+  w.a_rest += shift;
+  w.m = m;
+  return 1;
+}
+
+template <typename T, int KT, bool FULL, bool REST>
+__global__ void __launch_bounds__(256)
+k_distill_few_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
+                  float* __restrict__ per_row, double* __restrict__ partial) {
+  __shared__ double s_red[4];
+  const float unit = temperature * 0.6931471805599453f;              // of the logarithms to base 2
+  double loss_sum = 0., count = 0.;
+  for (int64_t n = blockIdx.y; n < s.N; n += gridDim.y) {
+    for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < s.V; v += (int64_t)gridDim.x * 256) {
+      const int64_t r = n * s.V + v;
+      FewRow<KT> w;
+      const int state = row_masked(t, r) ? 0 : few_row<T, KT, FULL, REST>(z + n * s.sN + v * s.sV, s.sK, s.K, t,
+                                                                         n * t.o.sN + v * t.o.sV, r, scale, inv_t, w);
+      float loss = 0.f;
+      if (state == 1) {
+#pragma unroll
+        for (int j = 0; j < KT; ++j) {
+          const float x = pick_class(w.x, w.c[j]);
+          const float d = x == neg_inf() ? __builtin_inff() : fmaf(w.off, unit, w.a[j] - (x - w.m));
+          loss += w.p[j] == 0.f ? 0.f : w.p[j] * d;
+        }
+        if constexpr (REST) {
+          const float d = w.sum_rest == 0.f ? __builtin_inff() : unit * ((w.a_rest - w.d_rest) + (w.off - log2_f(w.sum_rest)));
+          loss += w.p_rest == 0.f ? 0.f : w.p_rest * d;
+        }
+        loss *= temperature;                   // the terms are T (log p - log q)
+      } else if (state == 2) {
+        loss = __builtin_nanf("");
+      }
+      if (per_row) per_row[r] = loss;
+      loss_sum += (double)loss;
+      count += state ? 1. : 0.;
+    }
+  }
+  if (partial) {
+    loss_sum = block_sum<256>(loss_sum, s_red);
+    count = block_sum<256>(count, s_red);
+    if (threadIdx.x == 0) {
+      const int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+      partial[2 * b] = loss_sum;
+      partial[2 * b + 1] = count;
+    }
+  }
+}
+
+template <typename T, int KT, bool FULL, bool REST>
+__global__ void __launch_bounds__(256)
+k_distill_few_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
+                  const float* __restrict__ scal, const float* __restrict__ grad, int grad_rows, T* __restrict__ dz, RowShape d) {
+  const float g_all = grad_rows ? 0.f : grad[0] * scal[1];
+  for (int64_t n = blockIdx.y; n < s.N; n += gridDim.y) {
+    for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < s.V; v += (int64_t)gridDim.x * 256) {
+      const int64_t r = n * s.V + v;
+      FewRow<KT> w;
+      const int state = row_masked(t, r) ? 0 : few_row<T, KT, FULL, REST>(z + n * s.sN + v * s.sV, s.sK, s.K, t,
+                                                                         n * t.o.sN + v * t.o.sV, r, scale, inv_t, w);
+      const float f = temperature * (grad_rows ? grad[r] : g_all);
+      float out[KT];
+      if (state == 1) {
+        const float w_rest = REST && w.sum_rest != 0.f ? w.to_m * w.inv - w.p_rest * rcp_f(w.sum_rest) : 0.f;
+#pragma unroll
+        for (int c = 0; c < KT; ++c) {
+          float share = 0.f;
+#pragma unroll
+          for (int j = 0; j < KT; ++j) share += w.c[j] == c ? w.p[j] : 0.f;
+          const bool l = !REST || ((w.listed >> c) & 1u);
+          out[c] = f * (l ? fmaf(w.e[c], w.inv, -share) : w.e[c] * w_rest);
+        }
+      } else {
+        const float fill = state ? __builtin_nanf("") : 0.f;
+#pragma unroll
+        for (int c = 0; c < KT; ++c) out[c] = fill;
+      }
+      store_row<T, KT, FULL>(dz + n * d.sN + v * d.sV, d.sK, s.K, out);
+    }
+  }
+}
+
 static int distill_blocks(int64_t NV) { return (int)(NV < DIS_MAX_BLOCKS ? NV : DIS_MAX_BLOCKS); }
 
 static bool distill_args_ok(const devis_distill_params* a, const void* logits) {
@@ -307,6 +492,12 @@ static bool distill_args_ok(const devis_distill_params* a, const void* logits) {
 }  // namespace devis
 
 using namespace devis;
+
+#define DISTILL_DISPATCH_FEW(unit, KERNEL_REST, KERNEL)                                                          \
+  DEVIS_DISPATCH_DTYPE(a->dtype, {                                                                                \
+    if (a->rest) DEVIS_DISPATCH_FEW(a->K, unit, KERNEL_REST);                                                     \
+    else DEVIS_DISPATCH_FEW(a->K, unit, KERNEL);                                                                  \
+  })
 
 #define DISTILL_DISPATCH(KERNEL, ...)                                                                             \
   DEVIS_DISPATCH_DTYPE(a->dtype, {                                                                                \
@@ -326,22 +517,35 @@ size_t devis_distill_workspace_bytes(const devis_distill_params* a) {
 }
 
 size_t devis_distill_stats_bytes(const devis_distill_params* a) {
-  return a && a->N > 0 && a->V > 0 ? (size_t)a->N * (size_t)a->V * sizeof(RowStats) : 0;
+  return a && a->N > 0 && a->V > 0 && a->K > FEW_CLASSES ? (size_t)a->N * (size_t)a->V * sizeof(RowStats) : 0;
 }
 
 int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* per_row, float* scal, void* stats, void* ws,
                       size_t ws_bytes, void* stream) {
   if (!distill_args_ok(a, logits) || (!per_row && !scal) || (scal && !ws)) return DEVIS_ERR_BAD_ARG;
   if (scal && ws_bytes < devis_distill_workspace_bytes(a)) return DEVIS_ERR_WORKSPACE;
-  const RowShape s = {a->sN, a->sV, a->sK, a->N, a->V, (int)a->K};
-  const Teacher t = {a->values, a->indices, a->rest, a->row_mask, {a->oN, a->oV, a->oK, a->N, a->V, (int)a->k}, a->values_dtype, a->index_dtype};
+  RowShape s = {a->sN, a->sV, a->sK, a->N, a->V, (int)a->K};
+  Teacher t = {a->values, a->indices, a->rest, a->row_mask, {a->oN, a->oV, a->oK, a->N, a->V, (int)a->k}, a->values_dtype, a->index_dtype};
   const double inv_t = 1.0 / (double)a->temperature, t2 = (double)a->temperature * (double)a->temperature;
   const float scale = (float)(1.4426950408889634 * inv_t);
   const bool unit = a->sK == 1;
-  const int blocks = distill_blocks(a->N * a->V);
+  int blocks = distill_blocks(a->N * a->V);
   double* part = scal ? (double*)ws : nullptr;
+  if (a->K <= FEW_CLASSES) {
+    if (one_stride(s) && one_stride(t.o)) { merge_rows(s); merge_rows(t.o); }
+    const dim3 grid = few_grid(s.N, s.V, DIS_MAX_BLOCKS);
+    blocks = (int)(grid.x * grid.y);
+#define LAUNCH_FEW(REST, KT, FULL) hipLaunchKernelGGL((k_distill_few_fwd<T, KT, FULL, REST>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, per_row, part)
+#define LAUNCH_FEW_REST(KT, FULL) LAUNCH_FEW(true, KT, FULL)
+#define LAUNCH_FEW_TOP(KT, FULL) LAUNCH_FEW(false, KT, FULL)
+    DISTILL_DISPATCH_FEW(unit, LAUNCH_FEW_REST, LAUNCH_FEW_TOP);
+#undef LAUNCH_FEW_TOP
+#undef LAUNCH_FEW_REST
+#undef LAUNCH_FEW
+  } else {
 #define LAUNCH_DISTILL_FWD(UNIT, REST, BS) hipLaunchKernelGGL((k_distill_fwd<T, UNIT, REST, BS>), dim3(blocks), dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, t2, (RowStats*)stats, per_row, part)
-  DISTILL_DISPATCH(LAUNCH_DISTILL_FWD);
+    DISTILL_DISPATCH(LAUNCH_DISTILL_FWD);
+  }
 #undef LAUNCH_DISTILL_FWD
   const int rc = launch_status();
   if (rc || !scal) return rc;
@@ -351,13 +555,25 @@ int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* 
 
 int devis_distill_bwd(const devis_distill_params* a, const void* logits, const void* stats, const float* scal, const float* grad,
                       int grad_rows, void* dlogits, int64_t dN, int64_t dV, int64_t dK, void* stream) {
-  if (!distill_args_ok(a, logits) || !stats || !grad || !dlogits || (!grad_rows && !scal)) return DEVIS_ERR_BAD_ARG;
+  if (!distill_args_ok(a, logits) || (!stats && a->K > FEW_CLASSES) || !grad || !dlogits || (!grad_rows && !scal)) return DEVIS_ERR_BAD_ARG;
   if (!rows_ok(dN, dV, dK, a->N, a->V, a->K)) return DEVIS_ERR_BAD_ARG;
-  const RowShape s = {a->sN, a->sV, a->sK, a->N, a->V, (int)a->K}, d = {dN, dV, dK, a->N, a->V, (int)a->K};
-  const Teacher t = {a->values, a->indices, a->rest, a->row_mask, {a->oN, a->oV, a->oK, a->N, a->V, (int)a->k}, a->values_dtype, a->index_dtype};
+  RowShape s = {a->sN, a->sV, a->sK, a->N, a->V, (int)a->K}, d = {dN, dV, dK, a->N, a->V, (int)a->K};
+  Teacher t = {a->values, a->indices, a->rest, a->row_mask, {a->oN, a->oV, a->oK, a->N, a->V, (int)a->k}, a->values_dtype, a->index_dtype};
   const double inv_t = 1.0 / (double)a->temperature;
   const float scale = (float)(1.4426950408889634 * inv_t);
   const bool unit = a->sK == 1 && dK == 1;
+  if (a->K <= FEW_CLASSES) {
+    if (one_stride(s) && one_stride(t.o) && one_stride(d)) { merge_rows(s); merge_rows(t.o); merge_rows(d); }
+    const dim3 grid = few_grid(s.N, s.V, 8192);
+#define LAUNCH_FEW(REST, KT, FULL) hipLaunchKernelGGL((k_distill_few_bwd<T, KT, FULL, REST>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, scal, grad, grad_rows, (T*)dlogits, d)
+#define LAUNCH_FEW_REST(KT, FULL) LAUNCH_FEW(true, KT, FULL)
+#define LAUNCH_FEW_TOP(KT, FULL) LAUNCH_FEW(false, KT, FULL)
+    DISTILL_DISPATCH_FEW(unit, LAUNCH_FEW_REST, LAUNCH_FEW_TOP);
+#undef LAUNCH_FEW_TOP
+#undef LAUNCH_FEW_REST
+#undef LAUNCH_FEW
+    return launch_status();
+  }
   const int blocks = distill_blocks(a->N * a->V);
 #define LAUNCH_DISTILL_BWD(UNIT, REST, BS) hipLaunchKernelGGL((k_distill_bwd<T, UNIT, REST, BS>), dim3(blocks), dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, (const RowStats*)stats, scal, grad, grad_rows, (T*)dlogits, d)
   DISTILL_DISPATCH(LAUNCH_DISTILL_BWD);

@@ -136,6 +136,53 @@ template <int BS> __device__ __forceinline__ double block_sum(double v, double* 
   return v;
 }
 
+// ---- few classes: a thread takes a whole row into registers.  KT = 2, 4, 8 or 16 bounds K; FULL: K = KT adjacent
+// classes, one load of the whole row.
+constexpr int FEW_CLASSES = 16;
+
+template <typename T, int KT, bool FULL>
+__device__ __forceinline__ void load_row(const T* __restrict__ p, int64_t sK, int K, float (&x)[KT]) {
+  if constexpr (FULL) {
+    T raw[KT];
+    __builtin_memcpy(raw, p, sizeof raw);
+#pragma unroll
+    for (int c = 0; c < KT; ++c) x[c] = (float)raw[c];
+  } else {
+#pragma unroll
+    for (int c = 0; c < KT; ++c) x[c] = c < K ? (float)p[(int64_t)c * sK] : neg_inf();
+  }
+}
+template <typename T, int KT, bool FULL>
+__device__ __forceinline__ void store_row(T* __restrict__ p, int64_t sK, int K, const float (&x)[KT]) {
+  if constexpr (FULL) {
+    T raw[KT];
+#pragma unroll
+    for (int c = 0; c < KT; ++c) raw[c] = (T)x[c];
+    __builtin_memcpy(p, raw, sizeof raw);
+  } else {
+#pragma unroll
+    for (int c = 0; c < KT; ++c) if (c < K) p[(int64_t)c * sK] = (T)x[c];
+  }
+}
+
+// rows of several shapes walked together as (n, v): one long v where every shape allows it
+inline bool one_stride(const RowShape& s) { return s.N == 1 || s.V == 1 || s.sN == s.V * s.sV; }
+inline void merge_rows(RowShape& s) {
+  s.sV = s.V == 1 ? s.sN : s.sV;
+  s.V *= s.N;
+  s.N = 1;
+  s.sN = 0;
+}
+inline dim3 few_grid(int64_t N, int64_t V, int most) {
+  int64_t bx = cdiv(V, 256), by = N;
+  if (bx > most) bx = most;
+  const int64_t room = most / bx;
+  if (by > room) by = room;
+  return dim3((unsigned)bx, (unsigned)by);
+}
+
+#define DEVIS_DISPATCH_FEW(K, unit, LAUNCH)                                                 do {                                                                                        if ((K) <= 2) { if ((unit) && (K) == 2) LAUNCH(2, true); else LAUNCH(2, false); }         else if ((K) <= 4) { if ((unit) && (K) == 4) LAUNCH(4, true); else LAUNCH(4, false); }     else if ((K) <= 8) { if ((unit) && (K) == 8) LAUNCH(8, true); else LAUNCH(8, false); }     else { if ((unit) && (K) == 16) LAUNCH(16, true); else LAUNCH(16, false); }             } while (0)
+
 inline bool rows_ok(int64_t sN, int64_t sV, int64_t sK, int64_t N, int64_t V, int64_t K) {
   return N > 0 && V > 0 && K > 0 && K < 0x7fffffff && sN >= 0 && sV >= 0 && sK > 0 && N <= INT64_MAX / V;
 }

@@ -174,6 +174,53 @@ k_top_rows(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t
   }
 }
 
+// few classes: one thread a row.  Slot by slot the largest value left, the lowest class first (strict comparison).
+template <typename T, typename I, int KT, bool FULL>
+__global__ void __launch_bounds__(256)
+k_top_few(const T* __restrict__ z, RowShape s, int k, float scale, float inv_t, T* __restrict__ values, I* __restrict__ indices,
+          RowShape o, float* __restrict__ rest) {
+  for (int64_t n = blockIdx.y; n < s.N; n += gridDim.y) {
+    for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < s.V; v += (int64_t)gridDim.x * 256) {
+      float x[KT];
+      load_row<T, KT, FULL>(z + n * s.sN + v * s.sV, s.sK, s.K, x);
+      uint32_t key[KT];                      // ordered integer of the value; 0: taken, or no class
+#pragma unroll
+      for (int c = 0; c < KT; ++c) key[c] = FULL || c < s.K ? (uint32_t)(top_key(nan_high(x[c]), 0) >> 32) : 0;
+      const int64_t at = n * o.sN + v * o.sV;
+      for (int j = 0; j < k; ++j) {
+        uint32_t best = 0;
+        int bc = 0;
+        float bx = 0.f;
+#pragma unroll
+        for (int c = 0; c < KT; ++c) {
+          const bool more = key[c] > best;
+          best = more ? key[c] : best;
+          bc = more ? c : bc;
+          bx = more ? x[c] : bx;
+        }
+#pragma unroll
+        for (int c = 0; c < KT; ++c) key[c] = c == bc ? 0 : key[c];
+        values[at + j * o.sK] = (T)bx;
+        indices[at + j * o.sK] = (I)bc;
+      }
+      if (rest) {
+        float m = neg_inf();
+#pragma unroll
+        for (int c = 0; c < KT; ++c) {
+          x[c] = key[c] ? nan_high(x[c]) : neg_inf();
+          m = fmaxf(m, x[c]);
+        }
+        const float ref = fabsf(m) < __builtin_inff() ? m : 0.f;
+        float e[KT];
+#pragma unroll
+        for (int c = 0; c < KT; ++c) e[c] = exp2_f((x[c] - ref) * scale);
+        // m is -inf (nothing left) or +inf: it is the answer
+        rest[n * s.V + v] = ref == m ? fmaf(m, inv_t, __logf(sum_of(e))) : m;
+      }
+    }
+  }
+}
+
 }  // namespace devis
 
 using namespace devis;
@@ -184,11 +231,22 @@ extern "C" int devis_top_logits(const void* logits, int64_t sN, int64_t sV, int6
   if (!logits || !values || !indices || !rows_ok(sN, sV, sK, N, V, K) || !rows_ok(oN, oV, oK, N, V, K)) return DEVIS_ERR_BAD_ARG;
   if (k < 1 || k > K || k > TOP_MAX_K || !(temperature > 0x1p-100f) || !(temperature < 0x1p100f)) return DEVIS_ERR_BAD_ARG;
   if (index_dtype != DEVIS_LABEL_I32 && !(index_dtype == DEVIS_LABEL_U8 && K <= 256)) return DEVIS_ERR_BAD_ARG;
-  const RowShape s = {sN, sV, sK, N, V, (int)K}, o = {oN, oV, oK, N, V, (int)k};
+  RowShape s = {sN, sV, sK, N, V, (int)K}, o = {oN, oV, oK, N, V, (int)k};
   const int64_t NV = N * V;
   const double inv_t = 1.0 / (double)temperature;
   const float scale = (float)(1.4426950408889634 * inv_t);
   const hipStream_t st = (hipStream_t)stream;
+  if (K <= FEW_CLASSES) {
+    if (one_stride(s) && one_stride(o)) { merge_rows(s); merge_rows(o); }
+    const dim3 grid = few_grid(s.N, s.V, 8192);
+#define LAUNCH_FEW(KT, FULL) hipLaunchKernelGGL((k_top_few<T, I, KT, FULL>), grid, dim3(256), 0, st, (const T*)logits, s, (int)k, scale, (float)inv_t, (T*)values, (I*)indices, o, rest)
+    DEVIS_DISPATCH_DTYPE(dtype, {
+      if (index_dtype == DEVIS_LABEL_U8) { typedef uint8_t I; DEVIS_DISPATCH_FEW(K, sK == 1, LAUNCH_FEW); }
+      else { typedef int32_t I; DEVIS_DISPATCH_FEW(K, sK == 1, LAUNCH_FEW); }
+    });
+#undef LAUNCH_FEW
+    return launch_status();
+  }
   const unsigned blocks = (unsigned)(NV < (1 << 20) ? NV : (1 << 20));
 #define LAUNCH_TOP(I, UNIT, BS) hipLaunchKernelGGL((k_top_rows<T, I, UNIT, BS>), dim3(blocks), dim3(BS), 0, st, (const T*)logits, s, (int)k, scale, inv_t, (T*)values, (I*)indices, o, rest)
 #define LAUNCH_TOP_U(I, BS) do { if (sK == 1) LAUNCH_TOP(I, true, BS); else LAUNCH_TOP(I, false, BS); } while (0)

@@ -172,6 +172,69 @@ k_verify(const T* __restrict__ p, const T* __restrict__ q, VerifyArgs a) {
   }
 }
 
+// few classes: one thread a sequence.  The rows of each place are loaded whole (they share the cache line that the drafted
+// class's own probability is in), so a refused draft is drawn again from registers.
+template <typename T, int KT, bool FULL, bool DRAFTER>
+__global__ void __launch_bounds__(256)
+k_verify_few(const T* __restrict__ p, const T* __restrict__ q, VerifyArgs a) {
+  for (int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x; b < a.B; b += (int64_t)gridDim.x * 256) {
+    const int len = draft_length(a, b);
+    int n = 0, drawn = -1;
+    for (;; ++n) {
+      if (n >= a.Tp) break;                    // all accepted and no row behind them
+      float x[KT], y[KT] = {};
+      load_row<T, KT, FULL>(p + b * a.pB + n * a.pT, a.pK, a.K, x);
+      const bool drafted = n < len;
+      int64_t tok = -1;
+      if (drafted) {
+        tok = int_at(a.tokens, a.token_kind, b * a.T + n);
+        double u = (double)a.accept_u[b * a.T + n];
+        float pd = 0.f, qd = 0.f;
+        if (DRAFTER) load_row<T, KT, FULL>(q + b * a.qB + n * a.qT, a.qK, a.K, y);
+#pragma unroll
+        for (int c = 0; c < KT; ++c) {
+          pd = tok == c ? x[c] : pd;
+          if (DRAFTER) qd = tok == c ? y[c] : qd;
+        }
+        if (DRAFTER) u *= (double)qd;
+        if (tok >= 0 && tok < a.K && u < (double)pd) {
+          put_int(a.out_tokens, a.token_kind, b * a.Tp + n, tok);
+          continue;
+        }
+      }
+      double w[KT], total = 0.;
+#pragma unroll
+      for (int c = 0; c < KT; ++c) {
+        double v = (double)x[c];
+        if (DRAFTER) v = drafted ? v - (double)y[c] : v;
+        else v = drafted && tok == c ? 0. : v;
+        w[c] = (FULL || c < a.K) && v > 0. ? v : 0.;
+        total += w[c];
+      }
+      if (!(total > 0.)) {
+        total = 0.;
+#pragma unroll
+        for (int c = 0; c < KT; ++c) {
+          w[c] = (FULL || c < a.K) && x[c] > 0.f ? (double)x[c] : 0.;
+          total += w[c];
+        }
+      }
+      const double goal = (double)a.sample_u[b] * total;
+      double run = 0.;
+      bool open = true;
+#pragma unroll
+      for (int c = 0; c < KT; ++c) {
+        run += w[c];
+        drawn = open && w[c] > 0. ? c : drawn;               // the last with weight so far
+        open = open && !(w[c] > 0. && run > goal);
+      }
+      break;
+    }
+    for (int t = n; t < a.Tp; ++t) put_int(a.out_tokens, a.token_kind, b * a.Tp + t, t == n ? drawn : -1);
+    put_int(a.out_accepted, a.token_kind, b, n);
+  }
+}
+
 }  // namespace devis
 
 using namespace devis;
@@ -184,6 +247,21 @@ extern "C" int devis_verify_drafts(const devis_verify_params* v, const void* tar
   if (v->token_dtype != DEVIS_LABEL_I64 && v->token_dtype != DEVIS_LABEL_I32) return DEVIS_ERR_BAD_ARG;
   const VerifyArgs a = {v->tokens, v->accept_u, v->sample_u, v->lengths, out_tokens, out_accepted, v->B, (int)v->T, (int)v->Tp,
                         (int)v->K, v->pB, v->pT, v->pK, v->qB, v->qT, v->qK, v->token_dtype};
+  if (v->K <= FEW_CLASSES) {
+    const dim3 grid = few_grid(1, v->B, 8192);
+    const bool unit = v->pK == 1 && (!draft || v->qK == 1);
+#define LAUNCH_FEW(DRAFTER, KT, FULL) hipLaunchKernelGGL((k_verify_few<T, KT, FULL, DRAFTER>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)target, (const T*)draft, a)
+#define LAUNCH_FEW_DRAFTER(KT, FULL) LAUNCH_FEW(true, KT, FULL)
+#define LAUNCH_FEW_ALONE(KT, FULL) LAUNCH_FEW(false, KT, FULL)
+    DEVIS_DISPATCH_DTYPE(v->dtype, {
+      if (draft) DEVIS_DISPATCH_FEW(v->K, unit, LAUNCH_FEW_DRAFTER);
+      else DEVIS_DISPATCH_FEW(v->K, unit, LAUNCH_FEW_ALONE);
+    });
+#undef LAUNCH_FEW_ALONE
+#undef LAUNCH_FEW_DRAFTER
+#undef LAUNCH_FEW
+    return launch_status();
+  }
   const unsigned blocks = (unsigned)(v->B < (1 << 20) ? v->B : (1 << 20));
   DEVIS_DISPATCH_DTYPE(v->dtype, hipLaunchKernelGGL(k_verify<T>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, (const T*)target, (const T*)draft, a));
   return launch_status();
