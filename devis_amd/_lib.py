@@ -138,7 +138,7 @@ SIGNATURES = {
     "devis_top_logits": (_I, [_P, _I64, _I64, _I64, _I, _I64, _I64, _I64, _I64, _F, _P, _P, _I, _I64, _I64, _I64, _P, _P]),
     "devis_distill_workspace_bytes": (_SZ, [_DP]),
     "devis_distill_stats_bytes": (_SZ, [_DP]),
-    "devis_distill_fwd": (_I, [_DP, _P, _P, _P, _P, _P, _SZ, _P]),
+    "devis_distill_fwd": (_I, [_DP, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "devis_distill_bwd": (_I, [_DP, _P, _P, _P, _P, _I, _P, _I64, _I64, _I64, _P]),
     "devis_verify_drafts": (_I, [_VP, _P, _P, _P, _P, _P]),
     "devis_att_chunks": (_I64, [_I64]),

@@ -178,11 +178,12 @@ class _DistillFn(torch.autograd.Function):
             ctx.like = logits.shape, logits.dtype, dev
             return torch.zeros(shape if rows else (), dtype=torch.float32, device=dev)
         need = grad_on and ctx.needs_input_grad[0]
-        per_row, scal, stats = ops.distill_fwd(params, dev, shape, ts[0], rows, not rows, need)
-        ctx.save_for_backward(*ts, stats, scal)
-        ctx.params, ctx.channels_last, ctx.rows = params, channels_last, rows
-        ctx.at = tuple(None if t is None else (t.data_ptr(), t.stride()) for t in ts)
-        return per_row if rows else scal[0].clone()
+        loss, scratch = ops.distill_fwd(params, dev, shape, ts[0], rows, need)
+        if need:
+            ctx.save_for_backward(*ts, scratch)
+            ctx.params, ctx.channels_last, ctx.rows = params, channels_last, rows
+            ctx.at = tuple(None if t is None else (t.data_ptr(), t.stride()) for t in ts)
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -190,13 +191,13 @@ class _DistillFn(torch.autograd.Function):
         if ctx.empty:
             shape, dtype, dev = ctx.like
             return (torch.zeros(shape, dtype=dtype, device=dev),) + (None,) * 8
-        *ts, stats, scal = ctx.saved_tensors
+        *ts, scratch = ctx.saved_tensors
         x, params = ts[0], ctx.params
         if tuple(None if t is None else (t.data_ptr(), t.stride()) for t in ts) != ctx.at:      # moved by saved-tensor hooks
             params, _, _, ts = ops.distill_params(*ts, ctx.channels_last, params.temperature, params.mean)
             x = ts[0]
         g = g.contiguous().float()
-        return (ops.distill_bwd(params, x.device, x, ctx.channels_last, stats, scal, g, ctx.rows),) + (None,) * 8
+        return (ops.distill_bwd(params, x.device, x, ctx.channels_last, scratch, g, ctx.rows),) + (None,) * 8
 
 
 def distill_top_loss(logits: Tensor, values: Tensor, indices: Tensor, rest: Optional[Tensor] = None, channels_last: bool = True,

@@ -228,9 +228,9 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
   }
 }
 
-// scal[0] = sum or mean of the counted rows' losses, scal[1] = what a row's gradient is multiplied by, scal[2] = rows counted
+// the sum or mean of the counted rows' losses; scal = what a row's gradient is multiplied by, and the rows counted
 __global__ void __launch_bounds__(256)
-k_distill_finalize(const double* __restrict__ partial, int n, int mean, float* __restrict__ scal) {
+k_distill_finalize(const double* __restrict__ partial, int n, int mean, float* __restrict__ out, float* __restrict__ scal) {
   __shared__ double s_red[4];
   double loss = 0., count = 0.;
   for (int i = threadIdx.x; i < n; i += 256) { loss += partial[2 * i]; count += partial[2 * i + 1]; }
@@ -238,9 +238,9 @@ k_distill_finalize(const double* __restrict__ partial, int n, int mean, float* _
   count = block_sum<256>(count, s_red);
   if (threadIdx.x == 0) {
     const double f = mean ? 1. / (count > 0. ? count : 1.) : 1.;
-    scal[0] = (float)(loss * f);
-    scal[1] = (float)f;
-    scal[2] = (float)count;
+    out[0] = (float)(loss * f);
+    scal[0] = (float)f;
+    scal[1] = (float)count;
   }
 }
 
@@ -264,7 +264,7 @@ k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
     }
     __syncthreads();
     const bool live = sh.state != 0;
-    const float g = grad_rows ? grad[r] : grad[0] * scal[1];
+    const float g = grad_rows ? grad[r] : grad[0] * scal[0];
     const float f = g * temperature;
     RowStats st = {0.f, 0.f, 0.f, 0.f};
     if (live) st = stats[r];
@@ -449,7 +449,7 @@ template <typename T, int KT, bool FULL, bool REST>
 __global__ void __launch_bounds__(256)
 k_distill_few_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
                   const float* __restrict__ scal, const float* __restrict__ grad, int grad_rows, T* __restrict__ dz, RowShape d) {
-  const float g_all = grad_rows ? 0.f : grad[0] * scal[1];
+  const float g_all = grad_rows ? 0.f : grad[0] * scal[0];
   for (int64_t n = blockIdx.y; n < s.N; n += gridDim.y) {
     for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < s.V; v += (int64_t)gridDim.x * 256) {
       const int64_t r = n * s.V + v;
@@ -520,17 +520,17 @@ size_t devis_distill_stats_bytes(const devis_distill_params* a) {
   return a && a->N > 0 && a->V > 0 && a->K > FEW_CLASSES ? (size_t)a->N * (size_t)a->V * sizeof(RowStats) : 0;
 }
 
-int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* per_row, float* scal, void* stats, void* ws,
-                      size_t ws_bytes, void* stream) {
-  if (!distill_args_ok(a, logits) || (!per_row && !scal) || (scal && !ws)) return DEVIS_ERR_BAD_ARG;
-  if (scal && ws_bytes < devis_distill_workspace_bytes(a)) return DEVIS_ERR_WORKSPACE;
+int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* per_row, float* loss, float* scal, void* stats,
+                      void* ws, size_t ws_bytes, void* stream) {
+  if (!distill_args_ok(a, logits) || (!per_row && !loss) || (loss && (!ws || !scal))) return DEVIS_ERR_BAD_ARG;
+  if (loss && ws_bytes < devis_distill_workspace_bytes(a)) return DEVIS_ERR_WORKSPACE;
   RowShape s = {a->sN, a->sV, a->sK, a->N, a->V, (int)a->K};
   Teacher t = {a->values, a->indices, a->rest, a->row_mask, {a->oN, a->oV, a->oK, a->N, a->V, (int)a->k}, a->values_dtype, a->index_dtype};
   const double inv_t = 1.0 / (double)a->temperature, t2 = (double)a->temperature * (double)a->temperature;
   const float scale = (float)(1.4426950408889634 * inv_t);
   const bool unit = a->sK == 1;
   int blocks = distill_blocks(a->N * a->V);
-  double* part = scal ? (double*)ws : nullptr;
+  double* part = loss ? (double*)ws : nullptr;
   if (a->K <= FEW_CLASSES) {
     if (one_stride(s) && one_stride(t.o)) { merge_rows(s); merge_rows(t.o); }
     const dim3 grid = few_grid(s.N, s.V, DIS_MAX_BLOCKS);
@@ -548,8 +548,8 @@ int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* 
   }
 #undef LAUNCH_DISTILL_FWD
   const int rc = launch_status();
-  if (rc || !scal) return rc;
-  hipLaunchKernelGGL(k_distill_finalize, dim3(1), dim3(256), 0, (hipStream_t)stream, (const double*)ws, blocks, a->mean, scal);
+  if (rc || !loss) return rc;
+  hipLaunchKernelGGL(k_distill_finalize, dim3(1), dim3(256), 0, (hipStream_t)stream, (const double*)ws, blocks, a->mean, loss, scal);
   return launch_status();
 }
 

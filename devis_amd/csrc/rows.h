@@ -6,6 +6,8 @@
 
 namespace devis {
 
+constexpr int64_t MAX_CLASSES = (int64_t)1 << 30;      // class numbers, and a step past them, stay below 2^31
+
 struct RowShape { int64_t sN, sV, sK, N, V; int K; };
 
 __device__ __forceinline__ int64_t row_offset(const RowShape& s, int64_t r) {
@@ -184,7 +186,7 @@ inline dim3 few_grid(int64_t N, int64_t V, int most) {
 #define DEVIS_DISPATCH_FEW(K, unit, LAUNCH)                                                 do {                                                                                        if ((K) <= 2) { if ((unit) && (K) == 2) LAUNCH(2, true); else LAUNCH(2, false); }         else if ((K) <= 4) { if ((unit) && (K) == 4) LAUNCH(4, true); else LAUNCH(4, false); }     else if ((K) <= 8) { if ((unit) && (K) == 8) LAUNCH(8, true); else LAUNCH(8, false); }     else { if ((unit) && (K) == 16) LAUNCH(16, true); else LAUNCH(16, false); }             } while (0)
 
 inline bool rows_ok(int64_t sN, int64_t sV, int64_t sK, int64_t N, int64_t V, int64_t K) {
-  return N > 0 && V > 0 && K > 0 && K < 0x7fffffff && sN >= 0 && sV >= 0 && sK > 0 && N <= INT64_MAX / V;
+  return N > 0 && V > 0 && K > 0 && K <= MAX_CLASSES && sN >= 0 && sV >= 0 && sK > 0 && N <= INT64_MAX / V;
 }
 
 }  // namespace devis

@@ -14,8 +14,6 @@
 
 namespace devis {
 
-constexpr int VER_SEGS = 64;                  // segments of a row whose weights are summed apart
-
 struct VerifyArgs {
   const void* tokens; const float* accept_u; const float* sample_u; const void* lengths;
   void* out_tokens; void* out_accepted;
@@ -48,29 +46,80 @@ __device__ __forceinline__ bool draft_ok(const VerifyArgs& a, const T* p, const 
   return u < pd;
 }
 
-// the weights of one sequence's draw
+// what one sequence's class is drawn from
 template <typename T> struct Draw {
   const T* p; const T* q;                     // q null: the target's row alone
   int64_t pK, qK;
   int skip;                                   // class taken out, -1 none
-  __device__ __forceinline__ double whole(int c) const {
-    const double x = (double)(float)p[(int64_t)c * pK];
-    return x > 0. ? x : 0.;
-  }
-  __device__ __forceinline__ double weight(int c) const {
-    double x = (double)(float)p[(int64_t)c * pK];
-    if (q) x -= (double)(float)q[(int64_t)c * qK];
-    return x > 0. && c != skip ? x : 0.;
-  }
 };
+__device__ __forceinline__ double weight_of(float x, float y, bool keep) {
+  const double w = (double)x - (double)y;
+  return w > 0. && keep ? w : 0.;
+}
 
-template <typename T>
-__global__ void __launch_bounds__(256)
+// f(w, c): the weights of classes c, c + 1, .. of [lo, hi), dealt vector by vector to `stride` threads of which this is
+// number `me`; four vectors of each model in flight.
+template <typename T, bool UNIT, bool DRAFTER, typename F>
+__device__ __forceinline__ void each_weight(const Draw<T>& d, int lo, int hi, int me, int stride, F f) {
+  const auto one = [&](int c) {
+    double w[1] = {weight_of((float)d.p[(int64_t)c * (UNIT ? 1 : d.pK)], DRAFTER && d.q ? (float)d.q[(int64_t)c * (UNIT ? 1 : d.qK)] : 0.f, c != d.skip)};
+    f(w, c);
+  };
+  if constexpr (UNIT) {
+    constexpr int VEC = vec_of<T>();
+    const int full = (hi - lo) / VEC;
+    const bool two = DRAFTER && d.q;
+    const auto vec = [&](const Raw16& rp, const Raw16& rq, int c) {
+      float x[VEC], y[VEC];
+      unpack(rp, x);
+      unpack(rq, y);
+      double w[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) w[i] = weight_of(x[i], y[i], c + i != d.skip);
+      f(w, c);
+    };
+    int v = me;
+    for (; v + 3 * stride < full; v += 4 * stride) {
+      Raw16 rp[4], rq[4] = {};
+#pragma unroll
+      for (int u = 0; u < 4; ++u) rp[u] = load16(d.p + lo + (int64_t)(v + u * stride) * VEC);
+      if (two) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) rq[u] = load16(d.q + lo + (int64_t)(v + u * stride) * VEC);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) vec(rp[u], rq[u], lo + (v + u * stride) * VEC);
+    }
+    for (; v < full; v += stride) {
+      Raw16 rq = {};
+      if (two) rq = load16(d.q + lo + (int64_t)v * VEC);
+      vec(load16(d.p + lo + (int64_t)v * VEC), rq, lo + v * VEC);
+    }
+    const int c = lo + full * VEC + me;
+    if (c < hi) one(c);
+  } else {
+    for (int c = lo + me; c < hi; c += stride) one(c);
+  }
+}
+
+template <int N> __device__ __forceinline__ double sum_of(const double (&x)[N]) {
+  if constexpr (N == 1) return x[0];
+  else {
+    double y[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) y[i] = x[2 * i] + x[2 * i + 1];
+    return sum_of(y);
+  }
+}
+
+// One block a sequence.  Each wave sums the weights of one stretch of the row; the stretch in which the goal lies is read
+// once more, a vector a thread, and the class found by a prefix sum over the block.
+template <typename T, bool UNIT, bool DRAFTER, int BS>
+__global__ void __launch_bounds__(BS)
 k_verify(const T* __restrict__ p, const T* __restrict__ q, VerifyArgs a) {
-  __shared__ double s_w[VER_SEGS], s_p[VER_SEGS], s_run[256];
-  __shared__ int s_n, s_seg, s_pick, s_last;
-  __shared__ bool s_all;
-  __shared__ double s_goal;
+  constexpr int WAVES = BS / 64, VEC = UNIT ? vec_of<T>() : 1;
+  __shared__ double s_sum[WAVES], s_scan[WAVES];
+  __shared__ int s_n, s_pick, s_last;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int64_t b = blockIdx.x; b < a.B; b += gridDim.x) {
     const int len = draft_length(a, b);
@@ -82,90 +131,111 @@ k_verify(const T* __restrict__ p, const T* __restrict__ q, VerifyArgs a) {
         const unsigned long long bad = __ballot(!ok);
         if (bad) { n = t0 + __ffsll(bad) - 1; break; }
       }
-      if (lane == 0) s_n = n;
+      if (lane == 0) { s_n = n; s_pick = 0x7fffffff; s_last = -1; }
     }
     __syncthreads();
     const int n = s_n;
-    const bool draws = n < a.Tp;
     int drawn = -1;
-    if (draws) {
+    if (n < a.Tp) {                            // else all are accepted and there is no row behind them
       Draw<T> d = {p + b * a.pB + n * a.pT, nullptr, a.pK, a.qK, -1};
       if (n < len) {
-        if (q) d.q = q + b * a.qB + n * a.qT;
+        if (DRAFTER) d.q = q + b * a.qB + n * a.qT;
         else {
           const int64_t c = int_at(a.tokens, a.token_kind, b * a.T + n);
           d.skip = c < 0 || c >= a.K ? -1 : (int)c;
         }
       }
-      const int seg = ((a.K + VER_SEGS - 1) / VER_SEGS + 63) / 64 * 64;       // classes of a segment
-      for (int i = 0; i < VER_SEGS / 4; ++i) {
-        const int g = wave * (VER_SEGS / 4) + i;
-        const int64_t lo = (int64_t)g * seg;
-        const int hi = lo + seg < a.K ? (int)(lo + seg) : a.K;
-        double w = 0., v = 0.;
-        for (int64_t c = lo + lane; c < hi; c += 64) { w += d.weight((int)c); v += d.whole((int)c); }
-        w = wave_sum(w);
-        v = wave_sum(v);
-        if (lane == 0) { s_w[g] = w; s_p[g] = v; }
-      }
-      __syncthreads();
-      if (tid == 0) {
-        double total = 0., whole = 0.;
-        for (int g = 0; g < VER_SEGS; ++g) { total += s_w[g]; whole += s_p[g]; }
-        const bool all = !(total > 0.);
-        double* const sum = all ? s_p : s_w;
-        const double goal = (double)a.sample_u[b] * (all ? whole : total);
-        double run = 0.;
-        int pick = -1;
-        double before = 0.;
-        for (int g = 0; g < VER_SEGS; ++g) {
-          if (sum[g] > 0.) {
-            pick = g;                          // the last with weight, if the goal is never passed
-            before = run;
-            if (run + sum[g] > goal) break;
-          }
-          run += sum[g];
+      const int stretch = ((a.K + WAVES - 1) / WAVES + 64 * VEC - 1) / (64 * VEC) * (64 * VEC);
+      double total = 0.;
+      for (int round = 0; round < 2; ++round) {
+        const int64_t lo = (int64_t)wave * stretch;
+        double sum = 0.;
+        if (lo < a.K) {
+          const int hi = lo + stretch < a.K ? (int)(lo + stretch) : a.K;
+          each_weight<T, UNIT, DRAFTER>(d, (int)lo, hi, lane, 64, [&](auto& w, int) { sum += sum_of(w); });
         }
-        s_seg = pick;
-        s_all = all;
-        s_goal = goal - before;
-        s_pick = 0x7fffffff;
-        s_last = -1;
-      }
-      __syncthreads();
-      const bool all = s_all;
-      const int g = s_seg;
-      if (g >= 0) {                            // -1: no class has weight
-        const int64_t lo = (int64_t)g * seg;
-        const int hi = lo + seg < a.K ? (int)(lo + seg) : a.K;
-        const int each = (seg + 255) / 256;
-        const int64_t c0 = lo + (int64_t)tid * each;
-        const int c1 = c0 + each < hi ? (int)(c0 + each) : hi;
-        double mine = 0.;
-        for (int64_t c = c0; c < c1; ++c) mine += all ? d.whole((int)c) : d.weight((int)c);
-        s_run[tid] = mine;
+        sum = wave_sum(sum);
+        if (lane == 0) s_sum[wave] = sum;
         __syncthreads();
-        double run = 0.;
-        for (int i = 0; i < tid; ++i) run += s_run[i];
-        const double goal = s_goal;
-        if (mine > 0.) {
-          int last = -1, pick = -1;
-          for (int64_t c = c0; c < c1 && pick < 0; ++c) {
-            const double w = all ? d.whole((int)c) : d.weight((int)c);
-            if (w > 0.) {
-              last = (int)c;
-              run += w;
-              if (run > goal) pick = (int)c;
+        total = 0.;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) total += s_sum[i];
+        if (total > 0. || (!d.q && d.skip < 0)) break;
+        d.q = nullptr;                         // nothing is left over: the target's row itself
+        d.skip = -1;
+        __syncthreads();
+      }
+      if (total > 0.) {
+        const double goal = (double)a.sample_u[b] * total;
+        // the stretch in which the running sum passes the goal, or the last that holds weight
+        int pick = 0;
+        double before = 0., run = 0.;
+        bool open = true;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+          if (open && s_sum[i] > 0.) {
+            pick = i;
+            before = run;
+            open = !(run + s_sum[i] > goal);
+          }
+          run += s_sum[i];
+        }
+        const int lo = pick * stretch, hi = lo + (int64_t)stretch < a.K ? lo + stretch : a.K;
+        run = before;
+        for (int c0 = lo; c0 < hi; c0 += BS * VEC) {
+          // this thread's VEC classes
+          const int64_t c = (int64_t)c0 + tid * VEC;
+          double w[VEC];
+          if (UNIT && c + VEC <= hi) {
+            float x[VEC], y[VEC] = {};
+            if constexpr (UNIT) {
+              unpack(load16(d.p + c), x);
+              if (DRAFTER && d.q) unpack(load16(d.q + c), y);
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) w[i] = weight_of(x[i], y[i], c + i != d.skip);
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+              w[i] = c + i < hi ? weight_of((float)d.p[(c + i) * a.pK], DRAFTER && d.q ? (float)d.q[(c + i) * a.qK] : 0.f, c + i != d.skip) : 0.;
+          }
+          double mine = 0.;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) mine += w[i];
+          double scan = mine;
+#pragma unroll
+          for (int o = 1; o < 64; o <<= 1) {
+            const double up = __shfl_up(scan, o, 64);
+            if (lane >= o) scan += up;
+          }
+          if (lane == 63) s_scan[wave] = scan;
+          __syncthreads();
+          double at = run + (scan - mine);
+#pragma unroll
+          for (int i = 0; i < WAVES; ++i) {
+            if (i < wave) at += s_scan[i];
+            run += s_scan[i];
+          }
+          int here = -1, last = -1;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            at += w[i];
+            if (w[i] > 0.) {
+              last = (int)c + i;
+              if (here < 0 && at > goal) here = last;
             }
           }
-          if (pick >= 0) atomicMin(&s_pick, pick);
-          atomicMax(&s_last, last);
+          // lanes are in class order: the first lane that passes, the last that holds weight
+          const unsigned long long passes = __ballot(here >= 0), holds = __ballot(last >= 0);
+          if (passes && lane == __ffsll(passes) - 1) atomicMin(&s_pick, here);
+          if (holds && lane == 63 - __clzll((long long)holds)) atomicMax(&s_last, last);
+          __syncthreads();
+          if (s_pick != 0x7fffffff) break;
         }
-        __syncthreads();
         drawn = s_pick != 0x7fffffff ? s_pick : s_last;
       }
     }
-    for (int t = tid; t < a.Tp; t += 256)
+    for (int t = tid; t < a.Tp; t += BS)
       put_int(a.out_tokens, a.token_kind, b * a.Tp + t, t < n ? int_at(a.tokens, a.token_kind, b * a.T + t) : t == n ? drawn : -1);
     if (tid == 0) put_int(a.out_accepted, a.token_kind, b, n);
     __syncthreads();
@@ -242,8 +312,8 @@ using namespace devis;
 extern "C" int devis_verify_drafts(const devis_verify_params* v, const void* target, const void* draft, void* out_tokens,
                                    void* out_accepted, void* stream) {
   if (!v || !target || !out_tokens || !out_accepted || !v->sample_u) return DEVIS_ERR_BAD_ARG;
-  if (v->B <= 0 || v->T < 0 || v->T > 0x7ffffffe || (v->Tp != v->T && v->Tp != v->T + 1) || v->Tp < 1) return DEVIS_ERR_BAD_ARG;
-  if (v->K < 1 || v->K >= 0x7fffffff || (v->T > 0 && (!v->tokens || !v->accept_u))) return DEVIS_ERR_BAD_ARG;
+  if (v->B <= 0 || v->T < 0 || v->T > MAX_CLASSES || (v->Tp != v->T && v->Tp != v->T + 1) || v->Tp < 1) return DEVIS_ERR_BAD_ARG;
+  if (v->K < 1 || v->K > MAX_CLASSES || (v->T > 0 && (!v->tokens || !v->accept_u))) return DEVIS_ERR_BAD_ARG;
   if (v->token_dtype != DEVIS_LABEL_I64 && v->token_dtype != DEVIS_LABEL_I32) return DEVIS_ERR_BAD_ARG;
   const VerifyArgs a = {v->tokens, v->accept_u, v->sample_u, v->lengths, out_tokens, out_accepted, v->B, (int)v->T, (int)v->Tp,
                         (int)v->K, v->pB, v->pT, v->pK, v->qB, v->qT, v->qK, v->token_dtype};
@@ -263,6 +333,13 @@ extern "C" int devis_verify_drafts(const devis_verify_params* v, const void* tar
     return launch_status();
   }
   const unsigned blocks = (unsigned)(v->B < (1 << 20) ? v->B : (1 << 20));
-  DEVIS_DISPATCH_DTYPE(v->dtype, hipLaunchKernelGGL(k_verify<T>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, (const T*)target, (const T*)draft, a));
+  const bool unit = v->pK == 1 && (!draft || v->qK == 1);
+#define LAUNCH_VERIFY(UNIT, DRAFTER, BS) hipLaunchKernelGGL((k_verify<T, UNIT, DRAFTER, BS>), dim3(blocks), dim3(BS), 0, (hipStream_t)stream, (const T*)target, (const T*)draft, a)
+#define LAUNCH_VERIFY_U(DRAFTER, BS) do { if (unit) LAUNCH_VERIFY(true, DRAFTER, BS); else LAUNCH_VERIFY(false, DRAFTER, BS); } while (0)
+#define LAUNCH_VERIFY_B(DRAFTER) do { if (v->K <= 1024) LAUNCH_VERIFY_U(DRAFTER, 64); else if (v->K <= 8192) LAUNCH_VERIFY_U(DRAFTER, 256); else LAUNCH_VERIFY_U(DRAFTER, 1024); } while (0)
+  DEVIS_DISPATCH_DTYPE(v->dtype, { if (draft) LAUNCH_VERIFY_B(true); else LAUNCH_VERIFY_B(false); });
+#undef LAUNCH_VERIFY_B
+#undef LAUNCH_VERIFY_U
+#undef LAUNCH_VERIFY
   return launch_status();
 }

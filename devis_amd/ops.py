@@ -943,6 +943,16 @@ def softplus_bwd(z: Tensor, g: Tensor) -> Tensor:
 def class_rows(x: Tensor, channels_last: bool):
     """``x`` (copied only if its strides are not regular) as rows of classes: (x, N, V, K, sN, sV, sK) with N the first
     dimension and V the product of the others; row (n, v) starts at n*sN + v*sV, its classes are sK apart."""
+    shape = x.shape
+    if x.is_contiguous() and len(shape) > 1 and x.numel():
+        n = shape[0]
+        if channels_last:
+            k = shape[-1]
+            v = x.numel() // (n * k)
+            return x, n, v, k, v * k, k, 1
+        k = shape[1]
+        v = x.numel() // (n * k)
+        return x, n, v, k, v * k, 1, v
     if x.dim() < (1 if channels_last else 2):
         raise _lib.DevisError("expected %s, got %d dimensions" % ("(..., K)" if channels_last else "(N, K, ...)", x.dim()))
     kd = x.dim() - 1 if channels_last else 1
@@ -1061,32 +1071,38 @@ def distill_params(logits: Tensor, values: Tensor, indices: Tensor, rest: Option
     return p, dev, shape, (x, t, i, rest, row_mask)
 
 
-def distill_fwd(params, dev: torch.device, shape, x: Tensor, want_rows: bool, want_scal: bool, want_stats: bool):
-    """-> (per_row fp32 | None, scal (3,) fp32 | None, stats | None)"""
+def distill_fwd(params, dev: torch.device, shape, x: Tensor, rows: bool, want_stats: bool):
+    """-> (loss fp32: () or one per row, scratch): scratch = what the backward needs - scal (2 fp32), then the rows'
+    statistics - and the workspace.  It is the call's own (not `workspace`): a captured graph keeps what it allocates to
+    itself, so two graphs replayed side by side do not meet in it."""
     lib = _lib.load()
+    ref = C.byref(params)
     with _on_device(dev):
-        f = dict(dtype=torch.float32, device=dev)
-        per_row = torch.empty(shape, **f) if want_rows else None
-        scal = torch.empty((3,), **f) if want_scal else None
-        stats = torch.empty((lib.devis_distill_stats_bytes(C.byref(params)),), dtype=torch.uint8, device=dev) if want_stats else None
-        # the workspace is the call's own (not `workspace`): a captured graph keeps what it allocates to itself, so two
-        # graphs replayed side by side do not meet in it
-        nb = lib.devis_distill_workspace_bytes(C.byref(params)) if want_scal else 0
-        ws = torch.empty((nb,), dtype=torch.uint8, device=dev) if want_scal else None
-        check(lib.devis_distill_fwd(C.byref(params), _p(x), _p(per_row), _p(scal), _p(stats), _p(ws), nb, _stream()), "distill_fwd")
-    return per_row, scal, stats
+        loss = torch.empty(shape if rows else (), dtype=torch.float32, device=dev)
+        ns = lib.devis_distill_stats_bytes(ref) if want_stats else 0
+        nb = 0 if rows else lib.devis_distill_workspace_bytes(ref)
+        scratch = torch.empty((16 + ns + nb,), dtype=torch.uint8, device=dev)
+        at, out = scratch.data_ptr(), loss.data_ptr()
+        rc = lib.devis_distill_fwd(ref, x.data_ptr(), out if rows else None, None if rows else out, None if rows else at,
+                                   at + 16 if ns else None, None if rows else at + 16 + ns, nb, _stream())
+        if rc:
+            check(rc, "distill_fwd")
+    return loss, scratch
 
 
-def distill_bwd(params, dev: torch.device, x: Tensor, channels_last: bool, stats: Tensor, scal: Optional[Tensor],
-                grad: Tensor, grad_rows: bool) -> Tensor:
+def distill_bwd(params, dev: torch.device, x: Tensor, channels_last: bool, scratch: Tensor, grad: Tensor,
+                grad_rows: bool) -> Tensor:
     with _on_device(dev):
         dx = torch.empty_like(x)
         y, _, _, _, dn, dv, dk = class_rows(dx, channels_last)
         if y is not dx:                                    # strides the kernel does not take
             dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
             dn, dv, dk = class_rows(dx, channels_last)[4:]
-        check(_lib.load().devis_distill_bwd(C.byref(params), _p(x), _p(stats), _p(scal), _p(grad), 1 if grad_rows else 0,
-                                            _p(dx), dn, dv, dk, _stream()), "distill_bwd")
+        at = scratch.data_ptr()
+        rc = _lib.load().devis_distill_bwd(C.byref(params), x.data_ptr(), at + 16, at, grad.data_ptr(), 1 if grad_rows else 0,
+                                           dx.data_ptr(), dn, dv, dk, _stream())
+        if rc:
+            check(rc, "distill_bwd")
     return dx
 
 

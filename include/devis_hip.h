@@ -381,7 +381,7 @@ int devis_softplus_bwd(const float* z, const float* g, float* dz, int64_t n, voi
 
 /* ------------------------------------------- two models' class distributions -- */
 /* No counterpart in the reference.  A row is one voxel's or one token's K class values; row (n, v) of `logits` starts at
- * n*sN + v*sV and its classes are sK apart (elements), as in devis_evid_loss_fwd; K has no upper bound below 2^31 - 1.
+ * n*sN + v*sV and its classes are sK apart (elements), as in devis_evid_loss_fwd; K <= 2^30.
  *
  * devis_top_logits: the k <= DEVIS_TOP_MAX_K largest logits of every row.  Classes are ordered by (value descending,
  * class ascending), a NaN as +inf; values (dtype of the logits) and indices (index_dtype: DEVIS_LABEL_I32, or
@@ -398,10 +398,10 @@ int devis_top_logits(const void* logits, int64_t sN, int64_t sV, int64_t sK, int
  *   loss of a row = temperature^2 [ sum_j p_j (log p_j - log q_{i_j}) + p_rest (log p_rest - log q_rest) ].
  * A row with row_mask[r] = 0 (r = n*V + v) or without a filled slot has loss and gradient 0 and is not counted.  A
  * filled slot whose class is outside [0, K) makes its row's loss and gradient NaN; nothing is read there.
- * fwd: per_row (optional, [N*V] fp32) the rows' losses; scal (optional, 3 fp32, with workspace)
- *   [0] their sum, or mean over the counted rows (mean = 1; 0 if none is)  [1] 1 or 1/counted  [2] counted;
- *   stats (devis_distill_stats_bytes, optional: needed by the backward).
- * bwd: dlogits (dtype of the logits; strides dN, dV, dK) = gradient, times grad[0] * scal[1], or times grad[r] with
+ * fwd: per_row (optional, [N*V] fp32) the rows' losses; loss (optional, one fp32, with workspace) their sum, or with
+ *   mean = 1 their mean over the counted rows (0 if none is); scal (2 fp32, with loss): 1 or 1/counted, and counted;
+ *   stats (devis_distill_stats_bytes, 16-byte aligned, optional: needed by the backward; 0 bytes for few classes).
+ * bwd: dlogits (dtype of the logits; strides dN, dV, dK) = gradient, times grad[0] * scal[0], or times grad[r] with
  *   grad_rows = 1.  Results do not depend on the order in which blocks run. */
 typedef struct devis_distill_params {
   int64_t N, V, K, k;
@@ -417,8 +417,8 @@ typedef struct devis_distill_params {
 } devis_distill_params;
 size_t devis_distill_workspace_bytes(const devis_distill_params* p);
 size_t devis_distill_stats_bytes(const devis_distill_params* p);
-int devis_distill_fwd(const devis_distill_params* p, const void* logits, float* per_row, float* scal, void* stats,
-                      void* workspace, size_t workspace_bytes, void* stream);
+int devis_distill_fwd(const devis_distill_params* p, const void* logits, float* per_row, float* loss, float* scal,
+                      void* stats, void* workspace, size_t workspace_bytes, void* stream);
 int devis_distill_bwd(const devis_distill_params* p, const void* logits, const void* stats, const float* scal,
                       const float* grad, int grad_rows, void* dlogits, int64_t dN, int64_t dV, int64_t dK, void* stream);
 

@@ -159,7 +159,7 @@ def test_c_entries_refuse_bad_arguments_without_a_gpu():
         z, V * K, K, sK, dt, N, V, K, k, T, vals, ph, idt, V * k, k, 1, None, None)
     for kw in (dict(N=0), dict(V=0), dict(K=0), dict(k=0), dict(k=9), dict(K=500, k=129), dict(T=0.0), dict(T=float("nan")),
                dict(T=float("inf")), dict(T=1e-45), dict(idt=_lib.LABEL_I64), dict(K=257, idt=_lib.LABEL_U8), dict(z=None),
-               dict(vals=None), dict(sK=0), dict(sK=-1), dict(K=2 ** 31), dict(dt=2)):
+               dict(vals=None), dict(sK=0), dict(sK=-1), dict(K=2 ** 30 + 1), dict(K=2 ** 31), dict(dt=2)):
         assert top(**kw) == -1, kw
 
     def params(**kw):
@@ -169,16 +169,17 @@ def test_c_entries_refuse_bad_arguments_without_a_gpu():
         return _lib.DistillParams(**d)
     for kw in (dict(N=0), dict(K=0), dict(k=0), dict(k=9), dict(K=500, k=129), dict(sK=0), dict(oK=0), dict(values=None),
                dict(indices=None), dict(temperature=0.0), dict(temperature=float("nan")), dict(dtype=2), dict(values_dtype=7),
-               dict(index_dtype=3), dict(K=2 ** 31)):
-        assert lib.devis_distill_fwd(C.byref(params(**kw)), ph, ph, None, ph, None, 0, None) == -1, kw
+               dict(index_dtype=3), dict(K=2 ** 30 + 1), dict(K=2 ** 31)):
+        assert lib.devis_distill_fwd(C.byref(params(**kw)), ph, ph, None, None, ph, None, 0, None) == -1, kw
         assert lib.devis_distill_bwd(C.byref(params(**kw)), ph, ph, ph, ph, 0, ph, 24, 8, 1, None) == -1, kw
     ok = params()
     nb = lib.devis_distill_workspace_bytes(C.byref(ok))
-    assert lib.devis_distill_fwd(None, ph, ph, None, ph, None, 0, None) == -1
-    assert lib.devis_distill_fwd(C.byref(ok), None, ph, None, ph, None, 0, None) == -1
-    assert lib.devis_distill_fwd(C.byref(ok), ph, None, None, ph, ph, nb, None) == -1
-    assert lib.devis_distill_fwd(C.byref(ok), ph, None, ph, ph, None, nb, None) == -1
-    assert lib.devis_distill_fwd(C.byref(ok), ph, None, ph, ph, ph, nb - 1, None) == -4
+    assert lib.devis_distill_fwd(None, ph, ph, None, None, ph, None, 0, None) == -1
+    assert lib.devis_distill_fwd(C.byref(ok), None, ph, None, None, ph, None, 0, None) == -1
+    assert lib.devis_distill_fwd(C.byref(ok), ph, None, None, None, ph, ph, nb, None) == -1
+    assert lib.devis_distill_fwd(C.byref(ok), ph, None, ph, None, ph, ph, nb, None) == -1
+    assert lib.devis_distill_fwd(C.byref(ok), ph, None, ph, ph, ph, None, nb, None) == -1
+    assert lib.devis_distill_fwd(C.byref(ok), ph, None, ph, ph, ph, ph, nb - 1, None) == -4
     assert lib.devis_distill_bwd(C.byref(ok), ph, ph, None, ph, 0, ph, 24, 8, 1, None) == -1
     assert lib.devis_distill_bwd(C.byref(ok), ph, ph, ph, None, 0, ph, 24, 8, 1, None) == -1
     assert lib.devis_distill_bwd(C.byref(ok), ph, ph, ph, ph, 0, None, 24, 8, 1, None) == -1
@@ -189,7 +190,7 @@ def test_c_entries_refuse_bad_arguments_without_a_gpu():
                  dtype=0, token_dtype=0)
         d.update(kw)
         return _lib.VerifyParams(**d)
-    for kw in (dict(B=0), dict(T=-1), dict(Tp=5), dict(Tp=2), dict(T=0, Tp=0), dict(K=0), dict(K=2 ** 31), dict(tokens=None),
+    for kw in (dict(B=0), dict(T=-1), dict(Tp=5), dict(Tp=2), dict(T=0, Tp=0), dict(K=0), dict(K=2 ** 30 + 1), dict(K=2 ** 31), dict(tokens=None),
                dict(accept_u=None), dict(sample_u=None), dict(token_dtype=1), dict(dtype=2)):
         assert lib.devis_verify_drafts(C.byref(vparams(**kw)), ph, ph, ph, ph, None) == -1, kw
     v = vparams()

@@ -620,12 +620,14 @@ def test_outputs_end_where_they_should(K, dtype):
     p = _lib.DistillParams(rows, 1, K, k, K, 0, 1, k, 0, 1, v.data_ptr(), i.data_ptr(), r.data_ptr(), None, 1.0, ops.dt_code(dtype),
                            ops.dt_code(v.dtype), _lib.LABEL_I32, 1)
     ns, nw = lib.devis_distill_stats_bytes(C.byref(p)), lib.devis_distill_workspace_bytes(C.byref(p))
-    gl, gs, gst, gw = guard(rows, torch.float32), guard(3, torch.float32), guard(ns, torch.uint8), guard(nw, torch.uint8)
-    assert lib.devis_distill_fwd(C.byref(p), z.data_ptr(), gl.data_ptr(), gs.data_ptr(), gst.data_ptr(), gw.data_ptr(), nw, st) == 0
+    gl, g1, gs, gst, gw = (guard(n, d) for n, d in ((rows, torch.float32), (1, torch.float32), (2, torch.float32), (ns, torch.uint8),
+                                                    (nw, torch.uint8)))
+    assert lib.devis_distill_fwd(C.byref(p), z.data_ptr(), gl.data_ptr(), g1.data_ptr(), gs.data_ptr(), gst.data_ptr(), gw.data_ptr(),
+                                 nw, st) == 0
     gd, one = guard(rows * K, dtype), torch.ones((), device="cuda")
     assert lib.devis_distill_bwd(C.byref(p), z.data_ptr(), gst.data_ptr(), gs.data_ptr(), one.data_ptr(), 0, gd.data_ptr(), K, 0, 1,
                                  st) == 0
     torch.cuda.synchronize()
-    for t in (gv, gi, gr, gl, gs, gst, gw, gd):
+    for t in (gv, gi, gr, gl, g1, gs, gst, gw, gd):
         assert (t[-64:] == 77).all()
     assert torch.isfinite(gd[:-64].float()).all()
