@@ -302,9 +302,12 @@ __device__ __forceinline__ float rcp_f(float x) { return __builtin_amdgcn_rcpf(x
 
 template <int KT>
 __device__ __forceinline__ float pick_class(const float (&x)[KT], int c) {
-  float v = x[0];
+  float v = 0.f;
 #pragma unroll
-  for (int i = 1; i < KT; ++i) v = c == i ? x[i] : v;
+  for (int i = 0; i < KT; ++i) {
+    const float xi = x[i];
+    if (c == i) v = xi;
+  }
   return v;
 }
 
@@ -319,25 +322,52 @@ template <int KT> struct FewRow {
   float off;                   // log2(S_student / S_teacher), both against their own maxima
 };
 
-// -> state as SlotShared::state
+// Row (n, v0 + lane) with n and v0 the block's.  -> state as SlotShared::state
 template <typename T, int KT, bool FULL, bool REST>
-__device__ __forceinline__ int few_row(const T* __restrict__ p, int64_t sK, int K, const Teacher& t, int64_t at, int64_t r,
-                                       float scale, double inv_t, FewRow<KT>& w) {
+__device__ __forceinline__ int few_row(const T* __restrict__ z, const RowShape& s, const Teacher& t, int64_t n, int64_t v0,
+                                       uint32_t lane, float scale, double inv_t, FewRow<KT>& w) {
+  const int K = s.K;
+  const int64_t r0 = n * s.V + v0, at = n * t.o.sN + v0 * t.o.sV;
+  const uint32_t slot = lane * (uint32_t)t.o.sV;
   const int k = t.o.K;
-  load_row<T, KT, FULL>(p, sK, K, w.x);
+  // every load of the row first, raw: nothing is looked at before all of them are on their way
+  lane_load_row<T, KT, FULL>(z + n * s.sN + v0 * s.sV, lane * (uint32_t)s.sV, s.sK, K, w.x);
+  const float rest = REST ? lane_load(t.rest + r0, lane) : neg_inf();
+  const unsigned keep = t.mask ? lane_load(t.mask + r0, lane) : 1u;
+  uint32_t raw[KT];
+  const bool wide = t.value_kind == DEVIS_F32;
+#pragma unroll
+  for (int j = 0; j < KT; ++j) {
+    raw[j] = wide ? 0xff800000u : 0xff80u;                   // -inf
+    w.c[j] = -1;
+  }
+  if (wide) {
+#pragma unroll
+    for (int j = 0; j < KT; ++j) if (j < k) raw[j] = lane_load((const uint32_t*)t.values + at + j * t.o.sK, slot);
+  } else {
+#pragma unroll
+    for (int j = 0; j < KT; ++j) if (j < k) raw[j] = lane_load((const uint16_t*)t.values + at + j * t.o.sK, slot);
+  }
+  if (t.index_kind == DEVIS_LABEL_U8) {
+#pragma unroll
+    for (int j = 0; j < KT; ++j) if (j < k) w.c[j] = lane_load((const uint8_t*)t.indices + at + j * t.o.sK, slot);
+  } else if (t.index_kind == DEVIS_LABEL_I32) {
+#pragma unroll
+    for (int j = 0; j < KT; ++j) if (j < k) w.c[j] = lane_load((const int32_t*)t.indices + at + j * t.o.sK, slot);
+  } else {
+#pragma unroll
+    for (int j = 0; j < KT; ++j) {
+      if (j < k) {
+        const int64_t c = lane_load((const int64_t*)t.indices + at + j * t.o.sK, slot);
+        w.c[j] = c < 0 || c >= K ? -1 : (int)c;
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < KT; ++j) w.a[j] = __builtin_bit_cast(float, raw[j] << (wide ? 0 : 16));
   float hi = neg_inf();
   bool bad = false;
   w.listed = 0;
-#pragma unroll
-  for (int j = 0; j < KT; ++j) {
-    w.a[j] = neg_inf();
-    w.c[j] = -1;
-    if (j < k) {
-      const int64_t i = at + j * t.o.sK;
-      w.a[j] = t.value_kind == DEVIS_F32 ? ((const float*)t.values)[i] : (float)((const bf16*)t.values)[i];
-      w.c[j] = class_at(t.indices, t.index_kind, i);
-    }
-  }
 #pragma unroll
   for (int j = 0; j < KT; ++j) {
     const bool filled = w.a[j] != neg_inf();
@@ -346,13 +376,13 @@ __device__ __forceinline__ int few_row(const T* __restrict__ p, int64_t sK, int 
     w.listed |= filled ? 1u << w.c[j] : 0u;
     hi = fmaxf(hi, w.a[j]);
   }
-  if (w.listed == 0) return 0;
+  if (w.listed == 0 || keep == 0) return 0;
   if (bad) return 2;
   // teacher, in base 2 against its largest logarithm
   w.a_rest = neg_inf();
   float shift = 0.f;
   if constexpr (REST) {
-    w.a_rest = (float)(((double)t.rest[r] - (double)hi * inv_t) * 1.4426950408889634);
+    w.a_rest = (float)(((double)rest - (double)hi * inv_t) * 1.4426950408889634);
     shift = fmaxf(w.a_rest, 0.f);
     w.a_rest -= shift;
   }
@@ -407,12 +437,13 @@ k_distill_few_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
   __shared__ double s_red[4];
   const float unit = temperature * 0.6931471805599453f;              // of the logarithms to base 2
   double loss_sum = 0., count = 0.;
+  const int64_t tiles = (s.V + 255) / 256;
   for (int64_t n = blockIdx.y; n < s.N; n += gridDim.y) {
-    for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < s.V; v += (int64_t)gridDim.x * 256) {
-      const int64_t r = n * s.V + v;
+    for (int64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
+      const int64_t v0 = (int64_t)scalar((int)i) * 256, r = n * s.V + v0 + threadIdx.x;
+      if (v0 + threadIdx.x >= s.V) continue;
       FewRow<KT> w;
-      const int state = row_masked(t, r) ? 0 : few_row<T, KT, FULL, REST>(z + n * s.sN + v * s.sV, s.sK, s.K, t,
-                                                                         n * t.o.sN + v * t.o.sV, r, scale, inv_t, w);
+      const int state = few_row<T, KT, FULL, REST>(z, s, t, n, v0, threadIdx.x, scale, inv_t, w);
       float loss = 0.f;
       if (state == 1) {
 #pragma unroll
@@ -450,12 +481,13 @@ __global__ void __launch_bounds__(256)
 k_distill_few_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
                   const float* __restrict__ scal, const float* __restrict__ grad, int grad_rows, T* __restrict__ dz, RowShape d) {
   const float g_all = grad_rows ? 0.f : grad[0] * scal[0];
+  const int64_t tiles = (s.V + 255) / 256;
   for (int64_t n = blockIdx.y; n < s.N; n += gridDim.y) {
-    for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < s.V; v += (int64_t)gridDim.x * 256) {
-      const int64_t r = n * s.V + v;
+    for (int64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
+      const int64_t v0 = (int64_t)scalar((int)i) * 256, r = n * s.V + v0 + threadIdx.x;
+      if (v0 + threadIdx.x >= s.V) continue;
       FewRow<KT> w;
-      const int state = row_masked(t, r) ? 0 : few_row<T, KT, FULL, REST>(z + n * s.sN + v * s.sV, s.sK, s.K, t,
-                                                                         n * t.o.sN + v * t.o.sV, r, scale, inv_t, w);
+      const int state = few_row<T, KT, FULL, REST>(z, s, t, n, v0, threadIdx.x, scale, inv_t, w);
       const float f = temperature * (grad_rows ? grad[r] : g_all);
       float out[KT];
       if (state == 1) {
@@ -473,9 +505,14 @@ k_distill_few_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
 #pragma unroll
         for (int c = 0; c < KT; ++c) out[c] = fill;
       }
-      store_row<T, KT, FULL>(dz + n * d.sN + v * d.sV, d.sK, s.K, out);
+      store_row<T, KT, FULL>(dz + n * d.sN + (v0 + threadIdx.x) * d.sV, d.sK, s.K, out);
     }
   }
+}
+
+// few classes, and rows that a 32-bit offset reaches from the block's first
+static bool few_classes(const devis_distill_params* a) {
+  return a->K <= FEW_CLASSES && a->N * a->V <= FEW_ROWS && (a->V == 1 ? a->sN : a->sV) <= FEW_STRIDE && (a->V == 1 ? a->oN : a->oV) <= FEW_STRIDE;
 }
 
 static int distill_blocks(int64_t NV) { return (int)(NV < DIS_MAX_BLOCKS ? NV : DIS_MAX_BLOCKS); }
@@ -517,7 +554,7 @@ size_t devis_distill_workspace_bytes(const devis_distill_params* a) {
 }
 
 size_t devis_distill_stats_bytes(const devis_distill_params* a) {
-  return a && a->N > 0 && a->V > 0 && a->K > FEW_CLASSES ? (size_t)a->N * (size_t)a->V * sizeof(RowStats) : 0;
+  return a && a->N > 0 && a->V > 0 && !few_classes(a) ? (size_t)a->N * (size_t)a->V * sizeof(RowStats) : 0;
 }
 
 int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* per_row, float* loss, float* scal, void* stats,
@@ -531,7 +568,7 @@ int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* 
   const bool unit = a->sK == 1;
   int blocks = distill_blocks(a->N * a->V);
   double* part = loss ? (double*)ws : nullptr;
-  if (a->K <= FEW_CLASSES) {
+  if (few_classes(a)) {
     if (one_stride(s) && one_stride(t.o)) { merge_rows(s); merge_rows(t.o); }
     const dim3 grid = few_grid(s.N, s.V, DIS_MAX_BLOCKS);
     blocks = (int)(grid.x * grid.y);
@@ -555,14 +592,14 @@ int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* 
 
 int devis_distill_bwd(const devis_distill_params* a, const void* logits, const void* stats, const float* scal, const float* grad,
                       int grad_rows, void* dlogits, int64_t dN, int64_t dV, int64_t dK, void* stream) {
-  if (!distill_args_ok(a, logits) || (!stats && a->K > FEW_CLASSES) || !grad || !dlogits || (!grad_rows && !scal)) return DEVIS_ERR_BAD_ARG;
+  if (!distill_args_ok(a, logits) || (!stats && !few_classes(a)) || !grad || !dlogits || (!grad_rows && !scal)) return DEVIS_ERR_BAD_ARG;
   if (!rows_ok(dN, dV, dK, a->N, a->V, a->K)) return DEVIS_ERR_BAD_ARG;
   RowShape s = {a->sN, a->sV, a->sK, a->N, a->V, (int)a->K}, d = {dN, dV, dK, a->N, a->V, (int)a->K};
   Teacher t = {a->values, a->indices, a->rest, a->row_mask, {a->oN, a->oV, a->oK, a->N, a->V, (int)a->k}, a->values_dtype, a->index_dtype};
   const double inv_t = 1.0 / (double)a->temperature;
   const float scale = (float)(1.4426950408889634 * inv_t);
   const bool unit = a->sK == 1 && dK == 1;
-  if (a->K <= FEW_CLASSES) {
+  if (few_classes(a)) {
     if (one_stride(s) && one_stride(t.o) && one_stride(d)) { merge_rows(s); merge_rows(t.o); merge_rows(d); }
     const dim3 grid = few_grid(s.N, s.V, 8192);
 #define LAUNCH_FEW(REST, KT, FULL) hipLaunchKernelGGL((k_distill_few_bwd<T, KT, FULL, REST>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, scal, grad, grad_rows, (T*)dlogits, d)

@@ -141,6 +141,7 @@ template <int BS> __device__ __forceinline__ double block_sum(double v, double* 
 // ---- few classes: a thread takes a whole row into registers.  KT = 2, 4, 8 or 16 bounds K; FULL: K = KT adjacent
 // classes, one load of the whole row.
 constexpr int FEW_CLASSES = 16;
+constexpr int64_t FEW_ROWS = (int64_t)1 << 38;             // tile numbers stay below 2^31
 
 template <typename T, int KT, bool FULL>
 __device__ __forceinline__ void load_row(const T* __restrict__ p, int64_t sK, int K, float (&x)[KT]) {
@@ -152,6 +153,29 @@ __device__ __forceinline__ void load_row(const T* __restrict__ p, int64_t sK, in
   } else {
 #pragma unroll
     for (int c = 0; c < KT; ++c) x[c] = c < K ? (float)p[(int64_t)c * sK] : neg_inf();
+  }
+}
+// A lane's element `lane` of an array whose place the whole block shares: a scalar address and one 32-bit offset a lane,
+// where 64-bit addresses of every class and slot would take most of the registers.  `lane` stays below 256 * FEW_STRIDE.
+constexpr int64_t FEW_STRIDE = (int64_t)1 << 20;
+// The block's tiles of 256 rows: readfirstlane keeps the tile number scalar and the loop's addresses from becoming
+// running 64-bit pointers a lane, one for every class and slot.
+__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+template <typename T> __device__ __forceinline__ T lane_load(const T* __restrict__ shared, uint32_t lane) {
+  T v;
+  __builtin_memcpy(&v, (const char*)shared + lane * (uint32_t)sizeof(T), sizeof(T));
+  return v;
+}
+template <typename T, int KT, bool FULL>
+__device__ __forceinline__ void lane_load_row(const T* __restrict__ shared, uint32_t lane, int64_t sK, int K, float (&x)[KT]) {
+  if constexpr (FULL) {
+    T raw[KT];
+    __builtin_memcpy(raw, (const char*)shared + lane * (uint32_t)sizeof(T), sizeof raw);
+#pragma unroll
+    for (int c = 0; c < KT; ++c) x[c] = (float)raw[c];
+  } else {
+#pragma unroll
+    for (int c = 0; c < KT; ++c) x[c] = c < K ? (float)lane_load(shared + c * sK, lane) : neg_inf();
   }
 }
 template <typename T, int KT, bool FULL>
