@@ -166,10 +166,12 @@ def dce_evidence_u_loss(p, alpha, c, current_step, lamda_step, total_step, eps, 
 
 # --------------------------------------------------------------------------- distillation (no counterpart in the reference)
 class _DistillFn(torch.autograd.Function):
-    """logits -> loss (scalar, or one per row), given the teacher's top logits."""
+    """logits -> loss (scalar, or one per row), given the teacher's top logits.  `how` = (channels_last, temperature,
+    reduction, grad mode of the caller)."""
 
     @staticmethod
-    def forward(ctx, logits, values, indices, rest, row_mask, channels_last, temperature, reduction, grad_on):
+    def forward(ctx, logits, values, indices, rest, row_mask, how):
+        channels_last, temperature, reduction, grad_on = how
         rows = reduction == "none"
         params, dev, shape, ts = ops.distill_params(logits, values, indices, rest, row_mask, channels_last, temperature,
                                                     reduction == "mean")
@@ -182,22 +184,48 @@ class _DistillFn(torch.autograd.Function):
         if need:
             ctx.save_for_backward(*ts, scratch)
             ctx.params, ctx.channels_last, ctx.rows = params, channels_last, rows
-            ctx.at = tuple(None if t is None else (t.data_ptr(), t.stride()) for t in ts)
+            ctx.at = _places(ts)
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        if ctx.empty:
-            shape, dtype, dev = ctx.like
-            return (torch.zeros(shape, dtype=dtype, device=dev),) + (None,) * 8
-        *ts, scratch = ctx.saved_tensors
-        x, params = ts[0], ctx.params
-        if tuple(None if t is None else (t.data_ptr(), t.stride()) for t in ts) != ctx.at:      # moved by saved-tensor hooks
-            params, _, _, ts = ops.distill_params(*ts, ctx.channels_last, params.temperature, params.mean)
-            x = ts[0]
+        if not torch.is_grad_enabled():
+            return (_distill_backward(ctx, g),) + (None,) * 5
+        # under create_graph: a second derivative has to be refused, not taken as zero
+        logits = ctx.saved_tensors[0] if not ctx.empty else g
+        with torch.no_grad():
+            dz = _distill_backward(ctx, g)
+        return (_NoSecondDerivative.apply(dz, logits, g),) + (None,) * 5
+
+
+class _NoSecondDerivative(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, dz, logits, g):
+        return dz.view_as(dz)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("distill_top_loss has no second derivative")
+
+
+def _places(ts):
+    x, t, i, r, m = ts
+    return (x.data_ptr(), x.stride(), t.data_ptr(), t.stride(), i.data_ptr(), i.stride(),
+            None if r is None else r.data_ptr(), None if m is None else m.data_ptr())
+
+
+def _distill_backward(ctx, g):
+    if ctx.empty:
+        shape, dtype, dev = ctx.like
+        return torch.zeros(shape, dtype=dtype, device=dev)
+    *ts, scratch = ctx.saved_tensors
+    params = ctx.params
+    if _places(ts) != ctx.at:                     # moved by saved-tensor hooks
+        params, _, _, ts = ops.distill_params(*ts, ctx.channels_last, params.temperature, params.mean)
+    if g.dtype != torch.float32 or not g.is_contiguous():
         g = g.contiguous().float()
-        return (ops.distill_bwd(params, x.device, x, ctx.channels_last, scratch, g, ctx.rows),) + (None,) * 8
+    x = ts[0]
+    return ops.distill_bwd(params, x.device, x, ctx.channels_last, scratch, g, ctx.rows)
 
 
 def distill_top_loss(logits: Tensor, values: Tensor, indices: Tensor, rest: Optional[Tensor] = None, channels_last: bool = True,
@@ -217,8 +245,8 @@ def distill_top_loss(logits: Tensor, values: Tensor, indices: Tensor, rest: Opti
         raise ValueError("reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
     if values.requires_grad or (rest is not None and rest.requires_grad):
         raise ValueError("distill_top_loss does not differentiate in the teacher: detach values and rest")
-    return _DistillFn.apply(logits, values, indices, rest, row_mask, bool(channels_last), float(temperature), reduction,
-                            torch.is_grad_enabled())
+    return _DistillFn.apply(logits, values, indices, rest, row_mask,
+                            (bool(channels_last), float(temperature), reduction, torch.is_grad_enabled()))
 
 
 # --------------------------------------------------------------------------- API-compat shims (torch ops)

@@ -311,172 +311,167 @@ __device__ __forceinline__ float pick_class(const float (&x)[KT], int c) {
   return v;
 }
 
-template <int KT> struct FewRow {
+// KS bounds the slots as KT bounds the classes.
+template <int KT, int KS> struct FewRow {
   float x[KT], e[KT];          // logits; exponentials, of a class in a slot against the row's maximum, else against m_rest
-  float a[KT], p[KT];          // slots: logit below the largest, share
-  int c[KT];
+  float a[KS], p[KS];          // slots: logit below the largest, share
+  int c[KS];
   unsigned listed;
+  int state;                   // as SlotShared::state
   float m, sum, inv;           // student: maximum, sum of exponentials against it, 1 / sum
   float sum_rest, to_m;        // classes in no slot: sum against m_rest, exp((m_rest - m)/T)
   float d_rest, a_rest, p_rest;
   float off;                   // log2(S_student / S_teacher), both against their own maxima
 };
 
-// Row (n, v0 + lane) with n and v0 the block's.  -> state as SlotShared::state
-template <typename T, int KT, bool FULL, bool REST>
-__device__ __forceinline__ int few_row(const T* __restrict__ z, const RowShape& s, const Teacher& t, int64_t n, int64_t v0,
-                                       uint32_t lane, float scale, double inv_t, FewRow<KT>& w) {
-  const int K = s.K;
+// Row (n, v0 + lane) with n and v0 the block's.  Straight-line: a row that is not counted is worked out all the same and
+// dropped at the end.
+template <typename T, int KT, int KS, bool FULL, bool REST>
+__device__ __forceinline__ void few_row(const T* __restrict__ z, const RowShape& s, const Teacher& t, int64_t n, int64_t v0,
+                                        uint32_t lane, float scale, double inv_t, FewRow<KT, KS>& w) {
+  const int K = s.K, k = t.o.K;
   const int64_t r0 = n * s.V + v0, at = n * t.o.sN + v0 * t.o.sV;
   const uint32_t slot = lane * (uint32_t)t.o.sV;
-  const int k = t.o.K;
-  // every load of the row first, raw: nothing is looked at before all of them are on their way
+  // every load first, raw: nothing is looked at before all of them are on their way.  Slots behind the last read the last.
   lane_load_row<T, KT, FULL>(z + n * s.sN + v0 * s.sV, lane * (uint32_t)s.sV, s.sK, K, w.x);
   const float rest = REST ? lane_load(t.rest + r0, lane) : neg_inf();
   const unsigned keep = t.mask ? lane_load(t.mask + r0, lane) : 1u;
-  uint32_t raw[KT];
   const bool wide = t.value_kind == DEVIS_F32;
+  uint32_t raw[KS];
+  int64_t of[KS];
 #pragma unroll
-  for (int j = 0; j < KT; ++j) {
-    raw[j] = wide ? 0xff800000u : 0xff80u;                   // -inf
-    w.c[j] = -1;
-  }
+  for (int j = 0; j < KS; ++j) of[j] = at + (j < k ? j : k - 1) * t.o.sK;
   if (wide) {
 #pragma unroll
-    for (int j = 0; j < KT; ++j) if (j < k) raw[j] = lane_load((const uint32_t*)t.values + at + j * t.o.sK, slot);
+    for (int j = 0; j < KS; ++j) raw[j] = lane_load((const uint32_t*)t.values + of[j], slot);
   } else {
 #pragma unroll
-    for (int j = 0; j < KT; ++j) if (j < k) raw[j] = lane_load((const uint16_t*)t.values + at + j * t.o.sK, slot);
+    for (int j = 0; j < KS; ++j) raw[j] = lane_load((const uint16_t*)t.values + of[j], slot);
   }
   if (t.index_kind == DEVIS_LABEL_U8) {
 #pragma unroll
-    for (int j = 0; j < KT; ++j) if (j < k) w.c[j] = lane_load((const uint8_t*)t.indices + at + j * t.o.sK, slot);
+    for (int j = 0; j < KS; ++j) w.c[j] = lane_load((const uint8_t*)t.indices + of[j], slot);
   } else if (t.index_kind == DEVIS_LABEL_I32) {
 #pragma unroll
-    for (int j = 0; j < KT; ++j) if (j < k) w.c[j] = lane_load((const int32_t*)t.indices + at + j * t.o.sK, slot);
+    for (int j = 0; j < KS; ++j) w.c[j] = lane_load((const int32_t*)t.indices + of[j], slot);
   } else {
 #pragma unroll
-    for (int j = 0; j < KT; ++j) {
-      if (j < k) {
-        const int64_t c = lane_load((const int64_t*)t.indices + at + j * t.o.sK, slot);
-        w.c[j] = c < 0 || c >= K ? -1 : (int)c;
-      }
+    for (int j = 0; j < KS; ++j) {
+      const int64_t c = lane_load((const int64_t*)t.indices + of[j], slot);
+      w.c[j] = c < 0 || c >= K ? -1 : (int)c;
     }
   }
-#pragma unroll
-  for (int j = 0; j < KT; ++j) w.a[j] = __builtin_bit_cast(float, raw[j] << (wide ? 0 : 16));
   float hi = neg_inf();
   bool bad = false;
   w.listed = 0;
 #pragma unroll
-  for (int j = 0; j < KT; ++j) {
+  for (int j = 0; j < KS; ++j) {
+    w.a[j] = __builtin_bit_cast(float, raw[j] << (wide ? 0 : 16));
+    w.a[j] = j < k ? +w.a[j] : neg_inf();
     const bool filled = w.a[j] != neg_inf();
     bad = bad || (filled && (unsigned)w.c[j] >= (unsigned)K);
-    w.c[j] = filled ? w.c[j] & (FEW_CLASSES - 1) : -1;
-    w.listed |= filled ? 1u << w.c[j] : 0u;
+    w.c[j] = filled ? w.c[j] & (FEW_CLASSES - 1) : FEW_CLASSES;
+    w.listed |= 1u << w.c[j];
     hi = fmaxf(hi, w.a[j]);
   }
-  if (w.listed == 0 || keep == 0) return 0;
-  if (bad) return 2;
+  w.listed &= (1u << FEW_CLASSES) - 1;
+  w.state = w.listed == 0 || keep == 0 ? 0 : bad ? 2 : 1;
   // teacher, in base 2 against its largest logarithm
   w.a_rest = neg_inf();
   float shift = 0.f;
   if constexpr (REST) {
     w.a_rest = (float)(((double)rest - (double)hi * inv_t) * 1.4426950408889634);
     shift = fmaxf(w.a_rest, 0.f);
-    w.a_rest -= shift;
   }
-  float sum_t = REST ? exp2_f(w.a_rest) : 0.f;
-  w.p_rest = sum_t;
+  w.p_rest = REST ? exp2_f(w.a_rest - shift) : 0.f;
+  float sum_t = w.p_rest;
 #pragma unroll
-  for (int j = 0; j < KT; ++j) {
+  for (int j = 0; j < KS; ++j) {
     w.a[j] -= hi;
     w.p[j] = exp2_f(fmaf(w.a[j], scale, -shift));
+    w.p[j] = w.c[j] == FEW_CLASSES ? 0.f : +w.p[j];
     sum_t += w.p[j];
   }
   const float inv_sum_t = rcp_f(sum_t);
 #pragma unroll
-  for (int j = 0; j < KT; ++j) w.p[j] *= inv_sum_t;
+  for (int j = 0; j < KS; ++j) w.p[j] *= inv_sum_t;
   w.p_rest *= inv_sum_t;
   // student
   w.m = max_of(w.x);
-  const float m = w.m == neg_inf() ? 0.f : w.m;
+  w.m = w.m == neg_inf() ? 0.f : +w.m;
   if constexpr (REST) {
     float m_rest = neg_inf();
 #pragma unroll
-    for (int c = 0; c < KT; ++c) m_rest = fmaxf(m_rest, (w.listed >> c) & 1u ? neg_inf() : w.x[c]);
-    w.d_rest = m_rest == neg_inf() ? 0.f : (m_rest - m) * scale;
-    const float ref = m_rest == neg_inf() ? 0.f : m_rest;
+    for (int c = 0; c < KT; ++c) m_rest = fmaxf(m_rest, (w.listed >> c) & 1u ? neg_inf() : +w.x[c]);
+    const bool none = m_rest == neg_inf();
+    w.d_rest = none ? 0.f : (m_rest - w.m) * scale;
+    const float ref = none ? 0.f : m_rest;
     w.to_m = exp2_f(w.d_rest);
     float in = 0.f;
     w.sum_rest = 0.f;
 #pragma unroll
     for (int c = 0; c < KT; ++c) {
       const bool l = (w.listed >> c) & 1u;
-      w.e[c] = exp2_f((w.x[c] - (l ? m : ref)) * scale);
-      in += l ? w.e[c] : 0.f;
-      w.sum_rest += l ? 0.f : w.e[c];
+      w.e[c] = exp2_f((w.x[c] - (l ? +w.m : ref)) * scale);
+      in += l ? +w.e[c] : 0.f;
+      w.sum_rest += l ? 0.f : +w.e[c];
     }
     w.sum = fmaf(w.sum_rest, w.to_m, in);
   } else {
 #pragma unroll
-    for (int c = 0; c < KT; ++c) w.e[c] = exp2_f((w.x[c] - m) * scale);
+    for (int c = 0; c < KT; ++c) w.e[c] = exp2_f((w.x[c] - w.m) * scale);
     w.sum = sum_of(w.e);
   }
   w.inv = w.sum == 0.f ? 0.f : rcp_f(w.sum);
   w.off = log2_f(w.sum * inv_sum_t) - shift;
-  w.a_rest += shift;
-  w.m = m;
-  return 1;
 }
 
-template <typename T, int KT, bool FULL, bool REST>
+template <typename T, int KT, int KS, bool FULL, bool REST>
 __global__ void __launch_bounds__(256)
 k_distill_few_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
                   float* __restrict__ per_row, double* __restrict__ partial) {
   __shared__ double s_red[4];
   const float unit = temperature * 0.6931471805599453f;              // of the logarithms to base 2
-  double loss_sum = 0., count = 0.;
+  double loss_sum = 0.;
+  int count = 0;
   const int64_t tiles = (s.V + 255) / 256;
   for (int64_t n = blockIdx.y; n < s.N; n += gridDim.y) {
     for (int64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
-      const int64_t v0 = (int64_t)scalar((int)i) * 256, r = n * s.V + v0 + threadIdx.x;
-      if (v0 + threadIdx.x >= s.V) continue;
-      FewRow<KT> w;
-      const int state = few_row<T, KT, FULL, REST>(z, s, t, n, v0, threadIdx.x, scale, inv_t, w);
+      const int64_t v0 = (int64_t)scalar((int)i) * 256;
+      const uint32_t lane = lane_id();
+      if (v0 + lane >= s.V) continue;
+      FewRow<KT, KS> w;
+      few_row<T, KT, KS, FULL, REST>(z, s, t, n, v0, lane, scale, inv_t, w);
       float loss = 0.f;
-      if (state == 1) {
 #pragma unroll
-        for (int j = 0; j < KT; ++j) {
-          const float x = pick_class(w.x, w.c[j]);
-          const float d = x == neg_inf() ? __builtin_inff() : fmaf(w.off, unit, w.a[j] - (x - w.m));
-          loss += w.p[j] == 0.f ? 0.f : w.p[j] * d;
-        }
-        if constexpr (REST) {
-          const float d = w.sum_rest == 0.f ? __builtin_inff() : unit * ((w.a_rest - w.d_rest) + (w.off - log2_f(w.sum_rest)));
-          loss += w.p_rest == 0.f ? 0.f : w.p_rest * d;
-        }
-        loss *= temperature;                   // the terms are T (log p - log q)
-      } else if (state == 2) {
-        loss = __builtin_nanf("");
+      for (int j = 0; j < KS; ++j) {
+        const float x = pick_class(w.x, w.c[j]);
+        const float d = x == neg_inf() ? __builtin_inff() : fmaf(w.off, unit, w.a[j] - (x - w.m));
+        loss += w.p[j] == 0.f ? 0.f : w.p[j] * d;
       }
-      if (per_row) per_row[r] = loss;
+      if constexpr (REST) {
+        const float d = w.sum_rest == 0.f ? __builtin_inff() : unit * ((w.a_rest - w.d_rest) + (w.off - log2_f(w.sum_rest)));
+        loss += w.p_rest == 0.f ? 0.f : w.p_rest * d;
+      }
+      loss *= temperature;                     // the terms are T (log p - log q)
+      loss = w.state == 1 ? loss : w.state ? __builtin_nanf("") : 0.f;
+      if (per_row) per_row[n * s.V + v0 + lane] = loss;
       loss_sum += (double)loss;
-      count += state ? 1. : 0.;
+      count += w.state ? 1 : 0;
     }
   }
   if (partial) {
     loss_sum = block_sum<256>(loss_sum, s_red);
-    count = block_sum<256>(count, s_red);
+    const double counted = block_sum<256>((double)count, s_red);
     if (threadIdx.x == 0) {
       const int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
       partial[2 * b] = loss_sum;
-      partial[2 * b + 1] = count;
+      partial[2 * b + 1] = counted;
     }
   }
 }
 
-template <typename T, int KT, bool FULL, bool REST>
+template <typename T, int KT, int KS, bool FULL, bool REST>
 __global__ void __launch_bounds__(256)
 k_distill_few_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
                   const float* __restrict__ scal, const float* __restrict__ grad, int grad_rows, T* __restrict__ dz, RowShape d) {
@@ -484,28 +479,25 @@ k_distill_few_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
   const int64_t tiles = (s.V + 255) / 256;
   for (int64_t n = blockIdx.y; n < s.N; n += gridDim.y) {
     for (int64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
-      const int64_t v0 = (int64_t)scalar((int)i) * 256, r = n * s.V + v0 + threadIdx.x;
-      if (v0 + threadIdx.x >= s.V) continue;
-      FewRow<KT> w;
-      const int state = few_row<T, KT, FULL, REST>(z, s, t, n, v0, threadIdx.x, scale, inv_t, w);
-      const float f = temperature * (grad_rows ? grad[r] : g_all);
+      const int64_t v0 = (int64_t)scalar((int)i) * 256;
+      const uint32_t lane = lane_id();
+      if (v0 + lane >= s.V) continue;
+      const float f = temperature * (grad_rows ? lane_load(grad + n * s.V + v0, lane) : g_all);
+      FewRow<KT, KS> w;
+      few_row<T, KT, KS, FULL, REST>(z, s, t, n, v0, lane, scale, inv_t, w);
+      const float w_rest = REST && w.sum_rest != 0.f ? w.to_m * w.inv - w.p_rest * rcp_f(w.sum_rest) : 0.f;
+      const float fill = w.state ? __builtin_nanf("") : 0.f;
       float out[KT];
-      if (state == 1) {
-        const float w_rest = REST && w.sum_rest != 0.f ? w.to_m * w.inv - w.p_rest * rcp_f(w.sum_rest) : 0.f;
 #pragma unroll
-        for (int c = 0; c < KT; ++c) {
-          float share = 0.f;
+      for (int c = 0; c < KT; ++c) {
+        float share = 0.f;
 #pragma unroll
-          for (int j = 0; j < KT; ++j) share += w.c[j] == c ? w.p[j] : 0.f;
-          const bool l = !REST || ((w.listed >> c) & 1u);
-          out[c] = f * (l ? fmaf(w.e[c], w.inv, -share) : w.e[c] * w_rest);
-        }
-      } else {
-        const float fill = state ? __builtin_nanf("") : 0.f;
-#pragma unroll
-        for (int c = 0; c < KT; ++c) out[c] = fill;
+        for (int j = 0; j < KS; ++j) share += w.c[j] == c ? +w.p[j] : 0.f;
+        const bool l = !REST || ((w.listed >> c) & 1u);
+        out[c] = f * (l ? fmaf(w.e[c], w.inv, -share) : w.e[c] * w_rest);
+        out[c] = w.state == 1 ? +out[c] : fill;
       }
-      store_row<T, KT, FULL>(dz + n * d.sN + (v0 + threadIdx.x) * d.sV, d.sK, s.K, out);
+      store_row<T, KT, FULL>(dz + n * d.sN + (v0 + lane) * d.sV, d.sK, s.K, out);
     }
   }
 }
@@ -530,11 +522,18 @@ static bool distill_args_ok(const devis_distill_params* a, const void* logits) {
 
 using namespace devis;
 
-#define DISTILL_DISPATCH_FEW(unit, KERNEL_REST, KERNEL)                                                          \
-  DEVIS_DISPATCH_DTYPE(a->dtype, {                                                                                \
-    if (a->rest) DEVIS_DISPATCH_FEW(a->K, unit, KERNEL_REST);                                                     \
-    else DEVIS_DISPATCH_FEW(a->K, unit, KERNEL);                                                                  \
-  })
+// KERNEL(KT, KS, FULL, REST); up to two slots and more than two are apart, because the slots are half of the work of a row
+#define DISTILL_FEW_FULL(KERNEL, KT, KS, REST) do { if (unit && a->K == KT) KERNEL(KT, KS, true, REST); else KERNEL(KT, KS, false, REST); } while (0)
+#define DISTILL_FEW_KS(KERNEL, KT, REST) do { if (a->k <= 2) DISTILL_FEW_FULL(KERNEL, KT, 2, REST); else DISTILL_FEW_FULL(KERNEL, KT, KT, REST); } while (0)
+#define DISTILL_FEW_KT(KERNEL, REST)                                                                              \
+  do {                                                                                                            \
+    if (a->K <= 2) DISTILL_FEW_FULL(KERNEL, 2, 2, REST);                                                          \
+    else if (a->K <= 4) DISTILL_FEW_KS(KERNEL, 4, REST);                                                          \
+    else if (a->K <= 8) DISTILL_FEW_KS(KERNEL, 8, REST);                                                          \
+    else DISTILL_FEW_KS(KERNEL, 16, REST);                                                                        \
+  } while (0)
+#define DISTILL_DISPATCH_FEW(KERNEL) \
+  DEVIS_DISPATCH_DTYPE(a->dtype, { if (a->rest) DISTILL_FEW_KT(KERNEL, true); else DISTILL_FEW_KT(KERNEL, false); })
 
 #define DISTILL_DISPATCH(KERNEL, ...)                                                                             \
   DEVIS_DISPATCH_DTYPE(a->dtype, {                                                                                \
@@ -572,12 +571,8 @@ int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* 
     if (one_stride(s) && one_stride(t.o)) { merge_rows(s); merge_rows(t.o); }
     const dim3 grid = few_grid(s.N, s.V, DIS_MAX_BLOCKS);
     blocks = (int)(grid.x * grid.y);
-#define LAUNCH_FEW(REST, KT, FULL) hipLaunchKernelGGL((k_distill_few_fwd<T, KT, FULL, REST>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, per_row, part)
-#define LAUNCH_FEW_REST(KT, FULL) LAUNCH_FEW(true, KT, FULL)
-#define LAUNCH_FEW_TOP(KT, FULL) LAUNCH_FEW(false, KT, FULL)
-    DISTILL_DISPATCH_FEW(unit, LAUNCH_FEW_REST, LAUNCH_FEW_TOP);
-#undef LAUNCH_FEW_TOP
-#undef LAUNCH_FEW_REST
+#define LAUNCH_FEW(KT, KS, FULL, REST) hipLaunchKernelGGL((k_distill_few_fwd<T, KT, KS, FULL, REST>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, per_row, part)
+    DISTILL_DISPATCH_FEW(LAUNCH_FEW);
 #undef LAUNCH_FEW
   } else {
 #define LAUNCH_DISTILL_FWD(UNIT, REST, BS) hipLaunchKernelGGL((k_distill_fwd<T, UNIT, REST, BS>), dim3(blocks), dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, t2, (RowStats*)stats, per_row, part)
@@ -602,12 +597,8 @@ int devis_distill_bwd(const devis_distill_params* a, const void* logits, const v
   if (few_classes(a)) {
     if (one_stride(s) && one_stride(t.o) && one_stride(d)) { merge_rows(s); merge_rows(t.o); merge_rows(d); }
     const dim3 grid = few_grid(s.N, s.V, 8192);
-#define LAUNCH_FEW(REST, KT, FULL) hipLaunchKernelGGL((k_distill_few_bwd<T, KT, FULL, REST>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, scal, grad, grad_rows, (T*)dlogits, d)
-#define LAUNCH_FEW_REST(KT, FULL) LAUNCH_FEW(true, KT, FULL)
-#define LAUNCH_FEW_TOP(KT, FULL) LAUNCH_FEW(false, KT, FULL)
-    DISTILL_DISPATCH_FEW(unit, LAUNCH_FEW_REST, LAUNCH_FEW_TOP);
-#undef LAUNCH_FEW_TOP
-#undef LAUNCH_FEW_REST
+#define LAUNCH_FEW(KT, KS, FULL, REST) hipLaunchKernelGGL((k_distill_few_bwd<T, KT, KS, FULL, REST>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, scal, grad, grad_rows, (T*)dlogits, d)
+    DISTILL_DISPATCH_FEW(LAUNCH_FEW);
 #undef LAUNCH_FEW
     return launch_status();
   }

@@ -161,6 +161,12 @@ constexpr int64_t FEW_STRIDE = (int64_t)1 << 20;
 // The block's tiles of 256 rows: readfirstlane keeps the tile number scalar and the loop's addresses from becoming
 // running 64-bit pointers a lane, one for every class and slot.
 __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// the thread's number, opaque to the optimiser where it is asked for: offsets are formed per tile and not kept
+__device__ __forceinline__ uint32_t lane_id() {
+  uint32_t lane = threadIdx.x;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
 template <typename T> __device__ __forceinline__ T lane_load(const T* __restrict__ shared, uint32_t lane) {
   T v;
   __builtin_memcpy(&v, (const char*)shared + lane * (uint32_t)sizeof(T), sizeof(T));

@@ -394,6 +394,18 @@ def test_distill_saved_tensors_moved_to_the_host_and_back():
             assert torch.equal(want, zd.grad)
 
 
+def test_distill_refuses_a_second_derivative():
+    from devis_amd import criterions
+    z, v, i, r = pair(3, 20, 2, 1.0, torch.float32, 8)
+    zd = z.cuda().requires_grad_(True)
+    loss = criterions.distill_top_loss(zd, v.cuda(), i.cuda(), r.cuda())
+    (g,) = torch.autograd.grad(loss, zd, create_graph=True)
+    (plain,) = torch.autograd.grad(criterions.distill_top_loss(zd, v.cuda(), i.cuda(), r.cuda()), zd)
+    assert torch.equal(g.detach(), plain)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        g.sum().backward()
+
+
 def test_distill_is_reproducible():
     from devis_amd import criterions
     z, v, i, r = pair(300, 2000, 20, 1.0, torch.bfloat16, 8)
