@@ -52,8 +52,8 @@ template <typename T> __device__ __forceinline__ void store_vec(T* p, const floa
 
 // f(x, c): x = the values of classes c, c + 1, .. (VEC of them, or one at a time behind the last whole vector), over
 // the classes [lo, hi) of one row, dealt to the BS threads of a block vector by vector.  UNIT: the classes are
-// adjacent in memory (sK = 1) and travel 16 bytes at a time, four loads in flight; otherwise one by one.
-template <typename T, bool UNIT, int BS, typename F>
+// adjacent in memory (sK = 1) and travel 16 bytes at a time, U loads in flight; otherwise one by one.
+template <typename T, bool UNIT, int BS, int U = 4, typename F>
 __device__ __forceinline__ void each_class(const T* __restrict__ p, int64_t sK, int lo, int hi, F f) {
   const int tid = threadIdx.x;
   if constexpr (UNIT) {
@@ -61,15 +61,17 @@ __device__ __forceinline__ void each_class(const T* __restrict__ p, int64_t sK, 
     const int full = (hi - lo) / VEC;
     const T* q = p + lo;
     int v = tid;
-    for (; v + 3 * BS < full; v += 4 * BS) {
-      Raw16 r[4];
+    if constexpr (U > 1) {
+      for (; v + (U - 1) * BS < full; v += U * BS) {
+        Raw16 r[U];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) r[u] = load16(q + (int64_t)(v + u * BS) * VEC);
+        for (int u = 0; u < U; ++u) r[u] = load16(q + (int64_t)(v + u * BS) * VEC);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        float x[VEC];
-        unpack(r[u], x);
-        f(x, lo + (v + u * BS) * VEC);
+        for (int u = 0; u < U; ++u) {
+          float x[VEC];
+          unpack(r[u], x);
+          f(x, lo + (v + u * BS) * VEC);
+        }
       }
     }
     for (; v < full; v += BS) {

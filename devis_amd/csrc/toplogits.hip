@@ -30,145 +30,315 @@ __device__ __forceinline__ float key_value(uint64_t key) {
   return __builtin_bit_cast(float, b);
 }
 
+template <int BS> constexpr int top_groups() { return BS == 256 ? 8 : BS == 1024 ? 4 : 0; }     // k_top_wide: groups a thread
+template <int BS> struct TopShared {
+  union {
+    uint64_t group[BS];                      // general: the threads' largest keys
+    uint32_t thread_max[BS];                 // wide: their values as ordered integers
+  };
+  union {
+    struct { float max[top_groups<BS>() * BS + 1], sum[top_groups<BS>() * BS + 1]; } groups;       // wide, until the list is begun
+    uint64_t list[TOP_CAP];
+  };
+  uint64_t tau, kth;
+  double red[BS / 64];
+  float max[BS / 64];
+  int n, items;
+};
+
+// what becomes of the list: its first k are the answer, the others join the rest (`sum`, against `base`)
+template <typename T, typename I, bool UNIT, int BS>
+__device__ __forceinline__ void top_finish(const T* __restrict__ p, const RowShape& s, int64_t r, int k, float scale, double inv_t,
+                                           T* __restrict__ values, I* __restrict__ indices, const RowShape& o,
+                                           float* __restrict__ rest, TopShared<BS>& sh, int n, double sum, float base) {
+  const int tid = threadIdx.x, K = s.K;
+  // rank the list; what does not make the first k joins the rest
+  for (int i = tid; i < n; i += BS) {
+    const uint64_t key = sh.list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += sh.list[j] > key ? 1 : 0;
+    if (rank < k) {
+      const int64_t at_o = row_offset(o, r) + rank * o.sK;
+      const int c = key_class(key);
+      values[at_o] = p[(int64_t)c * s.sK];
+      indices[at_o] = (I)c;
+      if (rank == k - 1) sh.kth = key;
+    } else {
+      sum += (double)exp2_f((key_value(key) - base) * scale);
+    }
+  }
+  if (rest) {
+    sum = block_sum<BS>(sum, sh.red);
+    __syncthreads();
+    float ref = base;
+    // the rest lies far below the listed classes (or they are infinite): take its own largest value as reference
+    if (!(sum > 0x1p-60) || !(ref < __builtin_inff())) {
+      const uint64_t kth = sh.kth;
+      float m = neg_inf();
+      each_class<T, UNIT, BS, 1>(p, s.sK, 0, K, [&](auto& x, int c) {
+        constexpr int N = sizeof(x) / sizeof(float);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float y = nan_high(x[i]);
+          if (top_key(y, c + i) < kth) m = fmaxf(m, y);
+        }
+      });
+      ref = block_max<BS>(m, sh.max);
+      float acc = 0.f;
+      each_class<T, UNIT, BS, 1>(p, s.sK, 0, K, [&](auto& x, int c) {
+        constexpr int N = sizeof(x) / sizeof(float);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float y = nan_high(x[i]);
+          if (top_key(y, c + i) < kth && y > neg_inf()) acc += exp2_f((y - ref) * scale);
+        }
+      });
+      sum = block_sum<BS>((double)acc, sh.red);
+    }
+    if (tid == 0) {
+      const bool unbounded = !(fabsf(ref) < __builtin_inff());       // nothing is left (-inf), or infinities are
+      rest[r] = unbounded ? ref : (float)((double)ref * inv_t + log(sum));
+    }
+  }
+}
+
+// One row, any strides and any contents, by one block.
+template <typename T, typename I, bool UNIT, int BS, int U>
+__device__ __forceinline__ void top_row_general(const T* __restrict__ p, const RowShape& s, int64_t r, int k, float scale, double inv_t,
+                                T* __restrict__ values, I* __restrict__ indices, const RowShape& o, float* __restrict__ rest,
+                                TopShared<BS>& sh) {
+  const int tid = threadIdx.x, K = s.K;
+  // pass 1: this thread's largest key (the vector first, then the class within it)
+  float best = neg_inf();
+  int at = -1;
+  each_class<T, UNIT, BS, U>(p, s.sK, 0, K, [&](auto& x, int c) {
+    constexpr int N = sizeof(x) / sizeof(float);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = nan_high(x[i]);
+    const float m = max_of(x);
+    if (m > best || at < 0) { best = m; at = c; }
+  });
+  uint64_t mine = 0;
+  if (at >= 0) {
+    int c = at;
+    while (nan_high((float)p[(int64_t)c * s.sK]) != best) ++c;       // ends inside the vector that gave `best`
+    mine = top_key(best, c);
+  }
+  sh.group[tid] = mine;
+  if (tid == 0) { sh.tau = 0; sh.n = 0; }
+  __syncthreads();
+  {
+    int above = 0;
+#pragma unroll 8
+    for (int j = 0; j < BS; ++j) above += sh.group[j] > mine ? 1 : 0;
+    if (mine != 0 && above == k - 1) sh.tau = mine;       // fewer than k threads hold a class: tau stays 0, all are listed
+  }
+  __syncthreads();
+  uint64_t tau = sh.tau;
+  float floor_v, base;
+  double sum;
+  int n;
+  uint64_t below = ~0ull;                                // some key no class reaches
+  for (;;) {
+    floor_v = tau ? key_value(tau) : neg_inf();
+    base = floor_v == neg_inf() ? 0.f : floor_v;
+    float acc = 0.f;
+    each_class<T, UNIT, BS, U>(p, s.sK, 0, K, [&](auto& x, int c) {
+      constexpr int N = sizeof(x) / sizeof(float);
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = nan_high(x[i]);
+      if (max_of(x) >= floor_v) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const uint64_t key = top_key(x[i], c + i);
+          if (key >= tau) {
+            const int at_n = atomicAdd(&sh.n, 1);
+            if (at_n < TOP_CAP) sh.list[at_n] = key;
+            x[i] = neg_inf();
+          }
+        }
+      }
+      float e[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) e[i] = exp2_f((x[i] - base) * scale);
+      acc += sum_of(e);
+    });
+    __syncthreads();
+    n = sh.n;
+    sum = (double)acc;
+    if (n <= TOP_CAP) break;
+    // More keys than the list holds (many large classes dealt to few threads).  Halve the interval [tau, below) until
+    // between k and TOP_CAP keys are left: keys differ, so the count takes every value in between.
+    __syncthreads();
+    for (;;) {
+      const uint64_t mid = tau + (below - tau) / 2;
+      int cnt = 0;
+      each_class<T, UNIT, BS, U>(p, s.sK, 0, K, [&](auto& x, int c) {
+        constexpr int N = sizeof(x) / sizeof(float);
+#pragma unroll
+        for (int i = 0; i < N; ++i) cnt += top_key(nan_high(x[i]), c + i) >= mid ? 1 : 0;
+      });
+      const int total = (int)block_sum<BS>((double)cnt, sh.red);
+      if (total < k) below = mid;
+      else tau = mid;
+      if (total >= k && total <= TOP_CAP) break;
+    }
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+  }
+  top_finish<T, I, UNIT, BS>(p, s, r, k, scale, inv_t, values, indices, o, rest, sh, n, sum, base);
+}
+
 template <typename T, typename I, bool UNIT, int BS>
 __global__ void __launch_bounds__(BS)
 k_top_rows(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t, T* __restrict__ values,
            I* __restrict__ indices, RowShape o, float* __restrict__ rest) {
-  __shared__ uint64_t s_group[BS];
-  __shared__ uint64_t s_list[TOP_CAP];
-  __shared__ uint64_t s_tau, s_kth;
-  __shared__ int s_n;
-  __shared__ double s_red[BS / 64];
-  __shared__ float s_max[BS / 64];
-  const int tid = threadIdx.x, K = s.K;
+  __shared__ TopShared<BS> sh;
   const int64_t NV = s.N * s.V;
   for (int64_t r = blockIdx.x; r < NV; r += gridDim.x) {
+    top_row_general<T, I, UNIT, BS, 4>(z + row_offset(s, r), s, r, k, scale, inv_t, values, indices, o, rest, sh);
+    __syncthreads();
+  }
+}
+
+// Long rows of adjacent classes, read once.  The classes are summed in groups of 8 vectors of one thread, each group's
+// maximum and sum of exponentials against it kept in LDS (16 KB a block: eight blocks of 256 threads stay on a CU).  The
+// k-th largest of the threads' maxima, found bit by bit by one wave, is a floor under the first k; only the groups that
+// reach it (about k of them) are read again, vector by vector over the whole block, and every other group's sum goes
+// into the rest as it is.  Rows on which this stalls - most groups reach the floor, because classes are equal or masked -
+// go the general way.
+constexpr int TOP_GROUP = 8;                  // vectors of a group
+constexpr int TOP_ITEMS = 440;                // groups read again (with the rest of the LDS: 1/8 of a CU)
+
+template <typename T, typename I, int BS>
+__global__ void __launch_bounds__(BS, BS == 256 ? 8 : 4)
+k_top_wide(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t, T* __restrict__ values,
+           I* __restrict__ indices, RowShape o, float* __restrict__ rest) {
+  constexpr int VEC = vec_of<T>(), GROUPS = top_groups<BS>();
+  __shared__ TopShared<BS> sh;
+  __shared__ int s_item[TOP_ITEMS];
+  const int tid = threadIdx.x, K = s.K;
+  const int64_t NV = s.N * s.V;
+  const int full = K / VEC;                                    // whole vectors
+  const int groups = (full + TOP_GROUP * BS - 1) / (TOP_GROUP * BS);
+  const int each = (groups + GROUPS - 1) / GROUPS;             // longer rows: `each` times as many vectors a group
+  for (int64_t r = blockIdx.x; r < NV; r += gridDim.x) {
     const T* p = z + row_offset(s, r);
-    // pass 1: this thread's largest key (the vector first, then the class within it)
     float best = neg_inf();
-    int at = -1;
-    each_class<T, UNIT, BS>(p, s.sK, 0, K, [&](auto& x, int c) {
-      constexpr int N = sizeof(x) / sizeof(float);
+    bool holds = false;
+    for (int g = 0; g * each < groups; ++g) {
+      float gm = neg_inf(), gs = 0.f;
+      for (int h = 0; h < 2 * each; ++h) {
+        const int v0 = (g * each * TOP_GROUP + h * 4) * BS + tid;
+        Raw16 raw[4];
+        float x[4][VEC], m = neg_inf(), e[4];
+        if (v0 - tid + 4 * BS <= full) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = nan_high(x[i]);
-      const float m = max_of(x);
-      if (m > best || at < 0) { best = m; at = c; }
-    });
-    uint64_t mine = 0;
-    if (at >= 0) {
-      int c = at;
-      while (nan_high((float)p[(int64_t)c * s.sK]) != best) ++c;       // ends inside the vector that gave `best`
-      mine = top_key(best, c);
-    }
-    s_group[tid] = mine;
-    if (tid == 0) { s_tau = 0; s_n = 0; }
-    __syncthreads();
-    {
-      int above = 0;
-#pragma unroll 8
-      for (int j = 0; j < BS; ++j) above += s_group[j] > mine ? 1 : 0;
-      if (mine != 0 && above == k - 1) s_tau = mine;       // fewer than k threads hold a class: tau stays 0, all are listed
-    }
-    __syncthreads();
-    uint64_t tau = s_tau;
-    float floor_v, base;
-    double sum;
-    int n;
-    uint64_t below = ~0ull;                                // some key no class reaches
-    for (;;) {
-      floor_v = tau ? key_value(tau) : neg_inf();
-      base = floor_v == neg_inf() ? 0.f : floor_v;
-      float acc = 0.f;
-      each_class<T, UNIT, BS>(p, s.sK, 0, K, [&](auto& x, int c) {
-        constexpr int N = sizeof(x) / sizeof(float);
+          for (int u = 0; u < 4; ++u) raw[u] = load16(p + (int64_t)(v0 + u * BS) * VEC);
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = nan_high(x[i]);
-        if (max_of(x) >= floor_v) {
+          for (int u = 0; u < 4; ++u) unpack(raw[u], x[u]);
+        } else {
+          if (v0 >= full) continue;
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const uint64_t key = top_key(x[i], c + i);
-            if (key >= tau) {
-              const int at_n = atomicAdd(&s_n, 1);
-              if (at_n < TOP_CAP) s_list[at_n] = key;
-              x[i] = neg_inf();
-            }
+          for (int u = 0; u < 4; ++u) {
+            if (v0 + u * BS < full) unpack(load16(p + (int64_t)(v0 + u * BS) * VEC), x[u]);
+            else
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) x[u][i] = neg_inf();
           }
         }
-        float e[N];
+        holds = true;
 #pragma unroll
-        for (int i = 0; i < N; ++i) e[i] = exp2_f((x[i] - base) * scale);
-        acc += sum_of(e);
-      });
-      __syncthreads();
-      n = s_n;
-      sum = (double)acc;
-      if (n <= TOP_CAP) break;
-      // More keys than the list holds (many large classes dealt to few threads).  Halve the interval [tau, below) until
-      // between k and TOP_CAP keys are left: keys differ, so the count takes every value in between.
-      __syncthreads();
-      for (;;) {
-        const uint64_t mid = tau + (below - tau) / 2;
-        int cnt = 0;
-        each_class<T, UNIT, BS>(p, s.sK, 0, K, [&](auto& x, int c) {
-          constexpr int N = sizeof(x) / sizeof(float);
+        for (int u = 0; u < 4; ++u) m = fmaxf(m, max_of(x[u]));
+        const float ref = m == neg_inf() ? 0.f : m;
 #pragma unroll
-          for (int i = 0; i < N; ++i) cnt += top_key(nan_high(x[i]), c + i) >= mid ? 1 : 0;
-        });
-        const int total = (int)block_sum<BS>((double)cnt, s_red);
-        if (total < k) below = mid;
-        else tau = mid;
-        if (total >= k && total <= TOP_CAP) break;
+        for (int u = 0; u < 4; ++u) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) x[u][i] = exp2_f((x[u][i] - ref) * scale);
+          e[u] = sum_of(x[u]);
+        }
+        const float sum = sum_of(e);
+        if (m > gm) { gs *= exp2_f((gm - m) * scale); gm = m; gs += sum; }
+        else gs += m == neg_inf() ? sum : sum * exp2_f((m - gm) * scale);
       }
-      if (tid == 0) s_n = 0;
-      __syncthreads();
+      if (gs != gs) gm = __builtin_inff();                     // a NaN, which orders as +inf, or an infinity
+      sh.groups.max[g * BS + tid] = gm;
+      sh.groups.sum[g * BS + tid] = gs;
+      best = fmaxf(best, gm);
     }
-    // rank the list; what does not make the first k joins the rest
-    for (int i = tid; i < n; i += BS) {
-      const uint64_t key = s_list[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += s_list[j] > key ? 1 : 0;
-      if (rank < k) {
-        const int64_t at_o = row_offset(o, r) + rank * o.sK;
-        const int c = key_class(key);
-        values[at_o] = p[(int64_t)c * s.sK];
-        indices[at_o] = (I)c;
-        if (rank == k - 1) s_kth = key;
-      } else {
-        sum += (double)exp2_f((key_value(key) - base) * scale);
-      }
-    }
-    if (rest) {
-      sum = block_sum<BS>(sum, s_red);
-      __syncthreads();
-      float ref = base;
-      // the rest lies far below the listed classes (or they are infinite): take its own largest value as reference
-      if (!(sum > 0x1p-60) || !(ref < __builtin_inff())) {
-        const uint64_t kth = s_kth;
-        float m = neg_inf();
-        each_class<T, UNIT, BS>(p, s.sK, 0, K, [&](auto& x, int c) {
-          constexpr int N = sizeof(x) / sizeof(float);
+    const int c_tail = full * VEC + tid;
+    const bool tail = c_tail < K;
+    const float x_tail = tail ? nan_high((float)p[c_tail]) : neg_inf();
+    best = fmaxf(best, x_tail);
+    sh.thread_max[tid] = holds || tail ? (uint32_t)(top_key(best, 0) >> 32) : 0;
+    if (tid == 0) { sh.n = 0; sh.items = 0; }
+    __syncthreads();
+    if (tid < 64) {
+      // the largest value that at least k threads reach; a bf16 value is in the upper half of its key
+      constexpr int BITS = 8 * sizeof(T);
+      uint32_t key[BS / 64], floor_key = 0;
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const float y = nan_high(x[i]);
-            if (top_key(y, c + i) < kth) m = fmaxf(m, y);
-          }
-        });
-        ref = block_max<BS>(m, s_max);
-        float acc = 0.f;
-        each_class<T, UNIT, BS>(p, s.sK, 0, K, [&](auto& x, int c) {
-          constexpr int N = sizeof(x) / sizeof(float);
+      for (int i = 0; i < BS / 64; ++i) key[i] = sh.thread_max[i * 64 + tid] >> (32 - BITS);
+      for (int bit = BITS - 1; bit >= 0; --bit) {
+        const uint32_t probe = floor_key | (1u << bit);
+        int reach = 0;
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const float y = nan_high(x[i]);
-            if (top_key(y, c + i) < kth && y > neg_inf()) acc += exp2_f((y - ref) * scale);
-          }
-        });
-        sum = block_sum<BS>((double)acc, s_red);
+        for (int i = 0; i < BS / 64; ++i) reach += __popcll(__ballot(key[i] >= probe));
+        if (reach >= k) floor_key = probe;
       }
       if (tid == 0) {
-        const bool unbounded = !(fabsf(ref) < __builtin_inff());       // nothing is left (-inf), or infinities are
-        rest[r] = unbounded ? ref : (float)((double)ref * inv_t + log(sum));
+        uint32_t b = floor_key << (32 - BITS);
+        if (BITS == 16 && !(b >> 31) && floor_key) b |= 0xffffu;       // negative values are stored inverted
+        sh.tau = (uint64_t)b << 32;
       }
+    }
+    __syncthreads();
+    const uint64_t tau = sh.tau;
+    const float floor_v = tau ? key_value(tau) : neg_inf();
+    float base = floor_v == neg_inf() ? 0.f : floor_v;
+    float acc = 0.f;
+    for (int g = 0; g * each < groups; ++g) {
+      const float gm = sh.groups.max[g * BS + tid];
+      if (gm >= floor_v) {
+        const int at = atomicAdd(&sh.items, 1);
+        if (at < TOP_ITEMS) s_item[at] = g * BS + tid;
+      } else {
+        acc += sh.groups.sum[g * BS + tid] * exp2_f((gm - base) * scale);
+      }
+    }
+    __syncthreads();
+    const int items = sh.items;
+    bool stalled = items > TOP_ITEMS || !tau;
+    if (!stalled) {
+      const auto take = [&](float x, int c) {
+        if (x >= floor_v) {
+          const int at = atomicAdd(&sh.n, 1);
+          if (at < TOP_CAP) sh.list[at] = top_key(x, c);
+        } else {
+          acc += exp2_f((x - base) * scale);
+        }
+      };
+      for (int q = tid; q < items * TOP_GROUP; q += BS) {
+        const int item = s_item[q / TOP_GROUP], g = item / BS, t = item % BS;
+        for (int h = 0; h < each; ++h) {
+          const int v = ((g * each + h) * TOP_GROUP + q % TOP_GROUP) * BS + t;
+          if (v < full) {
+            float x[VEC];
+            unpack(load16(p + (int64_t)v * VEC), x);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) take(nan_high(x[i]), v * VEC + i);
+          }
+        }
+      }
+      if (tail) take(x_tail, c_tail);
+      __syncthreads();
+      stalled = sh.n > TOP_CAP;
+    }
+    if (stalled) {
+      __syncthreads();
+      top_row_general<T, I, true, BS, 1>(p, s, r, k, scale, inv_t, values, indices, o, rest, sh);
+    } else {
+      top_finish<T, I, true, BS>(p, s, r, k, scale, inv_t, values, indices, o, rest, sh, sh.n, (double)acc, base);
     }
     __syncthreads();
   }
@@ -250,9 +420,17 @@ extern "C" int devis_top_logits(const void* logits, int64_t sN, int64_t sV, int6
   const unsigned blocks = (unsigned)(NV < (1 << 20) ? NV : (1 << 20));
 #define LAUNCH_TOP(I, UNIT, BS) hipLaunchKernelGGL((k_top_rows<T, I, UNIT, BS>), dim3(blocks), dim3(BS), 0, st, (const T*)logits, s, (int)k, scale, inv_t, (T*)values, (I*)indices, o, rest)
 #define LAUNCH_TOP_U(I, BS) do { if (sK == 1) LAUNCH_TOP(I, true, BS); else LAUNCH_TOP(I, false, BS); } while (0)
-#define LAUNCH_TOP_B(I) do { if (K <= TOP_CAP) LAUNCH_TOP_U(I, 64); else LAUNCH_TOP_U(I, 256); } while (0)
+#define LAUNCH_WIDE(I, BS) hipLaunchKernelGGL((k_top_wide<T, I, BS>), dim3(blocks), dim3(BS), 0, st, (const T*)logits, s, (int)k, scale, inv_t, (T*)values, (I*)indices, o, rest)
+#define LAUNCH_TOP_B(I)                                                                                           \
+  do {                                                                                                            \
+    if (K <= TOP_CAP) LAUNCH_TOP_U(I, 64);                                                                        \
+    else if (sK != 1) LAUNCH_TOP(I, false, 256);                                                                  \
+    else if (K >= 16384 && NV < 256) LAUNCH_WIDE(I, 1024);                                                        \
+    else LAUNCH_WIDE(I, 256);                                                                                     \
+  } while (0)
   DEVIS_DISPATCH_DTYPE(dtype, { if (index_dtype == DEVIS_LABEL_U8) LAUNCH_TOP_B(uint8_t); else LAUNCH_TOP_B(int32_t); });
 #undef LAUNCH_TOP_B
+#undef LAUNCH_WIDE
 #undef LAUNCH_TOP_U
 #undef LAUNCH_TOP
   return launch_status();

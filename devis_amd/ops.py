@@ -1000,8 +1000,11 @@ def _same_device(what: str, *ts: Optional[Tensor]) -> torch.device:
 def _on_device(dev: torch.device):
     """Kernels launch on the current device: make it the tensors' own where it is another."""
     if dev.index == torch._C._cuda_getDevice():
-        return contextlib.nullcontext()
+        return _HERE
     return torch.cuda.device(dev)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def top_logits(logits: Tensor, k: int, channels_last: bool = True, temperature: float = 1.0, want_rest: bool = True):
@@ -1094,10 +1097,13 @@ def distill_bwd(params, dev: torch.device, x: Tensor, channels_last: bool, scrat
                 grad_rows: bool) -> Tensor:
     with _on_device(dev):
         dx = torch.empty_like(x)
-        y, _, _, _, dn, dv, dk = class_rows(dx, channels_last)
-        if y is not dx:                                    # strides the kernel does not take
-            dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-            dn, dv, dk = class_rows(dx, channels_last)[4:]
+        if dx.stride() == x.stride():
+            dn, dv, dk = params.sN, params.sV, params.sK
+        else:                                              # x had holes or shared elements: the gradient is dense
+            y, _, _, _, dn, dv, dk = class_rows(dx, channels_last)
+            if y is not dx:
+                dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+                dn, dv, dk = class_rows(dx, channels_last)[4:]
         at = scratch.data_ptr()
         rc = _lib.load().devis_distill_bwd(C.byref(params), x.data_ptr(), at + 16, at, grad.data_ptr(), 1 if grad_rows else 0,
                                            dx.data_ptr(), dn, dv, dk, _stream())
