@@ -141,7 +141,7 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
         }
         __syncthreads();
       }
-      each_class<T, UNIT, BS>(p, s.sK, lo, hi, [&](auto& x, int c) {
+      each_class<T, UNIT, BS>(tid, p, s.sK, lo, hi, [&](auto& x, int c) {
         constexpr int N = sizeof(x) / sizeof(float);
         if constexpr (REST) {
           const uint32_t b = s_bits[(c - lo) >> 5] >> ((c - lo) & 31);
@@ -272,7 +272,7 @@ k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
     if (!live) {
       for (int c = tid; c < K; c += BS) q[(int64_t)c * d.sK] = (T)0.f;
     } else {
-      each_class<T, UNIT, BS>(p, s.sK, 0, K, [&](auto& x, int c) {
+      each_class<T, UNIT, BS>(tid, p, s.sK, 0, K, [&](auto& x, int c) {
         constexpr int N = sizeof(x) / sizeof(float);
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = exp2_f((x[i] - st.ref) * scale) * w;
@@ -504,7 +504,7 @@ k_distill_few_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
 
 // few classes, and rows that a 32-bit offset reaches from the block's first
 static bool few_classes(const devis_distill_params* a) {
-  return a->K <= FEW_CLASSES && a->N * a->V <= FEW_ROWS && (a->V == 1 ? a->sN : a->sV) <= FEW_STRIDE && (a->V == 1 ? a->oN : a->oV) <= FEW_STRIDE;
+  return a->K <= FEW_CLASSES && (a->V == 1 ? a->sN : a->sV) <= FEW_STRIDE && (a->V == 1 ? a->oN : a->oV) <= FEW_STRIDE;
 }
 
 static int distill_blocks(int64_t NV) { return (int)(NV < DIS_MAX_BLOCKS ? NV : DIS_MAX_BLOCKS); }

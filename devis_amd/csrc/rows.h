@@ -50,12 +50,18 @@ __device__ __forceinline__ void store_vec(bf16* p, const float (&x)[8]) {
 __device__ __forceinline__ void store_vec(float* p, const float (&x)[4]) { __builtin_memcpy(p, x, 16); }
 template <typename T> __device__ __forceinline__ void store_vec(T* p, const float (&x)[1]) { *p = (T)x[0]; }
 
+// The thread's number, opaque to the optimiser where it is asked for: what is computed from it (offsets of a tile, of a
+// path that is rarely taken) is computed there and not kept in registers from the start.
+__device__ __forceinline__ uint32_t lane_id() {
+  uint32_t lane = threadIdx.x;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
 // f(x, c): x = the values of classes c, c + 1, .. (VEC of them, or one at a time behind the last whole vector), over
 // the classes [lo, hi) of one row, dealt to the BS threads of a block vector by vector.  UNIT: the classes are
 // adjacent in memory (sK = 1) and travel 16 bytes at a time, U loads in flight; otherwise one by one.
 template <typename T, bool UNIT, int BS, int U = 4, typename F>
-__device__ __forceinline__ void each_class(const T* __restrict__ p, int64_t sK, int lo, int hi, F f) {
-  const int tid = threadIdx.x;
+__device__ __forceinline__ void each_class(int tid, const T* __restrict__ p, int64_t sK, int lo, int hi, F f) {
   if constexpr (UNIT) {
     constexpr int VEC = vec_of<T>();
     const int full = (hi - lo) / VEC;
@@ -143,7 +149,6 @@ template <int BS> __device__ __forceinline__ double block_sum(double v, double* 
 // ---- few classes: a thread takes a whole row into registers.  KT = 2, 4, 8 or 16 bounds K; FULL: K = KT adjacent
 // classes, one load of the whole row.
 constexpr int FEW_CLASSES = 16;
-constexpr int64_t FEW_ROWS = (int64_t)1 << 38;             // tile numbers stay below 2^31
 
 template <typename T, int KT, bool FULL>
 __device__ __forceinline__ void load_row(const T* __restrict__ p, int64_t sK, int K, float (&x)[KT]) {
@@ -163,12 +168,6 @@ constexpr int64_t FEW_STRIDE = (int64_t)1 << 20;
 // The block's tiles of 256 rows: readfirstlane keeps the tile number scalar and the loop's addresses from becoming
 // running 64-bit pointers a lane, one for every class and slot.
 __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
-// the thread's number, opaque to the optimiser where it is asked for: offsets are formed per tile and not kept
-__device__ __forceinline__ uint32_t lane_id() {
-  uint32_t lane = threadIdx.x;
-  asm volatile("" : "+v"(lane));
-  return lane;
-}
 template <typename T> __device__ __forceinline__ T lane_load(const T* __restrict__ shared, uint32_t lane) {
   T v;
   __builtin_memcpy(&v, (const char*)shared + lane * (uint32_t)sizeof(T), sizeof(T));
@@ -217,8 +216,16 @@ inline dim3 few_grid(int64_t N, int64_t V, int most) {
 
 #define DEVIS_DISPATCH_FEW(K, unit, LAUNCH)                                                 do {                                                                                        if ((K) <= 2) { if ((unit) && (K) == 2) LAUNCH(2, true); else LAUNCH(2, false); }         else if ((K) <= 4) { if ((unit) && (K) == 4) LAUNCH(4, true); else LAUNCH(4, false); }     else if ((K) <= 8) { if ((unit) && (K) == 8) LAUNCH(8, true); else LAUNCH(8, false); }     else { if ((unit) && (K) == 16) LAUNCH(16, true); else LAUNCH(16, false); }             } while (0)
 
+// one block a row: rows over a 2-D grid (a dimension holds less than 2^32 threads)
+inline dim3 row_grid(int64_t rows) {
+  const int64_t x = rows < (1 << 20) ? rows : (1 << 20);
+  return dim3((unsigned)x, (unsigned)cdiv(rows, x));
+}
+constexpr int64_t MAX_ROWS = (int64_t)65535 << 20;
+__device__ __forceinline__ int64_t grid_row() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 inline bool rows_ok(int64_t sN, int64_t sV, int64_t sK, int64_t N, int64_t V, int64_t K) {
-  return N > 0 && V > 0 && K > 0 && K <= MAX_CLASSES && sN >= 0 && sV >= 0 && sK > 0 && N <= INT64_MAX / V;
+  return N > 0 && V > 0 && K > 0 && K <= MAX_CLASSES && sN >= 0 && sV >= 0 && sK > 0 && N <= MAX_ROWS / V;
 }
 
 }  // namespace devis

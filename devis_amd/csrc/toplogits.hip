@@ -70,12 +70,13 @@ __device__ __forceinline__ void top_finish(const T* __restrict__ p, const RowSha
   if (rest) {
     sum = block_sum<BS>(sum, sh.red);
     __syncthreads();
+    const int tid = lane_id();
     float ref = base;
     // the rest lies far below the listed classes (or they are infinite): take its own largest value as reference
     if (!(sum > 0x1p-60) || !(ref < __builtin_inff())) {
       const uint64_t kth = sh.kth;
       float m = neg_inf();
-      each_class<T, UNIT, BS, 1>(p, s.sK, 0, K, [&](auto& x, int c) {
+      each_class<T, UNIT, BS, 1>(tid, p, s.sK, 0, K, [&](auto& x, int c) {
         constexpr int N = sizeof(x) / sizeof(float);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -85,7 +86,7 @@ __device__ __forceinline__ void top_finish(const T* __restrict__ p, const RowSha
       });
       ref = block_max<BS>(m, sh.max);
       float acc = 0.f;
-      each_class<T, UNIT, BS, 1>(p, s.sK, 0, K, [&](auto& x, int c) {
+      each_class<T, UNIT, BS, 1>(tid, p, s.sK, 0, K, [&](auto& x, int c) {
         constexpr int N = sizeof(x) / sizeof(float);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -107,11 +108,11 @@ template <typename T, typename I, bool UNIT, int BS, int U>
 __device__ __forceinline__ void top_row_general(const T* __restrict__ p, const RowShape& s, int64_t r, int k, float scale, double inv_t,
                                 T* __restrict__ values, I* __restrict__ indices, const RowShape& o, float* __restrict__ rest,
                                 TopShared<BS>& sh) {
-  const int tid = threadIdx.x, K = s.K;
+  const int tid = lane_id(), K = s.K;
   // pass 1: this thread's largest key (the vector first, then the class within it)
   float best = neg_inf();
   int at = -1;
-  each_class<T, UNIT, BS, U>(p, s.sK, 0, K, [&](auto& x, int c) {
+  each_class<T, UNIT, BS, U>(tid, p, s.sK, 0, K, [&](auto& x, int c) {
     constexpr int N = sizeof(x) / sizeof(float);
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = nan_high(x[i]);
@@ -143,7 +144,7 @@ __device__ __forceinline__ void top_row_general(const T* __restrict__ p, const R
     floor_v = tau ? key_value(tau) : neg_inf();
     base = floor_v == neg_inf() ? 0.f : floor_v;
     float acc = 0.f;
-    each_class<T, UNIT, BS, U>(p, s.sK, 0, K, [&](auto& x, int c) {
+    each_class<T, UNIT, BS, U>(tid, p, s.sK, 0, K, [&](auto& x, int c) {
       constexpr int N = sizeof(x) / sizeof(float);
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] = nan_high(x[i]);
@@ -173,7 +174,7 @@ __device__ __forceinline__ void top_row_general(const T* __restrict__ p, const R
     for (;;) {
       const uint64_t mid = tau + (below - tau) / 2;
       int cnt = 0;
-      each_class<T, UNIT, BS, U>(p, s.sK, 0, K, [&](auto& x, int c) {
+      each_class<T, UNIT, BS, U>(tid, p, s.sK, 0, K, [&](auto& x, int c) {
         constexpr int N = sizeof(x) / sizeof(float);
 #pragma unroll
         for (int i = 0; i < N; ++i) cnt += top_key(nan_high(x[i]), c + i) >= mid ? 1 : 0;
@@ -194,11 +195,9 @@ __global__ void __launch_bounds__(BS)
 k_top_rows(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t, T* __restrict__ values,
            I* __restrict__ indices, RowShape o, float* __restrict__ rest) {
   __shared__ TopShared<BS> sh;
-  const int64_t NV = s.N * s.V;
-  for (int64_t r = blockIdx.x; r < NV; r += gridDim.x) {
+  const int64_t r = grid_row();
+  if (r < s.N * s.V)
     top_row_general<T, I, UNIT, BS, 4>(z + row_offset(s, r), s, r, k, scale, inv_t, values, indices, o, rest, sh);
-    __syncthreads();
-  }
 }
 
 // Long rows of adjacent classes, read once.  The classes are summed in groups of 8 vectors of one thread, each group's
@@ -218,129 +217,127 @@ k_top_wide(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t
   __shared__ TopShared<BS> sh;
   __shared__ int s_item[TOP_ITEMS];
   const int tid = threadIdx.x, K = s.K;
-  const int64_t NV = s.N * s.V;
+  const int64_t r = grid_row();
+  if (r >= s.N * s.V) return;
   const int full = K / VEC;                                    // whole vectors
   const int groups = (full + TOP_GROUP * BS - 1) / (TOP_GROUP * BS);
   const int each = (groups + GROUPS - 1) / GROUPS;             // longer rows: `each` times as many vectors a group
-  for (int64_t r = blockIdx.x; r < NV; r += gridDim.x) {
-    const T* p = z + row_offset(s, r);
-    float best = neg_inf();
-    bool holds = false;
-    for (int g = 0; g * each < groups; ++g) {
-      float gm = neg_inf(), gs = 0.f;
-      for (int h = 0; h < 2 * each; ++h) {
-        const int v0 = (g * each * TOP_GROUP + h * 4) * BS + tid;
-        Raw16 raw[4];
-        float x[4][VEC], m = neg_inf(), e[4];
-        if (v0 - tid + 4 * BS <= full) {
+  const T* p = z + row_offset(s, r);
+  float best = neg_inf();
+  bool holds = false;
+  for (int g = 0; g * each < groups; ++g) {
+    float gm = neg_inf(), gs = 0.f;
+    for (int h = 0; h < 2 * each; ++h) {
+      const int v0 = (g * each * TOP_GROUP + h * 4) * BS + tid;
+      Raw16 raw[4];
+      float x[4][VEC], m = neg_inf(), e[4];
+      if (v0 - tid + 4 * BS <= full) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) raw[u] = load16(p + (int64_t)(v0 + u * BS) * VEC);
+        for (int u = 0; u < 4; ++u) raw[u] = load16(p + (int64_t)(v0 + u * BS) * VEC);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) unpack(raw[u], x[u]);
-        } else {
-          if (v0 >= full) continue;
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if (v0 + u * BS < full) unpack(load16(p + (int64_t)(v0 + u * BS) * VEC), x[u]);
-            else
-#pragma unroll
-              for (int i = 0; i < VEC; ++i) x[u][i] = neg_inf();
-          }
-        }
-        holds = true;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) m = fmaxf(m, max_of(x[u]));
-        const float ref = m == neg_inf() ? 0.f : m;
+        for (int u = 0; u < 4; ++u) unpack(raw[u], x[u]);
+      } else {
+        if (v0 >= full) continue;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
+          if (v0 + u * BS < full) unpack(load16(p + (int64_t)(v0 + u * BS) * VEC), x[u]);
+          else
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) x[u][i] = exp2_f((x[u][i] - ref) * scale);
-          e[u] = sum_of(x[u]);
-        }
-        const float sum = sum_of(e);
-        if (m > gm) { gs *= exp2_f((gm - m) * scale); gm = m; gs += sum; }
-        else gs += m == neg_inf() ? sum : sum * exp2_f((m - gm) * scale);
-      }
-      if (gs != gs) gm = __builtin_inff();                     // a NaN, which orders as +inf, or an infinity
-      sh.groups.max[g * BS + tid] = gm;
-      sh.groups.sum[g * BS + tid] = gs;
-      best = fmaxf(best, gm);
-    }
-    const int c_tail = full * VEC + tid;
-    const bool tail = c_tail < K;
-    const float x_tail = tail ? nan_high((float)p[c_tail]) : neg_inf();
-    best = fmaxf(best, x_tail);
-    sh.thread_max[tid] = holds || tail ? (uint32_t)(top_key(best, 0) >> 32) : 0;
-    if (tid == 0) { sh.n = 0; sh.items = 0; }
-    __syncthreads();
-    if (tid < 64) {
-      // the largest value that at least k threads reach; a bf16 value is in the upper half of its key
-      constexpr int BITS = 8 * sizeof(T);
-      uint32_t key[BS / 64], floor_key = 0;
-#pragma unroll
-      for (int i = 0; i < BS / 64; ++i) key[i] = sh.thread_max[i * 64 + tid] >> (32 - BITS);
-      for (int bit = BITS - 1; bit >= 0; --bit) {
-        const uint32_t probe = floor_key | (1u << bit);
-        int reach = 0;
-#pragma unroll
-        for (int i = 0; i < BS / 64; ++i) reach += __popcll(__ballot(key[i] >= probe));
-        if (reach >= k) floor_key = probe;
-      }
-      if (tid == 0) {
-        uint32_t b = floor_key << (32 - BITS);
-        if (BITS == 16 && !(b >> 31) && floor_key) b |= 0xffffu;       // negative values are stored inverted
-        sh.tau = (uint64_t)b << 32;
-      }
-    }
-    __syncthreads();
-    const uint64_t tau = sh.tau;
-    const float floor_v = tau ? key_value(tau) : neg_inf();
-    float base = floor_v == neg_inf() ? 0.f : floor_v;
-    float acc = 0.f;
-    for (int g = 0; g * each < groups; ++g) {
-      const float gm = sh.groups.max[g * BS + tid];
-      if (gm >= floor_v) {
-        const int at = atomicAdd(&sh.items, 1);
-        if (at < TOP_ITEMS) s_item[at] = g * BS + tid;
-      } else {
-        acc += sh.groups.sum[g * BS + tid] * exp2_f((gm - base) * scale);
-      }
-    }
-    __syncthreads();
-    const int items = sh.items;
-    bool stalled = items > TOP_ITEMS || !tau;
-    if (!stalled) {
-      const auto take = [&](float x, int c) {
-        if (x >= floor_v) {
-          const int at = atomicAdd(&sh.n, 1);
-          if (at < TOP_CAP) sh.list[at] = top_key(x, c);
-        } else {
-          acc += exp2_f((x - base) * scale);
-        }
-      };
-      for (int q = tid; q < items * TOP_GROUP; q += BS) {
-        const int item = s_item[q / TOP_GROUP], g = item / BS, t = item % BS;
-        for (int h = 0; h < each; ++h) {
-          const int v = ((g * each + h) * TOP_GROUP + q % TOP_GROUP) * BS + t;
-          if (v < full) {
-            float x[VEC];
-            unpack(load16(p + (int64_t)v * VEC), x);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) take(nan_high(x[i]), v * VEC + i);
-          }
+            for (int i = 0; i < VEC; ++i) x[u][i] = neg_inf();
         }
       }
-      if (tail) take(x_tail, c_tail);
-      __syncthreads();
-      stalled = sh.n > TOP_CAP;
+      holds = true;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) m = fmaxf(m, max_of(x[u]));
+      const float ref = m == neg_inf() ? 0.f : m;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x[u][i] = exp2_f((x[u][i] - ref) * scale);
+        e[u] = sum_of(x[u]);
+      }
+      const float sum = sum_of(e);
+      if (m > gm) { gs *= exp2_f((gm - m) * scale); gm = m; gs += sum; }
+      else gs += m == neg_inf() ? sum : sum * exp2_f((m - gm) * scale);
     }
-    if (stalled) {
-      __syncthreads();
-      top_row_general<T, I, true, BS, 1>(p, s, r, k, scale, inv_t, values, indices, o, rest, sh);
+    if (gs != gs) gm = __builtin_inff();                     // a NaN, which orders as +inf, or an infinity
+    sh.groups.max[g * BS + tid] = gm;
+    sh.groups.sum[g * BS + tid] = gs;
+    best = fmaxf(best, gm);
+  }
+  const int c_tail = full * VEC + tid;
+  const bool tail = c_tail < K;
+  const float x_tail = tail ? nan_high((float)p[c_tail]) : neg_inf();
+  best = fmaxf(best, x_tail);
+  sh.thread_max[tid] = holds || tail ? (uint32_t)(top_key(best, 0) >> 32) : 0;
+  if (tid == 0) { sh.n = 0; sh.items = 0; }
+  __syncthreads();
+  if (tid < 64) {
+    // the largest value that at least k threads reach; a bf16 value is in the upper half of its key
+    constexpr int BITS = 8 * sizeof(T);
+    uint32_t key[BS / 64], floor_key = 0;
+#pragma unroll
+    for (int i = 0; i < BS / 64; ++i) key[i] = sh.thread_max[i * 64 + tid] >> (32 - BITS);
+    for (int bit = BITS - 1; bit >= 0; --bit) {
+      const uint32_t probe = floor_key | (1u << bit);
+      int reach = 0;
+#pragma unroll
+      for (int i = 0; i < BS / 64; ++i) reach += __popcll(__ballot(key[i] >= probe));
+      if (reach >= k) floor_key = probe;
+    }
+    if (tid == 0) {
+      uint32_t b = floor_key << (32 - BITS);
+      if (BITS == 16 && !(b >> 31) && floor_key) b |= 0xffffu;       // negative values are stored inverted
+      sh.tau = (uint64_t)b << 32;
+    }
+  }
+  __syncthreads();
+  const uint64_t tau = sh.tau;
+  const float floor_v = tau ? key_value(tau) : neg_inf();
+  float base = floor_v == neg_inf() ? 0.f : floor_v;
+  float acc = 0.f;
+  for (int g = 0; g * each < groups; ++g) {
+    const float gm = sh.groups.max[g * BS + tid];
+    if (gm >= floor_v) {
+      const int at = atomicAdd(&sh.items, 1);
+      if (at < TOP_ITEMS) s_item[at] = g * BS + tid;
     } else {
-      top_finish<T, I, true, BS>(p, s, r, k, scale, inv_t, values, indices, o, rest, sh, sh.n, (double)acc, base);
+      acc += sh.groups.sum[g * BS + tid] * exp2_f((gm - base) * scale);
     }
+  }
+  __syncthreads();
+  const int items = sh.items;
+  bool stalled = items > TOP_ITEMS || !tau;
+  if (!stalled) {
+    const auto take = [&](float x, int c) {
+      if (x >= floor_v) {
+        const int at = atomicAdd(&sh.n, 1);
+        if (at < TOP_CAP) sh.list[at] = top_key(x, c);
+      } else {
+        acc += exp2_f((x - base) * scale);
+      }
+    };
+    for (int q = tid; q < items * TOP_GROUP; q += BS) {
+      const int item = s_item[q / TOP_GROUP], g = item / BS, t = item % BS;
+      for (int h = 0; h < each; ++h) {
+        const int v = ((g * each + h) * TOP_GROUP + q % TOP_GROUP) * BS + t;
+        if (v < full) {
+          float x[VEC];
+          unpack(load16(p + (int64_t)v * VEC), x);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) take(nan_high(x[i]), v * VEC + i);
+        }
+      }
+    }
+    if (tail) take(x_tail, c_tail);
     __syncthreads();
+    stalled = sh.n > TOP_CAP;
+  }
+  if (stalled) {
+    __syncthreads();
+    top_row_general<T, I, true, BS, 1>(p, s, r, k, scale, inv_t, values, indices, o, rest, sh);
+  } else {
+    top_finish<T, I, true, BS>(p, s, r, k, scale, inv_t, values, indices, o, rest, sh, sh.n, (double)acc, base);
   }
 }
 
@@ -417,10 +414,9 @@ extern "C" int devis_top_logits(const void* logits, int64_t sN, int64_t sV, int6
 #undef LAUNCH_FEW
     return launch_status();
   }
-  const unsigned blocks = (unsigned)(NV < (1 << 20) ? NV : (1 << 20));
-#define LAUNCH_TOP(I, UNIT, BS) hipLaunchKernelGGL((k_top_rows<T, I, UNIT, BS>), dim3(blocks), dim3(BS), 0, st, (const T*)logits, s, (int)k, scale, inv_t, (T*)values, (I*)indices, o, rest)
+#define LAUNCH_TOP(I, UNIT, BS) hipLaunchKernelGGL((k_top_rows<T, I, UNIT, BS>), row_grid(NV), dim3(BS), 0, st, (const T*)logits, s, (int)k, scale, inv_t, (T*)values, (I*)indices, o, rest)
 #define LAUNCH_TOP_U(I, BS) do { if (sK == 1) LAUNCH_TOP(I, true, BS); else LAUNCH_TOP(I, false, BS); } while (0)
-#define LAUNCH_WIDE(I, BS) hipLaunchKernelGGL((k_top_wide<T, I, BS>), dim3(blocks), dim3(BS), 0, st, (const T*)logits, s, (int)k, scale, inv_t, (T*)values, (I*)indices, o, rest)
+#define LAUNCH_WIDE(I, BS) hipLaunchKernelGGL((k_top_wide<T, I, BS>), row_grid(NV), dim3(BS), 0, st, (const T*)logits, s, (int)k, scale, inv_t, (T*)values, (I*)indices, o, rest)
 #define LAUNCH_TOP_B(I)                                                                                           \
   do {                                                                                                            \
     if (K <= TOP_CAP) LAUNCH_TOP_U(I, 64);                                                                        \

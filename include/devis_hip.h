@@ -381,7 +381,8 @@ int devis_softplus_bwd(const float* z, const float* g, float* dz, int64_t n, voi
 
 /* ------------------------------------------- two models' class distributions -- */
 /* No counterpart in the reference.  A row is one voxel's or one token's K class values; row (n, v) of `logits` starts at
- * n*sN + v*sV and its classes are sK apart (elements), as in devis_evid_loss_fwd; K <= 2^30.
+ * n*sN + v*sV and its classes are sK apart (elements), as in devis_evid_loss_fwd; K <= 2^30 and
+ * N*V <= 65535 * 2^20.
  *
  * devis_top_logits: the k <= DEVIS_TOP_MAX_K largest logits of every row.  Classes are ordered by (value descending,
  * class ascending), a NaN as +inf; values (dtype of the logits) and indices (index_dtype: DEVIS_LABEL_I32, or
