@@ -16,6 +16,7 @@ namespace devis {
 
 constexpr int DIS_MAX_K = DEVIS_TOP_MAX_K;
 constexpr int DIS_SEG = 131072;               // classes whose slot bits are in LDS at a time (16 KB)
+constexpr int DIS_SHORT = 1024;               // classes up to which a wave takes a row, and the block several
 constexpr int DIS_MAX_BLOCKS = 2048;          // 8 blocks of 256 threads on each of 256 CUs
 
 // what the backward needs of a row
@@ -34,22 +35,30 @@ __device__ __forceinline__ int class_at(const void* idx, int kind, int64_t at) {
   return c < 0 || c > 0x7ffffffe ? -1 : (int)c;
 }
 
+__device__ __forceinline__ float slot_value(const Teacher& t, int64_t i) {
+  return t.value_kind == DEVIS_F32 ? ((const float*)t.values)[i] : (float)((const bf16*)t.values)[i];
+}
+
+// a row that takes no part; no counted row has this reference with a factor of zero
+__device__ __forceinline__ RowStats not_counted() { return RowStats{__builtin_inff(), 0.f, 0.f, 0.f}; }
+
 struct SlotShared {
-  float p[DIS_MAX_K];          // share of each slot
-  int c[DIS_MAX_K];            // its class
+  double logp[DIS_MAX_K];      // logarithm of each slot's share
+  float p[DIS_MAX_K];          // its share
+  int c[DIS_MAX_K];            // its class, -1 for an empty slot
+  int at[DIS_MAX_K];           // the same, before the shares are known (slot_classes)
   double p_rest, log_p_rest;
   int state;                   // 0 row not counted (masked, or every slot empty), 1 counted, 2 a slot names no class
 };
 
-// The teacher's softmax of one row, by the first wave; log p_j stay in registers (lane l: slots l and l + 64).  Shares
+// The teacher's softmax of one row, by the first wave (lane l: slots l and l + 64).  Shares
 // come from fp32 exponentials of fp64 differences; the normaliser and every logarithm are fp64, because the loss is
 // the difference of near-equal logarithms once the student is near the teacher.
-__device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int K, double inv_t, SlotShared& sh, double (&logp)[2],
-                                            int (&cls)[2]) {
-  const int lane = threadIdx.x;
+__device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int K, double inv_t, int lane, SlotShared& sh) {
   const int k = t.o.K;
   const int64_t at = row_offset(t.o, r);
   double y[2];
+  int cls[2];
   bool bad = false, any = false;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -58,7 +67,7 @@ __device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int K, 
     cls[u] = 0;
     if (j < k) {
       const int64_t i = at + j * t.o.sK;
-      const float v = t.value_kind == DEVIS_F32 ? ((const float*)t.values)[i] : (float)((const bf16*)t.values)[i];
+      const float v = slot_value(t, i);
       if (v != neg_inf()) {
         any = true;
         y[u] = (double)v * inv_t;
@@ -75,13 +84,12 @@ __device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int K, 
   const float e0 = expf((float)(y[0] - hi)), e1 = expf((float)(y[1] - hi)), er = expf((float)(yr - hi));
   const double sum = wave_sum((double)e0 + (double)e1) + (double)er;
   const double ls = log(sum);
-  logp[0] = y[0] - hi - ls;
-  logp[1] = y[1] - hi - ls;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int j = lane + 64 * u;
     if (j < k) {
       sh.p[j] = (float)((double)(u ? e1 : e0) / sum);
+      sh.logp[j] = y[u] - hi - ls;
       // an empty slot takes part in nothing
       sh.c[j] = y[u] == -__builtin_inf() ? -1 : cls[u];
     }
@@ -93,77 +101,128 @@ __device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int K, 
   }
 }
 
+// the classes of the filled slots, by the whole block
+template <int BS> __device__ __forceinline__ void slot_classes(const Teacher& t, int64_t r, int K, int tid, SlotShared& sh) {
+  const int64_t at = row_offset(t.o, r);
+  for (int j = tid; j < t.o.K; j += BS) {
+    const int64_t i = at + j * t.o.sK;
+    const int c = class_at(t.indices, t.index_kind, i);
+    sh.at[j] = slot_value(t, i) == neg_inf() || c >= K ? -1 : c;
+  }
+}
+
 __device__ __forceinline__ bool row_masked(const Teacher& t, int64_t r) { return t.mask && t.mask[r] == 0; }
 
 template <typename T, bool UNIT, bool REST, int BS>
-__global__ void __launch_bounds__(BS)
+__global__ void __launch_bounds__(BS, BS == 256 ? 8 : 1)
 k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, double t2, RowStats* __restrict__ stats,
               float* __restrict__ per_row, double* __restrict__ partial) {
+  constexpr bool LONG = BS > 64;
   __shared__ SlotShared sh;
   __shared__ uint32_t s_bits[REST ? DIS_SEG / 32 : 1];
   __shared__ double s_red[BS / 64];
   __shared__ float s_max[BS / 64];
-  const int tid = threadIdx.x, K = s.K;
+  const int K = s.K;
   const int64_t NV = s.N * s.V;
   double loss_sum = 0.;
-  int64_t count = 0;
-  for (int64_t r = blockIdx.x; r < NV; r += gridDim.x) {
+  int count = 0;
+  const int64_t first_row = grid_row();
+  if (first_row >= NV) return;
+  for (int64_t r = first_row; r < NV; r += gridDim.x) {
+    const int tid = lane_id();
     const T* p = z + row_offset(s, r);
-    double logp[2];
-    int cls[2];
     if (row_masked(t, r)) {
-      if (tid == 0) sh.state = 0;
-    } else if (tid < 64) {
-      teacher_row(t, r, K, inv_t, sh, logp, cls);
-    }
-    __syncthreads();
-    const int state = sh.state;
-    if (state != 1) {
-      const float v = state == 2 ? __builtin_nanf("") : 0.f;
       if (tid == 0) {
-        if (per_row) per_row[r] = v;
-        if (stats) stats[r] = RowStats{0.f, v, 0.f, v};
-        if (state == 2) { loss_sum += (double)v; ++count; }
+        if (per_row) per_row[r] = 0.f;
+        if (stats) stats[r] = not_counted();
       }
-      __syncthreads();
+      if (LONG) break;
       continue;
     }
+    // The first wave works out the teacher's shares, which nobody needs before the end, while the others begin; only
+    // the slots' classes are wanted first, for their bits.
+    if constexpr (REST) slot_classes<BS>(t, r, K, tid, sh);
+    if (tid < 64) teacher_row(t, r, K, inv_t, tid, sh);
     // running maximum and sum of the classes in no slot (all classes without REST)
     float m = neg_inf(), acc = 0.f;
+    const auto absorb = [&](auto& x) {
+      constexpr int N = sizeof(x) / sizeof(float);
+      const float mx = max_of(x);
+      if (mx > m) { acc *= exp2_f((m - mx) * scale); m = mx; }
+      const float ref = m == neg_inf() ? 0.f : m;
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = exp2_f((x[i] - ref) * scale);
+      acc += sum_of(x);
+    };
     for (int lo = 0; lo < K; lo += DIS_SEG) {
       const int hi = K - lo < DIS_SEG ? K : lo + DIS_SEG;
       if constexpr (REST) {
         for (int i = tid; i < (hi - lo + 31) / 32; i += BS) s_bits[i] = 0;
         __syncthreads();
         for (int j = tid; j < t.o.K; j += BS) {
-          const int c = sh.c[j];
+          const int c = sh.at[j];
           if (c >= lo && c < hi) atomicOr(&s_bits[(c - lo) >> 5], 1u << ((c - lo) & 31));
         }
         __syncthreads();
       }
-      each_class<T, UNIT, BS>(tid, p, s.sK, lo, hi, [&](auto& x, int c) {
-        constexpr int N = sizeof(x) / sizeof(float);
-        if constexpr (REST) {
-          const uint32_t b = s_bits[(c - lo) >> 5] >> ((c - lo) & 31);
-          if (b & ((1u << N) - 1u)) {
+      if constexpr (UNIT) {
+        constexpr int VEC = vec_of<T>();
+        const T* q = p + lo;
+        const int full = (hi - lo) / VEC;
+        // the slot bits of vector v: a byte, or half of one
+        const auto bits = [&](int v) -> uint32_t {
+          if constexpr (!REST) return 0;
+          else if constexpr (VEC == 8) return ((const uint8_t*)s_bits)[v];
+          else return (((const uint8_t*)s_bits)[v >> 1] >> ((v & 1) * 4)) & 15u;
+        };
+        int v = tid;
+        for (; v + 3 * BS < full; v += 4 * BS) {
+          Raw16 raw[4];
+          float x[4 * VEC];
+          uint32_t b = 0;
 #pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = (b >> i) & 1u ? neg_inf() : x[i];
+          for (int u = 0; u < 4; ++u) raw[u] = load16(q + (int64_t)(v + u * BS) * VEC);
+          if constexpr (REST) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) b |= bits(v + u * BS) << (u * VEC);
           }
-        }
-        const float mx = max_of(x);
-        if (mx > m) { acc *= exp2_f((m - mx) * scale); m = mx; }
-        const float ref = m == neg_inf() ? 0.f : m;
-        float e[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) e[i] = exp2_f((x[i] - ref) * scale);
-        acc += sum_of(e);
-      });
+          for (int u = 0; u < 4; ++u) unpack(raw[u], *(float(*)[VEC])(x + u * VEC));
+          if (REST && b) {
+#pragma unroll
+            for (int i = 0; i < 4 * VEC; ++i) x[i] = (b >> i) & 1u ? neg_inf() : +x[i];
+          }
+          absorb(x);
+        }
+        for (; v < full; v += BS) {
+          float x[VEC];
+          unpack(load16(q + (int64_t)v * VEC), x);
+          const uint32_t b = bits(v);
+          if (REST && b) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) x[i] = (b >> i) & 1u ? neg_inf() : +x[i];
+          }
+          absorb(x);
+        }
+        const int c = full * VEC + tid;
+        if (c < hi - lo && !(REST && (s_bits[c >> 5] >> (c & 31)) & 1u)) {
+          float x[1] = {(float)q[c]};
+          absorb(x);
+        }
+      } else {
+        for (int c = lo + tid; c < hi; c += BS) {
+          float x[1] = {(float)p[(int64_t)c * s.sK]};
+          if (REST && (s_bits[(c - lo) >> 5] >> ((c - lo) & 31)) & 1u) continue;
+          absorb(x);
+        }
+      }
       if constexpr (REST) __syncthreads();
     }
-    const float m_rest = block_max<BS>(m, s_max);
+    const float m_rest = block_max<BS>(m, s_max);              // (its barrier also ends the wait for the teacher's shares)
     const float ref = m_rest == neg_inf() ? 0.f : m_rest;
     double sum_rest = block_sum<BS>(m == neg_inf() ? (double)acc : (double)acc * (double)exp2_f((m - ref) * scale), s_red);
-    if (tid < 64) {
+    if (threadIdx.x < 64) {
+      const int tid = lane_id();
       // the listed classes' logits; a class in two slots counts once in the student's sum (its first slot)
       float x[2];
       bool first[2];
@@ -174,10 +233,12 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
         x[u] = neg_inf();
         first[u] = false;
         if (j < t.o.K && sh.c[j] >= 0) {
-          x[u] = (float)p[(int64_t)cls[u] * s.sK];
+          x[u] = (float)p[(int64_t)sh.c[j] * s.sK];
           if constexpr (REST) {
-            first[u] = true;
-            for (int i = 0; i < j; ++i) first[u] = first[u] && sh.c[i] != cls[u];
+            bool again = false;
+#pragma unroll 8
+            for (int i = 0; i < j; ++i) again |= sh.c[i] == sh.c[j];
+            first[u] = !again;
           }
         }
       }
@@ -199,11 +260,16 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
         if (j < t.o.K && sh.c[j] >= 0) {
           const double pj = (double)sh.p[j];
           const double logq = x[u] == neg_inf() ? -__builtin_inf() : ((double)x[u] - m_d) * inv_t - ls;
-          if (!(pj == 0.)) kl += pj * (logp[u] - logq);
+          if (!(pj == 0.)) kl += pj * (sh.logp[j] - logq);
         }
       }
       kl = wave_sum(kl);
-      if (tid == 0) {
+      if (tid == 0 && sh.state != 1) {
+        const float v = sh.state == 2 ? __builtin_nanf("") : 0.f;
+        if (per_row) per_row[r] = v;
+        if (stats) stats[r] = sh.state == 2 ? RowStats{0.f, v, 0.f, v} : not_counted();
+        if (sh.state == 2) { loss_sum += (double)v; ++count; }
+      } else if (tid == 0) {
         const double pr = sh.p_rest;
         double inv = sum > 0. ? 1. / sum : sum == 0. ? 0. : sum;
         double w = inv;
@@ -220,22 +286,38 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
         ++count;
       }
     }
+    if (LONG) break;                           // one row a block: nothing of the row's end is kept in registers from the start
     __syncthreads();
   }
-  if (partial && tid == 0) {
-    partial[2 * blockIdx.x] = loss_sum;
-    partial[2 * blockIdx.x + 1] = (double)count;
+  if (partial && threadIdx.x == 0) {
+    partial[2 * first_row] = loss_sum;
+    partial[2 * first_row + 1] = (double)count;
   }
 }
 
-// the sum or mean of the counted rows' losses; scal = what a row's gradient is multiplied by, and the rows counted
+// The sum or mean of the counted rows' losses; scal = what a row's gradient is multiplied by, and the rows counted.  More
+// partials than DIS_FINAL are first added up by DIS_STAGE blocks, in fixed order.
+constexpr int64_t DIS_FINAL = 16384;
+constexpr int DIS_STAGE = 512;
+
 __global__ void __launch_bounds__(256)
-k_distill_finalize(const double* __restrict__ partial, int n, int mean, float* __restrict__ out, float* __restrict__ scal) {
+k_distill_stage(const double* __restrict__ partial, int64_t n, double* __restrict__ out) {
   __shared__ double s_red[4];
+  const int64_t each = (n + DIS_STAGE - 1) / DIS_STAGE, lo = blockIdx.x * each, hi = lo + each < n ? lo + each : n;
   double loss = 0., count = 0.;
-  for (int i = threadIdx.x; i < n; i += 256) { loss += partial[2 * i]; count += partial[2 * i + 1]; }
+  for (int64_t i = lo + threadIdx.x; i < hi; i += 256) { loss += partial[2 * i]; count += partial[2 * i + 1]; }
   loss = block_sum<256>(loss, s_red);
   count = block_sum<256>(count, s_red);
+  if (threadIdx.x == 0) { out[2 * blockIdx.x] = loss; out[2 * blockIdx.x + 1] = count; }
+}
+
+__global__ void __launch_bounds__(1024)
+k_distill_finalize(const double* __restrict__ partial, int n, int mean, float* __restrict__ out, float* __restrict__ scal) {
+  __shared__ double s_red[16];
+  double loss = 0., count = 0.;
+  for (int i = threadIdx.x; i < n; i += 1024) { loss += partial[2 * i]; count += partial[2 * i + 1]; }
+  loss = block_sum<1024>(loss, s_red);
+  count = block_sum<1024>(count, s_red);
   if (threadIdx.x == 0) {
     const double f = mean ? 1. / (count > 0. ? count : 1.) : 1.;
     out[0] = (float)(loss * f);
@@ -245,29 +327,24 @@ k_distill_finalize(const double* __restrict__ partial, int n, int mean, float* _
 }
 
 template <typename T, bool UNIT, bool REST, int BS>
-__global__ void __launch_bounds__(BS)
+__global__ void __launch_bounds__(BS, BS == 256 ? 8 : 1)
 k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
               const RowStats* __restrict__ stats, const float* __restrict__ scal, const float* __restrict__ grad, int grad_rows,
               T* __restrict__ dz, RowShape d) {
   __shared__ SlotShared sh;
-  const int tid = threadIdx.x, K = s.K;
+  constexpr bool LONG = BS > 64;
+  const int K = s.K;
   const int64_t NV = s.N * s.V;
-  for (int64_t r = blockIdx.x; r < NV; r += gridDim.x) {
+  for (int64_t r = grid_row(); r < NV; r += gridDim.x) {
+    const int tid = lane_id();
     const T* p = z + row_offset(s, r);
     T* q = dz + row_offset(d, r);
-    double logp[2];
-    int cls[2];
-    if (row_masked(t, r)) {
-      if (tid == 0) sh.state = 0;
-    } else if (tid < 64) {
-      teacher_row(t, r, K, inv_t, sh, logp, cls);
-    }
-    __syncthreads();
-    const bool live = sh.state != 0;
+    RowStats st = not_counted();
+    if (!row_masked(t, r)) st = stats[r];
+    const bool live = !(st.ref == __builtin_inff() && st.w == 0.f);
+    if (live && tid < 64) teacher_row(t, r, K, inv_t, tid, sh);       // for the listed classes, at the end
     const float g = grad_rows ? grad[r] : grad[0] * scal[0];
     const float f = g * temperature;
-    RowStats st = {0.f, 0.f, 0.f, 0.f};
-    if (live) st = stats[r];
     const float w = f * st.w;
     if (!live) {
       for (int c = tid; c < K; c += BS) q[(int64_t)c * d.sK] = (T)0.f;
@@ -283,12 +360,14 @@ k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
         const int c = sh.c[j];
         if (c < 0 || sh.state == 2) continue;
         float share = 0.f;
+#pragma unroll 8
         for (int i = 0; i < t.o.K; ++i) share += sh.c[i] == c ? sh.p[i] : 0.f;
         const float x = (float)p[(int64_t)c * s.sK];
         const float qc = x == neg_inf() ? 0.f : exp2_f((x - st.m) * scale) * st.inv_s;
         q[(int64_t)c * d.sK] = (T)(f * (qc - share));
       }
     }
+    if (LONG) break;
     __syncthreads();
   }
 }
@@ -507,7 +586,13 @@ static bool few_classes(const devis_distill_params* a) {
   return a->K <= FEW_CLASSES && (a->V == 1 ? a->sN : a->sV) <= FEW_STRIDE && (a->V == 1 ? a->oN : a->oV) <= FEW_STRIDE;
 }
 
-static int distill_blocks(int64_t NV) { return (int)(NV < DIS_MAX_BLOCKS ? NV : DIS_MAX_BLOCKS); }
+// one block a row, or for short rows as many blocks as run at once
+static bool long_rows(const devis_distill_params* a) { return a->K > DIS_SHORT; }
+static dim3 distill_grid(const devis_distill_params* a) {
+  const int64_t NV = a->N * a->V;
+  return long_rows(a) ? row_grid(NV) : dim3((unsigned)(NV < DIS_MAX_BLOCKS ? NV : DIS_MAX_BLOCKS));
+}
+static int64_t distill_partials(const devis_distill_params* a) { return long_rows(a) ? a->N * a->V : DIS_MAX_BLOCKS; }
 
 static bool distill_args_ok(const devis_distill_params* a, const void* logits) {
   if (!a || !logits || !a->values || !a->indices) return false;
@@ -537,7 +622,7 @@ using namespace devis;
 
 #define DISTILL_DISPATCH(KERNEL, ...)                                                                             \
   DEVIS_DISPATCH_DTYPE(a->dtype, {                                                                                \
-    if (a->K <= 1024) {                                                                                           \
+    if (!long_rows(a)) {                                                                                          \
       if (unit) { if (a->rest) KERNEL(true, true, 64); else KERNEL(true, false, 64); }                            \
       else { if (a->rest) KERNEL(false, true, 64); else KERNEL(false, false, 64); }                               \
     } else {                                                                                                      \
@@ -549,7 +634,7 @@ using namespace devis;
 extern "C" {
 
 size_t devis_distill_workspace_bytes(const devis_distill_params* a) {
-  return a ? (size_t)DIS_MAX_BLOCKS * 2 * sizeof(double) : 0;
+  return a && a->N > 0 && a->V > 0 ? (size_t)(distill_partials(a) + DIS_STAGE) * 2 * sizeof(double) : 0;
 }
 
 size_t devis_distill_stats_bytes(const devis_distill_params* a) {
@@ -565,23 +650,29 @@ int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* 
   const double inv_t = 1.0 / (double)a->temperature, t2 = (double)a->temperature * (double)a->temperature;
   const float scale = (float)(1.4426950408889634 * inv_t);
   const bool unit = a->sK == 1;
-  int blocks = distill_blocks(a->N * a->V);
+  const dim3 rows = distill_grid(a);
+  int64_t parts = long_rows(a) ? a->N * a->V : rows.x;
   double* part = loss ? (double*)ws : nullptr;
   if (few_classes(a)) {
     if (one_stride(s) && one_stride(t.o)) { merge_rows(s); merge_rows(t.o); }
     const dim3 grid = few_grid(s.N, s.V, DIS_MAX_BLOCKS);
-    blocks = (int)(grid.x * grid.y);
+    parts = (int64_t)grid.x * grid.y;
 #define LAUNCH_FEW(KT, KS, FULL, REST) hipLaunchKernelGGL((k_distill_few_fwd<T, KT, KS, FULL, REST>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, per_row, part)
     DISTILL_DISPATCH_FEW(LAUNCH_FEW);
 #undef LAUNCH_FEW
   } else {
-#define LAUNCH_DISTILL_FWD(UNIT, REST, BS) hipLaunchKernelGGL((k_distill_fwd<T, UNIT, REST, BS>), dim3(blocks), dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, t2, (RowStats*)stats, per_row, part)
+#define LAUNCH_DISTILL_FWD(UNIT, REST, BS) hipLaunchKernelGGL((k_distill_fwd<T, UNIT, REST, BS>), rows, dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, t2, (RowStats*)stats, per_row, part)
     DISTILL_DISPATCH(LAUNCH_DISTILL_FWD);
   }
 #undef LAUNCH_DISTILL_FWD
   const int rc = launch_status();
   if (rc || !loss) return rc;
-  hipLaunchKernelGGL(k_distill_finalize, dim3(1), dim3(256), 0, (hipStream_t)stream, (const double*)ws, blocks, a->mean, loss, scal);
+  if (parts > DIS_FINAL) {
+    hipLaunchKernelGGL(k_distill_stage, dim3(DIS_STAGE), dim3(256), 0, (hipStream_t)stream, (const double*)part, parts, part + 2 * parts);
+    part += 2 * parts;
+    parts = DIS_STAGE;
+  }
+  hipLaunchKernelGGL(k_distill_finalize, dim3(1), dim3(1024), 0, (hipStream_t)stream, (const double*)part, (int)parts, a->mean, loss, scal);
   return launch_status();
 }
 
@@ -602,8 +693,8 @@ int devis_distill_bwd(const devis_distill_params* a, const void* logits, const v
 #undef LAUNCH_FEW
     return launch_status();
   }
-  const int blocks = distill_blocks(a->N * a->V);
-#define LAUNCH_DISTILL_BWD(UNIT, REST, BS) hipLaunchKernelGGL((k_distill_bwd<T, UNIT, REST, BS>), dim3(blocks), dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, (const RowStats*)stats, scal, grad, grad_rows, (T*)dlogits, d)
+  const dim3 rows = distill_grid(a);
+#define LAUNCH_DISTILL_BWD(UNIT, REST, BS) hipLaunchKernelGGL((k_distill_bwd<T, UNIT, REST, BS>), rows, dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, (const RowStats*)stats, scal, grad, grad_rows, (T*)dlogits, d)
   DISTILL_DISPATCH(LAUNCH_DISTILL_BWD);
 #undef LAUNCH_DISTILL_BWD
   return launch_status();
