@@ -17,6 +17,10 @@ namespace devis {
 constexpr int DIS_MAX_K = DEVIS_TOP_MAX_K;
 constexpr int DIS_SEG = 131072;               // classes whose slot bits are in LDS at a time (16 KB)
 constexpr int DIS_SHORT = 1024;               // classes up to which a wave takes a row, and the block several
+// A gradient as large as the 256 MB Infinity Cache cannot stay there for its reader: written past the caches it leaves the
+// logits in them, which the backward reads from the last row on.  Loss and gradient of 4096 x 131072 bf16 rows: 658 us with
+// ordinary stores, 613 past the caches; 2048 x 65536 (256 MB) 198 and 175; below, the gradient is better kept.
+constexpr double DIS_PAST_BYTES = 256. * 1024 * 1024;
 constexpr int DIS_MAX_BLOCKS = 2048;          // 8 blocks of 256 threads on each of 256 CUs
 
 // what the backward needs of a row
@@ -326,7 +330,7 @@ k_distill_finalize(const double* __restrict__ partial, int n, int mean, float* _
   }
 }
 
-template <typename T, bool UNIT, bool REST, int BS>
+template <typename T, bool UNIT, bool PAST, int BS>
 __global__ void __launch_bounds__(BS, BS == 256 ? 8 : 1)
 k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
               const RowStats* __restrict__ stats, const float* __restrict__ scal, const float* __restrict__ grad, int grad_rows,
@@ -335,7 +339,8 @@ k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
   constexpr bool LONG = BS > 64;
   const int K = s.K;
   const int64_t NV = s.N * s.V;
-  for (int64_t r = grid_row(); r < NV; r += gridDim.x) {
+  for (int64_t i = grid_row(); i < NV; i += gridDim.x) {
+    const int64_t r = NV - 1 - i;              // what the forward read last is still in the caches: it is read first
     const int tid = lane_id();
     const T* p = z + row_offset(s, r);
     T* q = dz + row_offset(d, r);
@@ -353,7 +358,7 @@ k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
         constexpr int N = sizeof(x) / sizeof(float);
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = exp2_f((x[i] - st.ref) * scale) * w;
-        store_vec(q + (int64_t)c * (UNIT ? 1 : d.sK), x);
+        store_vec<PAST>(q + (int64_t)c * (UNIT ? 1 : d.sK), x);
       });
       __syncthreads();                       // the listed classes are written again, by other threads
       for (int j = tid; j < t.o.K; j += BS) {
@@ -607,9 +612,9 @@ static bool distill_args_ok(const devis_distill_params* a, const void* logits) {
 
 using namespace devis;
 
-// KERNEL(KT, KS, FULL, REST); up to two slots and more than two are apart, because the slots are half of the work of a row
+// KERNEL(KT, KS, FULL, REST); the slots are bounded at 2, 4 or the classes, because they are half of the work of a row
 #define DISTILL_FEW_FULL(KERNEL, KT, KS, REST) do { if (unit && a->K == KT) KERNEL(KT, KS, true, REST); else KERNEL(KT, KS, false, REST); } while (0)
-#define DISTILL_FEW_KS(KERNEL, KT, REST) do { if (a->k <= 2) DISTILL_FEW_FULL(KERNEL, KT, 2, REST); else DISTILL_FEW_FULL(KERNEL, KT, KT, REST); } while (0)
+#define DISTILL_FEW_KS(KERNEL, KT, REST) do { if (a->k <= 2) DISTILL_FEW_FULL(KERNEL, KT, 2, REST); else if (a->k <= 4) DISTILL_FEW_FULL(KERNEL, KT, 4, REST); else DISTILL_FEW_FULL(KERNEL, KT, KT, REST); } while (0)
 #define DISTILL_FEW_KT(KERNEL, REST)                                                                              \
   do {                                                                                                            \
     if (a->K <= 2) DISTILL_FEW_FULL(KERNEL, 2, 2, REST);                                                          \
@@ -694,8 +699,14 @@ int devis_distill_bwd(const devis_distill_params* a, const void* logits, const v
     return launch_status();
   }
   const dim3 rows = distill_grid(a);
-#define LAUNCH_DISTILL_BWD(UNIT, REST, BS) hipLaunchKernelGGL((k_distill_bwd<T, UNIT, REST, BS>), rows, dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, (const RowStats*)stats, scal, grad, grad_rows, (T*)dlogits, d)
-  DISTILL_DISPATCH(LAUNCH_DISTILL_BWD);
+  const bool past = (double)(a->N * a->V) * (double)a->K * (a->dtype == DEVIS_F32 ? 4 : 2) >= DIS_PAST_BYTES;
+#define LAUNCH_DISTILL_BWD(UNIT, PAST, BS) hipLaunchKernelGGL((k_distill_bwd<T, UNIT, PAST, BS>), rows, dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, (const RowStats*)stats, scal, grad, grad_rows, (T*)dlogits, d)
+  DEVIS_DISPATCH_DTYPE(a->dtype, {
+    if (!long_rows(a)) { if (unit) LAUNCH_DISTILL_BWD(true, false, 64); else LAUNCH_DISTILL_BWD(false, false, 64); }
+    else if (!unit) LAUNCH_DISTILL_BWD(false, false, 256);
+    else if (past) LAUNCH_DISTILL_BWD(true, true, 256);
+    else LAUNCH_DISTILL_BWD(true, false, 256);
+  });
 #undef LAUNCH_DISTILL_BWD
   return launch_status();
 }

@@ -41,14 +41,26 @@ __device__ __forceinline__ void unpack(const Raw16& r, float (&x)[4]) {      // 
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = __builtin_bit_cast(float, r.w[i]);
 }
-__device__ __forceinline__ void store_vec(bf16* p, const float (&x)[8]) {
-  Raw16 r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r.w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
-  __builtin_memcpy(p, &r, 16);
+// PAST: write past the caches (an array that does not fit them, read by nobody before it has left them)
+typedef __attribute__((ext_vector_type(4))) uint32_t devis_u32x4;
+typedef devis_u32x4 devis_u32x4_any __attribute__((aligned(2)));
+template <bool PAST> __device__ __forceinline__ void store16(void* p, devis_u32x4 v) {
+  if constexpr (PAST) __builtin_nontemporal_store(v, (devis_u32x4_any*)p);
+  else *(devis_u32x4_any*)p = v;
 }
-__device__ __forceinline__ void store_vec(float* p, const float (&x)[4]) { __builtin_memcpy(p, x, 16); }
-template <typename T> __device__ __forceinline__ void store_vec(T* p, const float (&x)[1]) { *p = (T)x[0]; }
+template <bool PAST> __device__ __forceinline__ void store_vec(bf16* p, const float (&x)[8]) {
+  devis_u32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+  store16<PAST>(p, v);
+}
+template <bool PAST> __device__ __forceinline__ void store_vec(float* p, const float (&x)[4]) {
+  devis_u32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __builtin_bit_cast(uint32_t, x[i]);
+  store16<PAST>(p, v);
+}
+template <bool PAST, typename T> __device__ __forceinline__ void store_vec(T* p, const float (&x)[1]) { *p = (T)x[0]; }
 
 // The thread's number, opaque to the optimiser where it is asked for: what is computed from it (offsets of a tile, of a
 // path that is rarely taken) is computed there and not kept in registers from the start.
