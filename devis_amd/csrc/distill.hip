@@ -26,6 +26,12 @@ constexpr int DIS_MAX_BLOCKS = 2048;          // 8 blocks of 256 threads on each
 // what the backward needs of a row
 struct RowStats { float ref, w, m, inv_s; };  // gradient of a class in no slot: exp((z - ref)/T) w;  q = exp((z - m)/T) inv_s
 
+// The ends of a row: fp64 for long rows; for the short ones of a wave each, fp32 (there are many, and fp64 logarithms,
+// exponentials and quotients would cost more than the row).
+template <bool LONG> __device__ __forceinline__ double end_log(double x) { return LONG ? log(x) : 0.6931471805599453 * (double)__builtin_amdgcn_logf((float)x); }
+template <bool LONG> __device__ __forceinline__ double end_exp2(double x) { return LONG ? exp2(x) : (double)exp2_f((float)x); }
+template <bool LONG> __device__ __forceinline__ double end_div(double a, double b) { return LONG ? a / b : a * (double)(1.f / (float)b); }
+
 struct Teacher {
   const void* values; const void* indices; const float* rest; const uint8_t* mask;
   RowShape o;                                 // strides of values / indices, K = number of slots
@@ -58,6 +64,7 @@ struct SlotShared {
 // The teacher's softmax of one row, by the first wave (lane l: slots l and l + 64).  Shares
 // come from fp32 exponentials of fp64 differences; the normaliser and every logarithm are fp64, because the loss is
 // the difference of near-equal logarithms once the student is near the teacher.
+template <bool LONG>
 __device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int K, double inv_t, int lane, SlotShared& sh) {
   const int k = t.o.K;
   const int64_t at = row_offset(t.o, r);
@@ -87,19 +94,20 @@ __device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int K, 
   for (int o = 32; o > 0; o >>= 1) hi = fmax(hi, __shfl_xor(hi, o, 64));
   const float e0 = expf((float)(y[0] - hi)), e1 = expf((float)(y[1] - hi)), er = expf((float)(yr - hi));
   const double sum = wave_sum((double)e0 + (double)e1) + (double)er;
-  const double ls = log(sum);
+  const double ls = end_log<LONG>(sum);
+  const double inv = end_div<LONG>(1., sum);
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int j = lane + 64 * u;
     if (j < k) {
-      sh.p[j] = (float)((double)(u ? e1 : e0) / sum);
+      sh.p[j] = (float)((double)(u ? e1 : e0) * inv);
       sh.logp[j] = y[u] - hi - ls;
       // an empty slot takes part in nothing
       sh.c[j] = y[u] == -__builtin_inf() ? -1 : cls[u];
     }
   }
   if (lane == 0) {
-    sh.p_rest = (double)er / sum;
+    sh.p_rest = (double)er * inv;
     sh.log_p_rest = yr - hi - ls;
     sh.state = state;
   }
@@ -146,7 +154,7 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
     // The first wave works out the teacher's shares, which nobody needs before the end, while the others begin; only
     // the slots' classes are wanted first, for their bits.
     if constexpr (REST) slot_classes<BS>(t, r, K, tid, sh);
-    if (tid < 64) teacher_row(t, r, K, inv_t, tid, sh);
+    if (tid < 64) teacher_row<LONG>(t, r, K, inv_t, tid, sh);
     // running maximum and sum of the classes in no slot (all classes without REST)
     float m = neg_inf(), acc = 0.f;
     const auto absorb = [&](auto& x) {
@@ -253,10 +261,10 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
         double mine = 0.;
 #pragma unroll
         for (int u = 0; u < 2; ++u) if (first[u]) mine += (double)exp2_f((x[u] - ra) * scale);
-        sum = wave_sum(mine) + (m_rest == neg_inf() ? sum_rest : sum_rest * exp2(((double)m_rest - (double)ra) * (double)inv_t * 1.4426950408889634));
+        sum = wave_sum(mine) + (m_rest == neg_inf() ? sum_rest : sum_rest * end_exp2<LONG>(((double)m_rest - (double)ra) * inv_t * 1.4426950408889634));
       }
       const double m_d = m_all == neg_inf() ? 0. : (double)m_all;
-      const double ls = log(sum);             // log q = (x - m)/T - ls: the large part cancels first
+      const double ls = end_log<LONG>(sum);   // log q = (x - m)/T - ls: the large part cancels first
       double kl = 0.;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -275,13 +283,13 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
         if (sh.state == 2) { loss_sum += (double)v; ++count; }
       } else if (tid == 0) {
         const double pr = sh.p_rest;
-        double inv = sum > 0. ? 1. / sum : sum == 0. ? 0. : sum;
+        double inv = sum > 0. ? end_div<LONG>(1., sum) : sum == 0. ? 0. : sum;
         double w = inv;
         if constexpr (REST) {
-          const double log_q_rest = sum_rest == 0. ? -__builtin_inf() : ((double)ref - m_d) * inv_t + log(sum_rest) - ls;
+          const double log_q_rest = sum_rest == 0. ? -__builtin_inf() : ((double)ref - m_d) * inv_t + end_log<LONG>(sum_rest) - ls;
           if (!(pr == 0.)) kl += pr * (sh.log_p_rest - log_q_rest);
           // q = exp((z - m_rest)/T) * w before the teacher's share of the rest is taken off
-          w = m_rest == neg_inf() ? 0. : inv * exp2(((double)m_rest - m_d) * inv_t * 1.4426950408889634) - pr / sum_rest;
+          w = m_rest == neg_inf() ? 0. : inv * end_exp2<LONG>(((double)m_rest - m_d) * inv_t * 1.4426950408889634) - end_div<LONG>(pr, sum_rest);
         }
         const double loss = t2 * kl;
         if (per_row) per_row[r] = (float)loss;
@@ -347,7 +355,7 @@ k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
     RowStats st = not_counted();
     if (!row_masked(t, r)) st = stats[r];
     const bool live = !(st.ref == __builtin_inff() && st.w == 0.f);
-    if (live && tid < 64) teacher_row(t, r, K, inv_t, tid, sh);       // for the listed classes, at the end
+    if (live && tid < 64) teacher_row<LONG>(t, r, K, inv_t, tid, sh);       // for the listed classes, at the end
     const float g = grad_rows ? grad[r] : grad[0] * scal[0];
     const float f = g * temperature;
     const float w = f * st.w;
@@ -383,6 +391,10 @@ k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
 // where the large parts have cancelled before anything is rounded.  Sums over rows are fp64.
 __device__ __forceinline__ float log2_f(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ float rcp_f(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// a sum of shares of numbers in range stays in range where rounding alone would carry it past the largest (a student's mask
+// of the type's lowest value on a listed class); NaN stays
+__device__ __forceinline__ float in_range(float x) { return x > 3.4028235e38f ? 3.4028235e38f : x; }
 
 template <int KT>
 __device__ __forceinline__ float pick_class(const float (&x)[KT], int c) {
@@ -527,12 +539,15 @@ k_distill_few_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
       FewRow<KT, KS> w;
       few_row<T, KT, KS, FULL, REST>(z, s, t, n, v0, lane, scale, inv_t, w);
       float loss = 0.f;
+      bool barred = false;                     // a listed class has probability zero
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
         const float x = pick_class(w.x, w.c[j]);
         const float d = x == neg_inf() ? __builtin_inff() : fmaf(w.off, unit, w.a[j] - (x - w.m));
+        barred = barred || (d == __builtin_inff() && w.p[j] != 0.f);
         loss += w.p[j] == 0.f ? 0.f : w.p[j] * d;
       }
+      loss = barred ? +loss : in_range(loss);
       if constexpr (REST) {
         const float d = w.sum_rest == 0.f ? __builtin_inff() : unit * ((w.a_rest - w.d_rest) + (w.off - log2_f(w.sum_rest)));
         loss += w.p_rest == 0.f ? 0.f : w.p_rest * d;
@@ -582,6 +597,170 @@ k_distill_few_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
         out[c] = w.state == 1 ? +out[c] : fill;
       }
       store_row<T, KT, FULL>(dz + n * d.sN + (v0 + lane) * d.sV, d.sK, s.K, out);
+    }
+  }
+}
+
+// ---- a few dozen classes and many rows: one thread a row (rows.h), with the arithmetic of the few.
+// the teacher of one lane's row: largest value, whether a slot is filled, whether one names no class; f(j, value, class)
+template <typename F>
+__device__ __forceinline__ void each_slot(const Teacher& t, int64_t at, int K, F f) {
+  for (int j = 0; j < t.o.K; ++j) {
+    const int64_t i = at + j * t.o.sK;
+    const float v = slot_value(t, i);
+    const int c = class_at(t.indices, t.index_kind, i);
+    if (v != neg_inf()) f(j, v, c);
+  }
+}
+
+template <typename T, bool UNIT, bool REST>
+__global__ void __launch_bounds__(256)
+k_distill_lane_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
+                   RowStats* __restrict__ stats, float* __restrict__ per_row, double* __restrict__ partial) {
+  __shared__ uint32_t s_bits[REST ? 256 * (LANE_CLASSES / 32 + 1) : 1];       // a row's words, one apart from the next lane's
+  __shared__ double s_red[4];
+  const float unit = temperature * 0.6931471805599453f;
+  const int K = s.K, words = (K + 31) / 32;
+  uint32_t* const bits = s_bits + (REST ? threadIdx.x * (LANE_CLASSES / 32 + 1) : 0);
+  const int64_t NV = s.N * s.V;
+  double loss_sum = 0.;
+  int count = 0;
+  for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < NV; r += (int64_t)gridDim.x * 256) {
+    const T* p = z + row_offset(s, r);
+    const int64_t at = row_offset(t.o, r);
+    float hi = neg_inf();
+    bool any = false, bad = false;
+    if constexpr (REST) for (int i = 0; i < words; ++i) bits[i] = 0;
+    if (!row_masked(t, r)) {
+      each_slot(t, at, K, [&](int, float v, int c) {
+        any = true;
+        hi = fmaxf(hi, v);
+        if (c < 0 || c >= K) bad = true;
+        else if constexpr (REST) bits[c >> 5] |= 1u << (c & 31);
+      });
+    }
+    float loss = 0.f;
+    RowStats st = not_counted();
+    if (any && bad) {
+      loss = __builtin_nanf("");
+      st = RowStats{0.f, loss, 0.f, loss};
+    } else if (any) {
+      LaneSum in = {neg_inf(), 0.f}, left = {neg_inf(), 0.f};                // listed classes, and all others (all, without REST)
+      for (int c = 0; c < K; c += 8) {
+        float x[8];
+        load8<T, UNIT>(p, s.sK, c, K, x);
+        if constexpr (REST) {
+          uint32_t b = (bits[c >> 5] >> (c & 31)) & 255u;
+          if (b) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if ((b >> i) & 1u) {
+                const float xi = x[i];
+                in.add_one(xi, scale);
+                x[i] = neg_inf();
+              }
+            }
+          }
+        }
+        left.add(x, scale);
+      }
+      const float m_all = fmaxf(in.m, left.m), m = m_all == neg_inf() ? 0.f : m_all;
+      const float ref = left.m == neg_inf() ? 0.f : left.m;
+      const float d_rest = left.m == neg_inf() ? 0.f : (left.m - m) * scale, to_m = exp2_f(d_rest);
+      const float sum = fmaf(left.s, to_m, in.m == neg_inf() ? in.s : in.s * exp2_f((in.m - m) * scale));
+      float a_rest = neg_inf(), shift = 0.f;
+      if constexpr (REST) {
+        a_rest = (float)(((double)t.rest[r] - (double)hi * inv_t) * 1.4426950408889634);
+        shift = fmaxf(a_rest, 0.f);
+      }
+      const float e_rest = REST ? exp2_f(a_rest - shift) : 0.f;
+      // the shares are e / (e_all + e_rest): the terms are gathered before their sum is known, a sixteenth of each, so that
+      // sixteen of the largest do not pass the type's range before they are divided
+      float e_all = 0.f, terms = 0.f;
+      each_slot(t, at, K, [&](int, float v, int c) {
+        const float a = v - hi, e = exp2_f(fmaf(a, scale, -shift));
+        const float x = (float)p[(int64_t)c * s.sK];
+        const float d = x == neg_inf() ? __builtin_inff() : a - (x - m);
+        e_all += e;
+        terms += e == 0.f ? 0.f : e * (d * 0.0625f);
+      });
+      static_assert(LANE_SLOTS <= 16, "the terms' scale");
+      const float inv_t_sum = rcp_f(e_all + e_rest), off = log2_f(sum * inv_t_sum) - shift;
+      const float p_rest = e_rest * inv_t_sum;
+      // infinite where a listed class has probability zero, whatever else is added
+      loss = terms == __builtin_inff() ? terms : in_range(16.f * inv_t_sum * fmaf(e_all * off * 0.0625f, unit, terms));
+      if constexpr (REST) {
+        const float d = left.s == 0.f ? __builtin_inff() : unit * ((a_rest - d_rest) + (off - log2_f(left.s)));
+        loss += p_rest == 0.f ? 0.f : p_rest * d;
+      }
+      loss *= temperature;
+      const float inv = sum == 0.f ? 0.f : rcp_f(sum);
+      st = RowStats{ref, left.s == 0.f ? 0.f : to_m * inv - (REST ? p_rest * rcp_f(left.s) : 0.f), m, inv};
+    }
+    if (per_row) per_row[r] = loss;
+    if (stats) stats[r] = st;
+    loss_sum += (double)loss;
+    count += any ? 1 : 0;
+  }
+  if (partial) {
+    loss_sum = block_sum<256>(loss_sum, s_red);
+    const double counted = block_sum<256>((double)count, s_red);
+    if (threadIdx.x == 0) {
+      partial[2 * blockIdx.x] = loss_sum;
+      partial[2 * blockIdx.x + 1] = counted;
+    }
+  }
+}
+
+template <typename T, bool UNIT>
+__global__ void __launch_bounds__(256)
+k_distill_lane_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
+                   const RowStats* __restrict__ stats, const float* __restrict__ scal, const float* __restrict__ grad, int grad_rows,
+                   T* __restrict__ dz, RowShape d) {
+  const int K = s.K;
+  const int64_t NV = s.N * s.V;
+  const float g_all = grad_rows ? 0.f : grad[0] * scal[0];
+  for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < NV; r += (int64_t)gridDim.x * 256) {
+    const T* p = z + row_offset(s, r);
+    T* q = dz + row_offset(d, r);
+    RowStats st = not_counted();
+    if (!row_masked(t, r)) st = stats[r];
+    const bool live = !(st.ref == __builtin_inff() && st.w == 0.f);
+    const float f = temperature * (grad_rows ? grad[r] : g_all), w = f * st.w;
+    for (int c = 0; c < K; c += 8) {
+      float x[8];
+      load8<T, UNIT>(p, s.sK, c, K, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = live ? exp2_f((x[i] - st.ref) * scale) * w : 0.f;
+      if (UNIT && c + 8 <= K) {
+        if constexpr (sizeof(T) == 2) store_vec<false>(q + c, x);
+        else {
+          store_vec<false>(q + c, *(const float(*)[4])x);
+          store_vec<false>(q + c + 4, *(const float(*)[4])(x + 4));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) if (c + i < K) q[(int64_t)(c + i) * d.sK] = (T)x[i];
+      }
+    }
+    if (live && !(st.w != st.w && st.inv_s != st.inv_s)) {           // a NaN row is NaN as it stands
+      const int64_t at = row_offset(t.o, r);
+      float hi = neg_inf(), shift = 0.f, sum = 0.f;
+      each_slot(t, at, K, [&](int, float v, int) { hi = fmaxf(hi, v); });
+      if (t.rest) {
+        const float a_rest = (float)(((double)t.rest[r] - (double)hi * inv_t) * 1.4426950408889634);
+        shift = fmaxf(a_rest, 0.f);
+        sum = exp2_f(a_rest - shift);
+      }
+      each_slot(t, at, K, [&](int, float v, int) { sum += exp2_f(fmaf(v - hi, scale, -shift)); });
+      const float inv_sum = rcp_f(sum);
+      each_slot(t, at, K, [&](int, float, int c) {
+        float share = 0.f;
+        each_slot(t, at, K, [&](int, float v, int c2) { share += c2 == c ? exp2_f(fmaf(v - hi, scale, -shift)) : 0.f; });
+        const float x = (float)p[(int64_t)c * s.sK];
+        const float qc = x == neg_inf() ? 0.f : exp2_f((x - st.m) * scale) * st.inv_s;
+        q[(int64_t)c * d.sK] = (T)(f * (qc - share * inv_sum));
+      });
     }
   }
 }
@@ -665,6 +844,15 @@ int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* 
 #define LAUNCH_FEW(KT, KS, FULL, REST) hipLaunchKernelGGL((k_distill_few_fwd<T, KT, KS, FULL, REST>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, per_row, part)
     DISTILL_DISPATCH_FEW(LAUNCH_FEW);
 #undef LAUNCH_FEW
+  } else if (lane_rows(a->N * a->V, a->K, a->k)) {
+    const int64_t blocks = cdiv(a->N * a->V, 256);
+    parts = blocks < DIS_MAX_BLOCKS ? blocks : DIS_MAX_BLOCKS;
+#define LAUNCH_LANE(UNIT, REST) hipLaunchKernelGGL((k_distill_lane_fwd<T, UNIT, REST>), dim3((unsigned)parts), dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, (RowStats*)stats, per_row, part)
+    DEVIS_DISPATCH_DTYPE(a->dtype, {
+      if (unit) { if (a->rest) LAUNCH_LANE(true, true); else LAUNCH_LANE(true, false); }
+      else { if (a->rest) LAUNCH_LANE(false, true); else LAUNCH_LANE(false, false); }
+    });
+#undef LAUNCH_LANE
   } else {
 #define LAUNCH_DISTILL_FWD(UNIT, REST, BS) hipLaunchKernelGGL((k_distill_fwd<T, UNIT, REST, BS>), rows, dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, t2, (RowStats*)stats, per_row, part)
     DISTILL_DISPATCH(LAUNCH_DISTILL_FWD);
@@ -699,6 +887,14 @@ int devis_distill_bwd(const devis_distill_params* a, const void* logits, const v
     return launch_status();
   }
   const dim3 rows = distill_grid(a);
+  if (lane_rows(a->N * a->V, a->K, a->k)) {
+    const int64_t blocks = cdiv(a->N * a->V, 256);
+    const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192));
+#define LAUNCH_LANE(UNIT) hipLaunchKernelGGL((k_distill_lane_bwd<T, UNIT>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, (const RowStats*)stats, scal, grad, grad_rows, (T*)dlogits, d)
+    DEVIS_DISPATCH_DTYPE(a->dtype, { if (unit) LAUNCH_LANE(true); else LAUNCH_LANE(false); });
+#undef LAUNCH_LANE
+    return launch_status();
+  }
   const bool past = (double)(a->N * a->V) * (double)a->K * (a->dtype == DEVIS_F32 ? 4 : 2) >= DIS_PAST_BYTES;
 #define LAUNCH_DISTILL_BWD(UNIT, PAST, BS) hipLaunchKernelGGL((k_distill_bwd<T, UNIT, PAST, BS>), rows, dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, (const RowStats*)stats, scal, grad, grad_rows, (T*)dlogits, d)
   DEVIS_DISPATCH_DTYPE(a->dtype, {

@@ -388,6 +388,59 @@ k_top_few(const T* __restrict__ z, RowShape s, int k, float scale, float inv_t, 
   }
 }
 
+// A few dozen classes and many rows (rows.h): a thread a row, the KS >= k largest keys so far in registers, in order.  Each
+// class that comes leaves one loser, itself or the last of the list, for the rest.
+template <typename T, typename I, bool UNIT, int KS>
+__global__ void __launch_bounds__(256)
+k_top_lane(const T* __restrict__ z, RowShape s, int k, float scale, float inv_t, T* __restrict__ values, I* __restrict__ indices,
+           RowShape o, float* __restrict__ rest) {
+  const int K = s.K;
+  const int64_t NV = s.N * s.V;
+  const auto value = [](uint32_t key) { return key ? key_value((uint64_t)key << 32) : neg_inf(); };
+  for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < NV; r += (int64_t)gridDim.x * 256) {
+    const T* p = z + row_offset(s, r);
+    uint32_t top[KS];                          // ordered integers of the values, 0: none yet
+    int at[KS];
+#pragma unroll
+    for (int j = 0; j < KS; ++j) top[j] = at[j] = 0;
+    LaneSum left = {neg_inf(), 0.f};
+    for (int c0 = 0; c0 < K; c0 += 8) {
+      float x[8];
+      load8<T, UNIT>(p, s.sK, c0, K, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t key = c0 + i < K ? (uint32_t)(top_key(nan_high(x[i]), 0) >> 32) : 0;
+        uint32_t loser = key;
+        if (key > top[KS - 1]) {
+          loser = top[KS - 1];
+#pragma unroll
+          for (int j = KS - 1; j > 0; --j) {
+            const bool past = key > top[j - 1], here = key > top[j];         // strict: the lower class stays in front
+            at[j] = past ? +at[j - 1] : here ? c0 + i : +at[j];
+            top[j] = past ? +top[j - 1] : here ? key : +top[j];
+          }
+          at[0] = key > top[0] ? c0 + i : +at[0];
+          top[0] = key > top[0] ? key : +top[0];
+        }
+        x[i] = value(loser);
+      }
+      left.add(x, scale);
+    }
+    const int64_t out = row_offset(o, r);
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+      if (j < k) {
+        values[out + j * o.sK] = p[(int64_t)at[j] * s.sK];
+        indices[out + j * o.sK] = (I)at[j];
+      } else if (top[j]) {
+        left.add_one(value(top[j]), scale);
+      }
+    }
+    // nothing left (-inf), or infinities are: the maximum is the answer
+    if (rest) rest[r] = fabsf(left.m) < __builtin_inff() ? fmaf(left.m, inv_t, __logf(left.s)) : left.m;
+  }
+}
+
 }  // namespace devis
 
 using namespace devis;
@@ -412,6 +465,19 @@ extern "C" int devis_top_logits(const void* logits, int64_t sN, int64_t sV, int6
       else { typedef int32_t I; DEVIS_DISPATCH_FEW(K, sK == 1, LAUNCH_FEW); }
     });
 #undef LAUNCH_FEW
+    return launch_status();
+  }
+  if (lane_rows(NV, K, k)) {
+    const int64_t tiles = cdiv(NV, 256);
+    const dim3 grid((unsigned)(tiles < 8192 ? tiles : 8192));
+#define LAUNCH_LANE(UNIT, KS) hipLaunchKernelGGL((k_top_lane<T, I, UNIT, KS>), grid, dim3(256), 0, st, (const T*)logits, s, (int)k, scale, (float)inv_t, (T*)values, (I*)indices, o, rest)
+#define LAUNCH_LANE_U(KS) do { if (sK == 1) LAUNCH_LANE(true, KS); else LAUNCH_LANE(false, KS); } while (0)
+    DEVIS_DISPATCH_DTYPE(dtype, {
+      if (index_dtype == DEVIS_LABEL_U8) { typedef uint8_t I; if (k <= 4) LAUNCH_LANE_U(4); else LAUNCH_LANE_U(16); }
+      else { typedef int32_t I; if (k <= 4) LAUNCH_LANE_U(4); else LAUNCH_LANE_U(16); }
+    });
+#undef LAUNCH_LANE_U
+#undef LAUNCH_LANE
     return launch_status();
   }
 #define LAUNCH_TOP(I, UNIT, BS) hipLaunchKernelGGL((k_top_rows<T, I, UNIT, BS>), row_grid(NV), dim3(BS), 0, st, (const T*)logits, s, (int)k, scale, inv_t, (T*)values, (I*)indices, o, rest)

@@ -39,10 +39,14 @@ def logits(rows, K, dtype, seed, spread=3.0):
 
 
 # ------------------------------------------------------------------ top logits
-def check_top(z, k, T=1.0, channels_last=True, device_z=None):
-    """z (rows, K) on the CPU as the oracle sees it; device_z the tensor given to the call (default z)."""
+def check_top(z, k, T=1.0, channels_last=True, device_z=None, times=1):
+    """z (rows, K) on the CPU as the oracle sees it; device_z the tensor given to the call (default z, `times` over)."""
     from devis_amd import ops
-    out = ops.top_logits(z.cuda() if device_z is None else device_z, k, channels_last=channels_last, temperature=T)
+    out = ops.top_logits(torch.cat([z] * times).cuda() if device_z is None else device_z, k, channels_last=channels_last, temperature=T)
+    if times > 1:
+        for n in out:
+            assert torch.equal(out[n].reshape(times, -1).nan_to_num(7.25), out[n].reshape(times, -1)[:1].expand(times, -1).nan_to_num(7.25))
+            out[n] = out[n][:z.shape[0]]
     vals, idx, rest = out["values"], out["indices"], out["rest"]
     K = z.shape[1]
     assert vals.dtype == z.dtype and idx.dtype == (torch.uint8 if K <= 256 else torch.int32) and rest.dtype == torch.float32
@@ -70,8 +74,8 @@ def test_top_sizes(K, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("K", [5, 100, 3001])
-def test_top_ties_masks_and_infinities(K, dtype):
+@pytest.mark.parametrize("K, times", [(5, 1), (100, 1), (3001, 1), (30, 700)])
+def test_top_ties_masks_and_infinities(K, times, dtype):
     inf, low = math.inf, torch.finfo(dtype).min
     rows = [torch.zeros(K),                                         # every class alike: the lowest classes
             torch.arange(K).float() // 7,                           # rising plateaus
@@ -87,7 +91,7 @@ def test_top_ties_masks_and_infinities(K, dtype):
             torch.where(torch.arange(K) < 3, 300.0, -torch.arange(K) / K)]      # the rest far below the listed
     z = torch.stack([r.expand(K).float() for r in rows]).to(dtype)
     for k in (1, 3, 5):
-        check_top(z, k)
+        check_top(z, k, times=times)
 
 
 def test_top_all_infinite_rows():
@@ -143,16 +147,26 @@ def test_top_without_rest_and_without_rows():
     assert e["values"].shape == (0, 4) and e["rest"].shape == (0,)
 
 
-def test_top_many_rows():
-    """More rows than blocks run at once; a sample of them against the oracle, all of them against sorting."""
+@pytest.mark.parametrize("first", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K, k", [(5, 3), (17, 1), (37, 4), (64, 5), (100, 16), (256, 7), (300, 6), (37, 20)])
+def test_top_many_rows(K, k, dtype, first):
+    """More rows than blocks run at once, all of them against sorting; bf16 rows hold many ties."""
     from devis_amd import ops
     g = torch.Generator(device="cuda").manual_seed(2)
-    z = torch.randn((70000, 37), generator=g, device="cuda")
-    out = ops.top_logits(z, 6)
+    z = torch.randn((9, 8001, K), generator=g, device="cuda").to(dtype)
+    z[0, :, K // 2:] = -math.inf
+    z[1, :, 3:] = 1.0
+    z[2] = z[2].float().round().to(dtype)
+    z[3, :, ::3] = torch.finfo(dtype).min
     order = torch.sort(z, dim=-1, descending=True, stable=True)
-    assert torch.equal(out["indices"].long(), order[1][:, :6]) and torch.equal(out["values"], order[0][:, :6])
-    want = torch.logsumexp(order[0][:, 6:].double(), -1)
-    assert (out["rest"].double() - want).abs().max().item() < (3 * 12 + 13) * E + 8 * E
+    want = torch.logsumexp(order[0][..., k:].double(), -1)
+    out = ops.top_logits(z.movedim(-1, 1).contiguous() if first else z, k, channels_last=not first)
+    vals, idx = (x.movedim(1, -1) if first else x for x in (out["values"], out["indices"]))
+    assert torch.equal(idx.long(), order[1][..., :k]) and torch.equal(vals, order[0][..., :k])
+    off = (out["rest"].double() - want).abs()
+    off = torch.where(out["rest"].double() == want, torch.zeros_like(off), off)
+    assert (off / (1 + want.abs())).max().item() < (3 * 12 + K / 64 + 13) * E
 
 
 # ------------------------------------------------------------------ distillation
@@ -180,11 +194,14 @@ def oracle_rows(z, v, i, rest, mask, T):
     return loss, grad, counted, scale, err
 
 
-def check_distill(z, v, i, rest=None, mask=None, T=1.0, reduction="mean", layout=None, g=0.7):
-    """z (rows, K), v, i (rows, k) on the CPU.  `layout`: (rows, c) CPU tensor -> what the call takes, channels_last."""
+def check_distill(z, v, i, rest=None, mask=None, T=1.0, reduction="mean", layout=None, g=0.7, times=1):
+    """z (rows, K), v, i (rows, k) on the CPU.  `layout`: (rows, c) CPU tensor -> what the call takes, channels_last.
+    `times`: the rows are given that often, one lot behind the other."""
     from devis_amd import criterions
     last, put = (True, lambda x: x) if layout is None else layout
-    loss, grad, counted, scale, err = oracle_rows(z, v, i, rest, mask, T)
+    out = oracle_rows(z, v, i, rest, mask, T)
+    loss, grad, counted, scale, err = (np.concatenate([x] * times) for x in out)
+    z, v, i, rest, mask = (None if x is None else torch.cat([x] * times) for x in (z, v, i, rest, mask))
     zd = put(z).cuda().detach().requires_grad_(True)
     one = lambda x: None if x is None else put(x[:, None]).select(-1 if last else 1, 0).cuda()
     got = criterions.distill_top_loss(zd, put(v).cuda(), put(i).cuda(), one(rest), last, T, one(mask), reduction)
@@ -202,15 +219,21 @@ def check_distill(z, v, i, rest=None, mask=None, T=1.0, reduction="mean", layout
         dz = torch.autograd.grad(got, zd, torch.tensor(g, device="cuda"))[0]
         want = loss.sum() / (n if reduction == "mean" else 1)
         tol = err.sum() / (n if reduction == "mean" else 1) + E * abs(want)
-        assert np.isnan(want) and math.isnan(got.item()) or abs(got.item() - want) <= tol or got.item() == want, (got.item(), want, tol)
+        with np.errstate(over="ignore"):
+            rounded = float(np.float32(want))          # the loss is fp32: a sum past 3.4e38 is infinite
+        assert np.isnan(want) and math.isnan(got.item()) or abs(got.item() - want) <= tol or got.item() == rounded, (got.item(), want, tol)
         f = np.full((z.shape[0], 1), float(np.float32(g)) / (n if reduction == "mean" else 1))
     assert dz.dtype == z.dtype and dz.shape == zd.shape
     d = (dz if last else dz.movedim(1, -1)).reshape(z.shape).cpu().double().numpy()
     want = grad * f
     listed = [np.unique(a[(b > -np.inf).numpy() & (a >= 0).numpy() & (a < z.shape[1]).numpy()].numpy()) for a, b in zip(i.long(), v)]
+    sums = {}
     for r in range(z.shape[0]):
         # q, the shares and the factor of the row: a sum, an exponential and four roundings each; then the type's
-        tol = np.abs(f[r]) * scale[r] * (2 * sum_error(z[r].double().numpy(), T, listed[r]) + 8 * E) + HALF[z.dtype] * np.abs(want[r]) + 1e-37
+        n = r % (z.shape[0] // times)
+        if n not in sums:
+            sums[n] = 2 * sum_error(z[r].double().numpy(), T, listed[r]) + 8 * E
+        tol = np.abs(f[r]) * scale[r] * sums[n] + HALF[z.dtype] * np.abs(want[r]) + 1e-37
         if np.isnan(loss[r]):
             assert np.isnan(d[r]).all()
         else:
@@ -256,15 +279,27 @@ def test_distill_types_masks_reductions(itype, reduction):
 
 @pytest.mark.parametrize("K", [6, 40, 3000])
 def test_distill_empty_slots_masked_classes_and_bad_rows(K):
+    z, v, i, r, r8, ok = odd_rows(K, torch.float32)
+    for rest in (None, r8):
+        check_distill(z, v, i, rest, None, 1.0, "none")
+    check_distill(z, v, i, r8, ok, 1.0, "mean")
+    # masked rows may hold anything
+    z[6], v[7], i[8] = math.nan, math.nan, 2 ** 30
+    check_distill(z, v, i, r8, ok, 1.0, "mean")
+
+
+def odd_rows(K, dtype):
+    """Fourteen rows of what can go wrong, and which of them have finite losses."""
     inf = math.inf
-    z, v, i, r = pair(14, K, 4, 1.0, torch.float32, K)
+    z, v, i, r = pair(14, K, 4, 1.0, dtype, K)
+    low = torch.finfo(dtype).min
     v[1, 2:] = -inf                                # a short list
     v[2] = -inf                                    # no list: not counted
     i[2] = 2 ** 30
     i[1, 3] = -5                                   # an empty slot's class is not looked at
     v[3, 0] = -inf                                 # an empty slot in front
-    z[4, :] = torch.finfo(torch.float32).min       # the student's mask: the lowest value everywhere
-    z[5, 1:] = torch.finfo(torch.float32).min
+    z[4, :] = low                                  # the student's mask: the lowest value everywhere
+    z[5, 1:] = low
     z[6, i[6].long()] = -inf                       # listed classes the student may not use: infinite loss, finite gradient
     z[7, :] = -inf
     keep = torch.zeros(K, dtype=torch.bool)
@@ -276,16 +311,30 @@ def test_distill_empty_slots_masked_classes_and_bad_rows(K):
     z[11, i[11].long()] += 200.0                   # the rest far below
     z[12, i[12].long()] -= 200.0                   # the list far below
     r[13] = -inf                                   # no rest in this row
-    r8 = r.clone()
-    for rest in (None, r8):
-        for reduction in ("none",):
-            check_distill(z, v, i, rest, None, 1.0, reduction)
     ok = torch.ones(14, dtype=torch.bool)
     ok[6] = ok[7] = ok[8] = False
-    check_distill(z, v, i, r8, ok, 1.0, "mean")
-    # masked rows may hold anything
+    return z, v, i, r, r.clone(), ok
+
+
+LANES = 586                                        # 14 rows 586 times: enough rows for one thread each
+
+
+@pytest.mark.parametrize("first", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K", [17, 31, 64, 100, 256])
+def test_distill_many_rows_of_some_classes(K, dtype, first):
+    layout = (False, lambda x: x.view(14, -1, x.shape[1]).movedim(-1, 1).contiguous()) if first else None
+    z, v, i, r, r8, ok = odd_rows(K, dtype)
+    for rest in (None, r8):
+        check_distill(z, v, i, rest, None, 1.0, "none", layout, times=LANES)
+    check_distill(z, v, i, r8, ok, 1.0, "mean", layout, times=LANES)
     z[6], v[7], i[8] = math.nan, math.nan, 2 ** 30
-    check_distill(z, v, i, r8, ok, 1.0, "mean")
+    check_distill(z, v, i, r8, ok, 1.0, "sum", layout, times=LANES)
+    i[9, 1], i[10, 3] = K, -1                      # filled slots that name no class
+    check_distill(z, v, i, r8, ok, 1.0, "none", layout, times=LANES)
+    for k, T in ((1, 3.0), (16, 2.0)):
+        z, v, i, r = pair(14, K, k, T, dtype, K, torch.int64)
+        check_distill(z, v, i, r, None, T, "none", layout, times=LANES)
 
 
 @pytest.mark.parametrize("K", [5, 3000])
