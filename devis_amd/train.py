@@ -65,6 +65,13 @@ def getArgs(argv=None):
     p.add_argument('--synthetic_val', type=int, default=1)
     p.add_argument('--seed', type=int, default=1234, help='data seed; rank r draws from seed + r')
     p.add_argument('--backend', default='nccl', choices=['nccl', 'gloo'], help='torch.distributed backend under torchrun')
+    # not in the reference: learn from a teacher's largest class logits as well (criterions.distill_top_loss).  --teacher is a
+    # checkpoint as val() writes it, of a model of --teacher_model (default: --model_name) for the same dataset
+    p.add_argument('--teacher', default='', type=str)
+    p.add_argument('--teacher_model', default='', type=str)
+    p.add_argument('--distill_top', type=int, default=2, help='logits kept of every voxel')
+    p.add_argument('--distill_temperature', type=float, default=2.0)
+    p.add_argument('--distill_weight', type=float, default=1.0)
     args = p.parse_args(argv)
     args.compute_dtype = torch.bfloat16 if args.compute_dtype == 'bf16' else torch.float32
     apply_dataset_overrides(args)
@@ -172,9 +179,28 @@ class LossMeter:
         return float(self.total.item() / self.count) if self.count else 0.0
 
 
-def train(args, model, optimizer, epoch, train_loader, reducer=None, log=print):
+def load_teacher(args):
+    """The TMSU of `--teacher`, in eval mode and without gradients (None without the flag)."""
+    path = getattr(args, 'teacher', '')
+    if not path:
+        return None
+    from . import TMSU
+    if not 1 <= args.distill_top <= args.num_classes:
+        raise ValueError("--distill_top must be in [1, %d] on %s, got %d" % (args.num_classes, args.dataset, args.distill_top))
+    if not (args.distill_weight >= 0 and args.distill_temperature > 0):
+        raise ValueError("--distill_weight must not be negative and --distill_temperature must be positive")
+    checkpoint = torch.load(path, map_location='cpu', weights_only=True)
+    own = argparse.Namespace(**vars(args))
+    own.model_name = args.teacher_model or args.model_name
+    teacher = TMSU(own)
+    teacher.load_state_dict(checkpoint['state_dict'])
+    teacher.cuda()
+    return teacher.eval().requires_grad_(False)
+
+
+def train(args, model, optimizer, epoch, train_loader, reducer=None, log=print, teacher=None):
     """One epoch; same order of operations as trainUMIS.py:239-263.  `reducer` (devis_amd.parallel)
-    averages gradients across ranks.  The per-iteration loss lines are kept, in order, but are printed
+    averages gradients across ranks; `teacher` (`load_teacher`) adds the distillation term of `--distill_*`.  The per-iteration loss lines are kept, in order, but are printed
     through LossMeter: the launch thread never waits for the GPU inside the loop."""
     model.train()
     meter = LossMeter(log)
@@ -187,7 +213,12 @@ def train(args, model, optimizer, epoch, train_loader, reducer=None, log=print):
         x = x.cuda(non_blocking=True)
         target = target.cuda(non_blocking=True)
         args.mode = 'train'
-        evidences, loss = model(x, target, epoch, args.mode, args.dataset)
+        if teacher is None:
+            evidences, loss = model(x, target, epoch, args.mode, args.dataset)
+        else:
+            top = teacher.top_logits(x, args.distill_top, args.distill_temperature)
+            evidences, loss = model(x, target, epoch, args.mode, args.dataset,
+                                    distill=(top, args.distill_temperature, args.distill_weight))
         optimizer.zero_grad()
         loss.requires_grad_(True).backward()
         if reducer is not None:
@@ -499,6 +530,7 @@ def run(args, loaders=None, log=print):
         get = lambda a, salt=0: loaders
     train_loader, valid_loader, test_loader = get(args)
     model, optimizer, reducer = build(args, rank)
+    teacher = load_teacher(args)
     out = dict(loss_list=[], dice_list=[], best_dice=0, test=None)
     best_dice = 0
     if mode in ('train&test', 'train'):
@@ -506,7 +538,7 @@ def run(args, loaders=None, log=print):
         for epoch in range(first, args.end_epochs + 1):
             say('===========Train begining!===========')
             say('Epoch {}/{}'.format(epoch, args.end_epochs - 1))
-            epoch_loss = train(args, model, optimizer, epoch, train_loader, reducer=reducer, log=say)
+            epoch_loss = train(args, model, optimizer, epoch, train_loader, reducer=reducer, log=say, teacher=teacher)
             say("epoch %d avg_loss:%0.3f" % (epoch, epoch_loss))
             _, best_dice = val(args, model, epoch, best_dice, valid_loader)
             out['loss_list'].append(epoch_loss)

@@ -14,7 +14,7 @@ import torch
 import torch.nn as nn
 
 from . import ops
-from .criterions import evidential_head_loss
+from .criterions import distill_top_loss, evidential_head_loss
 from .predict import tailor_and_concat
 from .unet2d import Unet2D, Unet2DDRIVE
 from .unet3d import Unet
@@ -79,19 +79,36 @@ class TMSU(nn.Module):
         self.total_epochs = args.end_epochs + 1
         self.u_loss = args.Uncertainty_Loss
 
-    def forward(self, X, y, global_step, mode, dataset):
+    def forward(self, X, y, global_step, mode, dataset, distill=None):
+        """`distill` (train mode; not in the reference): (a teacher's `top_logits(X, k, temperature)`, temperature,
+        weight) adds weight * distill_top_loss of this model's logits."""
         if mode == 'train':
             logits = self.backbone.forward_channels_last(X)
             evidence, loss = evidential_head_loss(logits, _labels(y), global_step, self.lambda_epochs,
                                                   channels_last=True, want_evidence=True, u_loss=bool(self.u_loss),
                                                   total_step=self.total_epochs, eps=self.eps,
                                                   disentangle=self.disentangle)
+            if distill is not None:
+                top, temperature, weight = distill
+                loss = loss + weight * distill_top_loss(logits, top["values"], top["indices"], top["rest"],
+                                                        channels_last=True, temperature=temperature)
             return evidence, loss
         if dataset == 'BraTS':
             out = tailor_and_concat(X, self.backbone)
         else:
             out = self.backbone(X)
         return self.infer(out)
+
+    def top_logits(self, X, k, temperature=1.0):
+        """This model as a teacher: the k largest logits of every voxel of X and the mass of the others
+        (`ops.top_logits`), channels last.  Runs in eval mode without gradients."""
+        training = self.training
+        self.eval()
+        try:
+            with torch.no_grad():
+                return ops.top_logits(self.backbone.forward_channels_last(X), k, channels_last=True, temperature=temperature)
+        finally:
+            self.train(training)
 
     def infer(self, input):
         """softplus evidence of NC(D)HW logits (TrustworthySeg.py:160-166)."""
