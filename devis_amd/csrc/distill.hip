@@ -12,6 +12,8 @@
 // factor of the row, W = 1/s - p_rest/s_rest; the k listed classes are put right afterwards.
 #include "rows.h"
 
+#include <type_traits>
+
 namespace devis {
 
 constexpr int DIS_MAX_K = DEVIS_TOP_MAX_K;
@@ -28,7 +30,7 @@ struct RowStats { float ref, w, m, inv_s; };  // gradient of a class in no slot:
 
 // The ends of a row: fp64 for long rows; for the short ones of a wave each, fp32 (there are many, and fp64 logarithms,
 // exponentials and quotients would cost more than the row).
-template <bool LONG> __device__ __forceinline__ double end_log(double x) { return LONG ? log(x) : 0.6931471805599453 * (double)__builtin_amdgcn_logf((float)x); }
+template <bool LONG> __device__ __forceinline__ double end_log(double x) { return LONG || !(x > 0.) ? log(x) : 0.6931471805599453 * log2_split(x); }
 template <bool LONG> __device__ __forceinline__ double end_exp2(double x) { return LONG ? exp2(x) : (double)exp2_f((float)x); }
 template <bool LONG> __device__ __forceinline__ double end_div(double a, double b) { return LONG ? a / b : a * (double)(1.f / (float)b); }
 
@@ -395,6 +397,7 @@ __device__ __forceinline__ float rcp_f(float x) { return __builtin_amdgcn_rcpf(x
 // a sum of shares of numbers in range stays in range where rounding alone would carry it past the largest (a student's mask
 // of the type's lowest value on a listed class); NaN stays
 __device__ __forceinline__ float in_range(float x) { return x > 3.4028235e38f ? 3.4028235e38f : x; }
+__device__ __forceinline__ double in_range(double x) { return x; }
 
 template <int KT>
 __device__ __forceinline__ float pick_class(const float (&x)[KT], int c) {
@@ -407,25 +410,41 @@ __device__ __forceinline__ float pick_class(const float (&x)[KT], int c) {
   return v;
 }
 
-// KS bounds the slots as KT bounds the classes.
-template <int KT, int KS> struct FewRow {
-  float x[KT], e[KT];          // logits; exponentials, of a class in a slot against the row's maximum, else against m_rest
-  float a[KS], p[KS];          // slots: logit below the largest, share
+// What few_row works out.  A row's own loss is what is left when logarithms cancel (a student near its teacher at a high
+// temperature: 0.02 of numbers near 1), so for it everything is fp64; in a mean over many rows the roundings of fp32
+// average out, and in the gradient they stay at the shares' own size.  8 x 64^3 voxels of 9 classes at temperature 4: the
+// rows' losses are off by 2.4e-6 relative in fp32.
+enum { FEW_GRADIENT, FEW_MEAN_LOSS, FEW_ROW_LOSS };
+
+// KS bounds the slots as KT bounds the classes; S is the type of shares and sums.
+template <int KT, int KS, typename S> struct FewRow {
+  float x[KT], a[KS];          // logits; slots: logit below the largest
+  S e[KT], p[KS];              // exponentials, of a class in a slot against the row's maximum, else against m_rest; shares
   int c[KS];
   unsigned listed;
   int state;                   // as SlotShared::state
-  float m, sum, inv;           // student: maximum, sum of exponentials against it, 1 / sum
-  float sum_rest, to_m;        // classes in no slot: sum against m_rest, exp((m_rest - m)/T)
-  float d_rest, a_rest, p_rest;
-  float off;                   // log2(S_student / S_teacher), both against their own maxima
+  float m;                     // student: maximum, sum of exponentials against it, 1 / sum
+  S sum, inv;
+  S sum_rest, to_m;            // classes in no slot: sum against m_rest, exp((m_rest - m)/T)
+  S p_rest;
+  S off;                       // with a loss: log2(S_student / S_teacher), both against their own maxima
+  S off_rest;                  // with a loss: log2(p_rest / q_rest)
 };
+
+__device__ __forceinline__ float few_exp(float x, float ref, float scale, double) { return exp2_f((x - ref) * scale); }
+__device__ __forceinline__ double few_exp(double x, double ref, float, double scale) { return exp2_series((x - ref) * scale); }
+__device__ __forceinline__ float few_log(float x) { return log2_f(x); }
+__device__ __forceinline__ double few_log(double x) { return log2_newton(x); }
+__device__ __forceinline__ float few_rcp(float x) { return rcp_f(x); }
+__device__ __forceinline__ double few_rcp(double x) { return 1. / x; }
 
 // Row (n, v0 + lane) with n and v0 the block's.  Straight-line: a row that is not counted is worked out all the same and
 // dropped at the end.
-template <typename T, int KT, int KS, bool FULL, bool REST>
+template <typename T, int KT, int KS, bool FULL, bool REST, int WANT, typename S>
 __device__ __forceinline__ void few_row(const T* __restrict__ z, const RowShape& s, const Teacher& t, int64_t n, int64_t v0,
-                                        uint32_t lane, float scale, double inv_t, FewRow<KT, KS>& w) {
+                                        uint32_t lane, float scale, double inv_t, FewRow<KT, KS, S>& w) {
   const int K = s.K, k = t.o.K;
+  const double scale_d = inv_t * 1.4426950408889634;
   const int64_t r0 = n * s.V + v0, at = n * t.o.sN + v0 * t.o.sV;
   const uint32_t slot = lane * (uint32_t)t.o.sV;
   // every load first, raw: nothing is looked at before all of them are on their way.  Slots behind the last read the last.
@@ -473,61 +492,64 @@ __device__ __forceinline__ void few_row(const T* __restrict__ z, const RowShape&
   w.listed &= (1u << FEW_CLASSES) - 1;
   w.state = w.listed == 0 || keep == 0 ? 0 : bad ? 2 : 1;
   // teacher, in base 2 against its largest logarithm
-  w.a_rest = neg_inf();
-  float shift = 0.f;
+  double a_rest = -__builtin_inf();
+  S shift = 0;
   if constexpr (REST) {
-    w.a_rest = (float)(((double)rest - (double)hi * inv_t) * 1.4426950408889634);
-    shift = fmaxf(w.a_rest, 0.f);
+    a_rest = (double)rest * 1.4426950408889634 - (double)hi * scale_d;
+    shift = (S)fmax(a_rest, 0.);
   }
-  w.p_rest = REST ? exp2_f(w.a_rest - shift) : 0.f;
-  float sum_t = w.p_rest;
+  w.p_rest = REST ? few_exp((S)a_rest, shift, 1.f, 1.) : (S)0;
+  S sum_t = w.p_rest;
 #pragma unroll
   for (int j = 0; j < KS; ++j) {
     w.a[j] -= hi;
-    w.p[j] = exp2_f(fmaf(w.a[j], scale, -shift));
-    w.p[j] = w.c[j] == FEW_CLASSES ? 0.f : +w.p[j];
+    w.p[j] = REST ? few_exp((S)w.a[j] * (S)scale_d, shift, 1.f, 1.) : few_exp((S)w.a[j], (S)0, scale, scale_d);
+    w.p[j] = w.c[j] == FEW_CLASSES ? (S)0 : +w.p[j];
     sum_t += w.p[j];
   }
-  const float inv_sum_t = rcp_f(sum_t);
+  const S inv_sum_t = few_rcp(sum_t);
 #pragma unroll
   for (int j = 0; j < KS; ++j) w.p[j] *= inv_sum_t;
   w.p_rest *= inv_sum_t;
   // student
   w.m = max_of(w.x);
   w.m = w.m == neg_inf() ? 0.f : +w.m;
+  float m_rest = neg_inf();
+  w.sum = w.sum_rest = w.to_m = 0;
   if constexpr (REST) {
-    float m_rest = neg_inf();
 #pragma unroll
     for (int c = 0; c < KT; ++c) m_rest = fmaxf(m_rest, (w.listed >> c) & 1u ? neg_inf() : +w.x[c]);
-    const bool none = m_rest == neg_inf();
-    w.d_rest = none ? 0.f : (m_rest - w.m) * scale;
-    const float ref = none ? 0.f : m_rest;
-    w.to_m = exp2_f(w.d_rest);
-    float in = 0.f;
-    w.sum_rest = 0.f;
+    m_rest = m_rest == neg_inf() ? +w.m : m_rest;
+    w.to_m = few_exp((S)m_rest, (S)w.m, scale, scale_d);
 #pragma unroll
     for (int c = 0; c < KT; ++c) {
       const bool l = (w.listed >> c) & 1u;
-      w.e[c] = exp2_f((w.x[c] - (l ? +w.m : ref)) * scale);
-      in += l ? +w.e[c] : 0.f;
-      w.sum_rest += l ? 0.f : +w.e[c];
+      w.e[c] = few_exp((S)w.x[c], (S)(l ? +w.m : m_rest), scale, scale_d);
+      w.sum += l ? +w.e[c] : (S)0;
+      w.sum_rest += l ? (S)0 : +w.e[c];
     }
-    w.sum = fmaf(w.sum_rest, w.to_m, in);
+    w.sum += w.sum_rest * w.to_m;
   } else {
 #pragma unroll
-    for (int c = 0; c < KT; ++c) w.e[c] = exp2_f((w.x[c] - w.m) * scale);
+    for (int c = 0; c < KT; ++c) w.e[c] = few_exp((S)w.x[c], (S)w.m, scale, scale_d);
     w.sum = sum_of(w.e);
   }
-  w.inv = w.sum == 0.f ? 0.f : rcp_f(w.sum);
-  w.off = log2_f(w.sum * inv_sum_t) - shift;
+  if constexpr (WANT == FEW_GRADIENT) {
+    w.inv = w.sum == (S)0 ? (S)0 : few_rcp(w.sum);
+  } else {
+    if constexpr (WANT == FEW_ROW_LOSS) w.off = few_log(w.sum) - few_log(sum_t) - shift;
+    else w.off = few_log(w.sum * inv_sum_t) - shift;
+    if constexpr (REST) w.off_rest = (S)(a_rest - ((double)m_rest - (double)w.m) * scale_d) + (w.off - few_log(w.sum_rest));
+  }
 }
 
-template <typename T, int KT, int KS, bool FULL, bool REST>
+template <typename T, int KT, int KS, bool FULL, bool REST, bool ROWS>
 __global__ void __launch_bounds__(256)
 k_distill_few_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
                   float* __restrict__ per_row, double* __restrict__ partial) {
+  typedef typename std::conditional<ROWS, double, float>::type S;
   __shared__ double s_red[4];
-  const float unit = temperature * 0.6931471805599453f;              // of the logarithms to base 2
+  const S unit = (S)((double)temperature * 0.6931471805599453);      // of the logarithms to base 2
   double loss_sum = 0.;
   int count = 0;
   const int64_t tiles = (s.V + 255) / 256;
@@ -536,25 +558,25 @@ k_distill_few_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
       const int64_t v0 = (int64_t)scalar((int)i) * 256;
       const uint32_t lane = lane_id();
       if (v0 + lane >= s.V) continue;
-      FewRow<KT, KS> w;
-      few_row<T, KT, KS, FULL, REST>(z, s, t, n, v0, lane, scale, inv_t, w);
-      float loss = 0.f;
+      FewRow<KT, KS, S> w;
+      few_row<T, KT, KS, FULL, REST, ROWS ? FEW_ROW_LOSS : FEW_MEAN_LOSS>(z, s, t, n, v0, lane, scale, inv_t, w);
+      S sum = 0;
       bool barred = false;                     // a listed class has probability zero
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
         const float x = pick_class(w.x, w.c[j]);
-        const float d = x == neg_inf() ? __builtin_inff() : fmaf(w.off, unit, w.a[j] - (x - w.m));
-        barred = barred || (d == __builtin_inff() && w.p[j] != 0.f);
-        loss += w.p[j] == 0.f ? 0.f : w.p[j] * d;
+        const S d = x == neg_inf() ? (S)__builtin_inff() : w.off * unit + ((S)w.a[j] - ((S)x - (S)w.m));
+        barred = barred || (d == (S)__builtin_inff() && w.p[j] != (S)0);
+        sum += w.p[j] == (S)0 ? (S)0 : w.p[j] * d;
       }
-      loss = barred ? +loss : in_range(loss);
+      sum = barred ? +sum : in_range(sum);
       if constexpr (REST) {
-        const float d = w.sum_rest == 0.f ? __builtin_inff() : unit * ((w.a_rest - w.d_rest) + (w.off - log2_f(w.sum_rest)));
-        loss += w.p_rest == 0.f ? 0.f : w.p_rest * d;
+        const S d = w.sum_rest == (S)0 ? (S)__builtin_inff() : w.off_rest * unit;
+        sum += w.p_rest == (S)0 ? (S)0 : w.p_rest * d;
       }
-      loss *= temperature;                     // the terms are T (log p - log q)
+      float loss = (float)(sum * (S)temperature);              // the terms are T (log p - log q)
       loss = w.state == 1 ? loss : w.state ? __builtin_nanf("") : 0.f;
-      if (per_row) per_row[n * s.V + v0 + lane] = loss;
+      if (ROWS) per_row[n * s.V + v0 + lane] = loss;
       loss_sum += (double)loss;
       count += w.state ? 1 : 0;
     }
@@ -582,8 +604,8 @@ k_distill_few_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
       const uint32_t lane = lane_id();
       if (v0 + lane >= s.V) continue;
       const float f = temperature * (grad_rows ? lane_load(grad + n * s.V + v0, lane) : g_all);
-      FewRow<KT, KS> w;
-      few_row<T, KT, KS, FULL, REST>(z, s, t, n, v0, lane, scale, inv_t, w);
+      FewRow<KT, KS, float> w;
+      few_row<T, KT, KS, FULL, REST, FEW_GRADIENT>(z, s, t, n, v0, lane, scale, inv_t, w);
       const float w_rest = REST && w.sum_rest != 0.f ? w.to_m * w.inv - w.p_rest * rcp_f(w.sum_rest) : 0.f;
       const float fill = w.state ? __builtin_nanf("") : 0.f;
       float out[KT];
@@ -841,9 +863,11 @@ int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* 
     if (one_stride(s) && one_stride(t.o)) { merge_rows(s); merge_rows(t.o); }
     const dim3 grid = few_grid(s.N, s.V, DIS_MAX_BLOCKS);
     parts = (int64_t)grid.x * grid.y;
-#define LAUNCH_FEW(KT, KS, FULL, REST) hipLaunchKernelGGL((k_distill_few_fwd<T, KT, KS, FULL, REST>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, per_row, part)
+#define LAUNCH_FEW_R(KT, KS, FULL, REST, ROWS) hipLaunchKernelGGL((k_distill_few_fwd<T, KT, KS, FULL, REST, ROWS>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, per_row, part)
+#define LAUNCH_FEW(KT, KS, FULL, REST) do { if (per_row) LAUNCH_FEW_R(KT, KS, FULL, REST, true); else LAUNCH_FEW_R(KT, KS, FULL, REST, false); } while (0)
     DISTILL_DISPATCH_FEW(LAUNCH_FEW);
 #undef LAUNCH_FEW
+#undef LAUNCH_FEW_R
   } else if (lane_rows(a->N * a->V, a->K, a->k)) {
     const int64_t blocks = cdiv(a->N * a->V, 256);
     parts = blocks < DIS_MAX_BLOCKS ? blocks : DIS_MAX_BLOCKS;

@@ -19,6 +19,41 @@ __device__ __forceinline__ int64_t row_offset(const RowShape& s, int64_t r) {
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 __device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// log2 of a positive sum to about 2^-25 absolute at the price of a fp32 logarithm: the exponent is taken off, so that the
+// hardware logarithm's result is at most 1/2, and what rounding the sum to fp32 left over is added in first order.
+__device__ __forceinline__ double log2_split(double x) {
+  const float f = (float)x;
+  float mant = __builtin_amdgcn_frexp_mantf(f);
+  int e = __builtin_amdgcn_frexp_expf(f);
+  const bool low = mant < 0.70710678f;
+  mant = low ? 2.f * mant : mant;
+  e -= low ? 1 : 0;
+  const float left = (float)(x - (double)f) * __builtin_amdgcn_rcpf(f) * 1.4426950408889634f;
+  return (double)e + ((double)__builtin_amdgcn_logf(mant) + (double)left);
+}
+
+// 2^y to about 1e-11 relative: 2^(y - n) by the exponential's series, nine terms of it at |y - n| ln 2 <= 0.35.  A dozen fp64
+// operations, no more than a fp32 exponential with its argument split.
+__device__ __forceinline__ double exp2_series(double y) {
+  const double n = rint(fmin(fmax(y, -1050.), 1020.)), f = (y - n) * 0.6931471805599453;
+  double e = 1. / 362880.;
+  e = fma(e, f, 1. / 40320.);
+  e = fma(e, f, 1. / 5040.);
+  e = fma(e, f, 1. / 720.);
+  e = fma(e, f, 1. / 120.);
+  e = fma(e, f, 1. / 24.);
+  e = fma(e, f, 1. / 6.);
+  e = fma(e, f, 0.5);
+  e = fma(e, f, 1.);
+  e = fma(e, f, 1.);
+  return y < -1050. ? 0. : ldexp(e, (int)n);
+}
+// log2 of a positive sum as exactly: one Newton step from log2_split
+__device__ __forceinline__ double log2_newton(double x) {
+  const double l = log2_split(x);
+  return fma(x * exp2_series(-l) - 1., 1.4426950408889634, l);
+}
+
 // 16 bytes of consecutive classes.  A row of an odd vocabulary starts at any multiple of the element size: the copies
 // below compile to one 16-byte access that the hardware takes at any address.
 template <typename T> constexpr int vec_of() { return 16 / (int)sizeof(T); }
@@ -120,6 +155,16 @@ template <int N> __device__ __forceinline__ float sum_of(const float (&x)[N]) {
   if constexpr (N == 1) return x[0];
   else {
     float y[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) y[i] = x[2 * i] + x[2 * i + 1];
+    return sum_of(y);
+  }
+}
+
+template <int N> __device__ __forceinline__ double sum_of(const double (&x)[N]) {
+  if constexpr (N == 1) return x[0];
+  else {
+    double y[N / 2];
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) y[i] = x[2 * i] + x[2 * i + 1];
     return sum_of(y);

@@ -341,10 +341,15 @@ k_top_wide(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t
   }
 }
 
+// the largest value over T and the logarithm may cancel: in fp64, rounded once
+__device__ __forceinline__ float log_rest(float m, float sum, double inv_t) {
+  return (float)fma((double)m, inv_t, 0.6931471805599453 * log2_split((double)sum));
+}
+
 // few classes: one thread a row.  Slot by slot the largest value left, the lowest class first (strict comparison).
 template <typename T, typename I, int KT, bool FULL>
 __global__ void __launch_bounds__(256)
-k_top_few(const T* __restrict__ z, RowShape s, int k, float scale, float inv_t, T* __restrict__ values, I* __restrict__ indices,
+k_top_few(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t, T* __restrict__ values, I* __restrict__ indices,
           RowShape o, float* __restrict__ rest) {
   for (int64_t n = blockIdx.y; n < s.N; n += gridDim.y) {
     for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < s.V; v += (int64_t)gridDim.x * 256) {
@@ -382,7 +387,7 @@ k_top_few(const T* __restrict__ z, RowShape s, int k, float scale, float inv_t, 
 #pragma unroll
         for (int c = 0; c < KT; ++c) e[c] = exp2_f((x[c] - ref) * scale);
         // m is -inf (nothing left) or +inf: it is the answer
-        rest[n * s.V + v] = ref == m ? fmaf(m, inv_t, __logf(sum_of(e))) : m;
+        rest[n * s.V + v] = ref == m ? log_rest(m, sum_of(e), inv_t) : m;
       }
     }
   }
@@ -392,7 +397,7 @@ k_top_few(const T* __restrict__ z, RowShape s, int k, float scale, float inv_t, 
 // class that comes leaves one loser, itself or the last of the list, for the rest.
 template <typename T, typename I, bool UNIT, int KS>
 __global__ void __launch_bounds__(256)
-k_top_lane(const T* __restrict__ z, RowShape s, int k, float scale, float inv_t, T* __restrict__ values, I* __restrict__ indices,
+k_top_lane(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t, T* __restrict__ values, I* __restrict__ indices,
            RowShape o, float* __restrict__ rest) {
   const int K = s.K;
   const int64_t NV = s.N * s.V;
@@ -437,7 +442,7 @@ k_top_lane(const T* __restrict__ z, RowShape s, int k, float scale, float inv_t,
       }
     }
     // nothing left (-inf), or infinities are: the maximum is the answer
-    if (rest) rest[r] = fabsf(left.m) < __builtin_inff() ? fmaf(left.m, inv_t, __logf(left.s)) : left.m;
+    if (rest) rest[r] = fabsf(left.m) < __builtin_inff() ? log_rest(left.m, left.s, inv_t) : left.m;
   }
 }
 
@@ -459,7 +464,7 @@ extern "C" int devis_top_logits(const void* logits, int64_t sN, int64_t sV, int6
   if (K <= FEW_CLASSES) {
     if (one_stride(s) && one_stride(o)) { merge_rows(s); merge_rows(o); }
     const dim3 grid = few_grid(s.N, s.V, 8192);
-#define LAUNCH_FEW(KT, FULL) hipLaunchKernelGGL((k_top_few<T, I, KT, FULL>), grid, dim3(256), 0, st, (const T*)logits, s, (int)k, scale, (float)inv_t, (T*)values, (I*)indices, o, rest)
+#define LAUNCH_FEW(KT, FULL) hipLaunchKernelGGL((k_top_few<T, I, KT, FULL>), grid, dim3(256), 0, st, (const T*)logits, s, (int)k, scale, inv_t, (T*)values, (I*)indices, o, rest)
     DEVIS_DISPATCH_DTYPE(dtype, {
       if (index_dtype == DEVIS_LABEL_U8) { typedef uint8_t I; DEVIS_DISPATCH_FEW(K, sK == 1, LAUNCH_FEW); }
       else { typedef int32_t I; DEVIS_DISPATCH_FEW(K, sK == 1, LAUNCH_FEW); }
@@ -470,7 +475,7 @@ extern "C" int devis_top_logits(const void* logits, int64_t sN, int64_t sV, int6
   if (lane_rows(NV, K, k)) {
     const int64_t tiles = cdiv(NV, 256);
     const dim3 grid((unsigned)(tiles < 8192 ? tiles : 8192));
-#define LAUNCH_LANE(UNIT, KS) hipLaunchKernelGGL((k_top_lane<T, I, UNIT, KS>), grid, dim3(256), 0, st, (const T*)logits, s, (int)k, scale, (float)inv_t, (T*)values, (I*)indices, o, rest)
+#define LAUNCH_LANE(UNIT, KS) hipLaunchKernelGGL((k_top_lane<T, I, UNIT, KS>), grid, dim3(256), 0, st, (const T*)logits, s, (int)k, scale, inv_t, (T*)values, (I*)indices, o, rest)
 #define LAUNCH_LANE_U(KS) do { if (sK == 1) LAUNCH_LANE(true, KS); else LAUNCH_LANE(false, KS); } while (0)
     DEVIS_DISPATCH_DTYPE(dtype, {
       if (index_dtype == DEVIS_LABEL_U8) { typedef uint8_t I; if (k <= 4) LAUNCH_LANE_U(4); else LAUNCH_LANE_U(16); }

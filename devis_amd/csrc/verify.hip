@@ -102,16 +102,6 @@ __device__ __forceinline__ void each_weight(const Draw<T>& d, int lo, int hi, in
   }
 }
 
-template <int N> __device__ __forceinline__ double sum_of(const double (&x)[N]) {
-  if constexpr (N == 1) return x[0];
-  else {
-    double y[N / 2];
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) y[i] = x[2 * i] + x[2 * i + 1];
-    return sum_of(y);
-  }
-}
-
 // One block a sequence.  Each wave sums the weights of one stretch of the row; the stretch in which the goal lies is read
 // once more, a vector a thread, and the class found by a prefix sum over the block.
 template <typename T, bool UNIT, bool DRAFTER, int BS>
