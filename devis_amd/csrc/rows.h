@@ -282,21 +282,22 @@ constexpr int LANE_SLOTS = 16;                // slots at most: every pair of th
 constexpr int64_t LANE_ROWS = 8192;           // rows at least: fewer are too few lanes
 inline bool lane_rows(int64_t rows, int64_t K, int64_t k) { return K <= LANE_CLASSES && k <= LANE_SLOTS && rows >= LANE_ROWS; }
 
-// running maximum and sum of exponentials against it
+// running maximum and sum of exponentials against it (fp64: one lane adds up the whole row)
 struct LaneSum {
-  float m, s;
+  float m;
+  double s;
   __device__ __forceinline__ void add(const float (&x)[8], float scale) {
     const float mx = max_of(x);
-    if (mx > m) { s *= exp2_f((m - mx) * scale); m = mx; }
+    if (mx > m) { s *= (double)exp2_f((m - mx) * scale); m = mx; }
     const float ref = m == neg_inf() ? 0.f : m;
     float e[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) e[i] = exp2_f((x[i] - ref) * scale);
-    s += sum_of(e);
+    s += (double)sum_of(e);
   }
   __device__ __forceinline__ void add_one(float x, float scale) {
-    if (x > m) { s *= exp2_f((m - x) * scale); m = x; }
-    s += exp2_f((x - (m == neg_inf() ? 0.f : m)) * scale);
+    if (x > m) { s *= (double)exp2_f((m - x) * scale); m = x; }
+    s += (double)exp2_f((x - (m == neg_inf() ? 0.f : m)) * scale);
   }
 };
 

@@ -342,8 +342,8 @@ k_top_wide(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t
 }
 
 // the largest value over T and the logarithm may cancel: in fp64, rounded once
-__device__ __forceinline__ float log_rest(float m, float sum, double inv_t) {
-  return (float)fma((double)m, inv_t, 0.6931471805599453 * log2_split((double)sum));
+__device__ __forceinline__ float log_rest(float m, double sum, double inv_t) {
+  return (float)fma((double)m, inv_t, 0.6931471805599453 * log2_split(sum));
 }
 
 // few classes: one thread a row.  Slot by slot the largest value left, the lowest class first (strict comparison).
@@ -387,7 +387,7 @@ k_top_few(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t,
 #pragma unroll
         for (int c = 0; c < KT; ++c) e[c] = exp2_f((x[c] - ref) * scale);
         // m is -inf (nothing left) or +inf: it is the answer
-        rest[n * s.V + v] = ref == m ? log_rest(m, sum_of(e), inv_t) : m;
+        rest[n * s.V + v] = ref == m ? log_rest(m, (double)sum_of(e), inv_t) : m;
       }
     }
   }
@@ -408,7 +408,7 @@ k_top_lane(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t
     int at[KS];
 #pragma unroll
     for (int j = 0; j < KS; ++j) top[j] = at[j] = 0;
-    LaneSum left = {neg_inf(), 0.f};
+    LaneSum left = {neg_inf(), 0.};
     for (int c0 = 0; c0 < K; c0 += 8) {
       float x[8];
       load8<T, UNIT>(p, s.sK, c0, K, x);
