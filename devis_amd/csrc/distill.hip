@@ -129,7 +129,7 @@ template <int BS> __device__ __forceinline__ void slot_classes(const Teacher& t,
 __device__ __forceinline__ bool row_masked(const Teacher& t, int64_t r) { return t.mask && t.mask[r] == 0; }
 
 template <typename T, bool UNIT, bool REST, int BS>
-__global__ void __launch_bounds__(BS, BS == 256 ? 8 : 1)
+__global__ void __launch_bounds__(BS, BS == 256 ? 8 : BS == 1024 ? 4 : 1)
 k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, double t2, RowStats* __restrict__ stats,
               float* __restrict__ per_row, double* __restrict__ partial) {
   constexpr bool LONG = BS > 64;
@@ -342,7 +342,7 @@ k_distill_finalize(const double* __restrict__ partial, int n, int mean, float* _
 }
 
 template <typename T, bool UNIT, bool PAST, int BS>
-__global__ void __launch_bounds__(BS, BS == 256 ? 8 : 1)
+__global__ void __launch_bounds__(BS, BS == 256 ? 8 : BS == 1024 ? 4 : 1)
 k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
               const RowStats* __restrict__ stats, const float* __restrict__ scal, const float* __restrict__ grad, int grad_rows,
               T* __restrict__ dz, RowShape d) {
@@ -371,7 +371,9 @@ k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
         for (int i = 0; i < N; ++i) x[i] = exp2_f((x[i] - st.ref) * scale) * w;
         store_vec<PAST>(q + (int64_t)c * (UNIT ? 1 : d.sK), x);
       });
-      __syncthreads();                       // the listed classes are written again, by other threads
+      // the listed classes are written again, by other threads: after these stores have been taken
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
       for (int j = tid; j < t.o.K; j += BS) {
         const int c = sh.c[j];
         if (c < 0 || sh.state == 2) continue;
@@ -793,6 +795,8 @@ static bool few_classes(const devis_distill_params* a) {
 
 // one block a row, or for short rows as many blocks as run at once
 static bool long_rows(const devis_distill_params* a) { return a->K > DIS_SHORT; }
+// fewer rows than CUs: a block four times as large takes each
+static bool few_rows(const devis_distill_params* a) { return a->K >= 8192 && a->N * a->V < 256; }
 static dim3 distill_grid(const devis_distill_params* a) {
   const int64_t NV = a->N * a->V;
   return long_rows(a) ? row_grid(NV) : dim3((unsigned)(NV < DIS_MAX_BLOCKS ? NV : DIS_MAX_BLOCKS));
@@ -830,6 +834,8 @@ using namespace devis;
     if (!long_rows(a)) {                                                                                          \
       if (unit) { if (a->rest) KERNEL(true, true, 64); else KERNEL(true, false, 64); }                            \
       else { if (a->rest) KERNEL(false, true, 64); else KERNEL(false, false, 64); }                               \
+    } else if (unit && few_rows(a)) {                                                                             \
+      if (a->rest) KERNEL(true, true, 1024); else KERNEL(true, false, 1024);                                      \
     } else {                                                                                                      \
       if (unit) { if (a->rest) KERNEL(true, true, 256); else KERNEL(true, false, 256); }                          \
       else { if (a->rest) KERNEL(false, true, 256); else KERNEL(false, false, 256); }                             \
@@ -923,6 +929,7 @@ int devis_distill_bwd(const devis_distill_params* a, const void* logits, const v
   DEVIS_DISPATCH_DTYPE(a->dtype, {
     if (!long_rows(a)) { if (unit) LAUNCH_DISTILL_BWD(true, false, 64); else LAUNCH_DISTILL_BWD(false, false, 64); }
     else if (!unit) LAUNCH_DISTILL_BWD(false, false, 256);
+    else if (few_rows(a)) LAUNCH_DISTILL_BWD(true, false, 1024);
     else if (past) LAUNCH_DISTILL_BWD(true, true, 256);
     else LAUNCH_DISTILL_BWD(true, false, 256);
   });

@@ -984,16 +984,13 @@ def class_rows(x: Tensor, channels_last: bool):
     return (x, n, v, x.shape[kd]) + s
 
 
-def _same_device(what: str, *ts: Optional[Tensor]) -> torch.device:
-    dev = None
-    for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise _lib.DevisError("devis_amd kernels need GPU tensors (got a %s tensor); there is no CPU fallback" % t.device)
-        if dev is not None and t.device != dev:
+def _same_device(what: str, first: Tensor, *others: Optional[Tensor]) -> torch.device:
+    dev = first.device
+    if dev.type != "cuda":
+        raise _lib.DevisError("devis_amd kernels need GPU tensors (got a %s tensor); there is no CPU fallback" % dev)
+    for t in others:
+        if t is not None and t.device != dev:
             raise _lib.DevisError("%s: tensors on %s and %s" % (what, dev, t.device))
-        dev = t.device
     return dev
 
 
@@ -1015,24 +1012,30 @@ def top_logits(logits: Tensor, k: int, channels_last: bool = True, temperature: 
     the logits' shape with k in the place of K, largest first, the lowest class first among equals; a NaN counts as
     +inf.  ``rest`` (fp32, one per row; None without ``want_rest``) = log of the sum over the other classes of
     exp(z / temperature), -inf if none is left.  1 <= k <= min(K, 128).  Not differentiable."""
-    code = dt_code(logits.dtype)
-    x, n, v, kk, sn, sv, sk = class_rows(logits.detach(), channels_last)
     k, temperature = int(k), float(temperature)
-    if not 1 <= k <= min(kk, _lib.TOP_MAX_K):
+    code = dt_code(logits.dtype)
+    x, n, v, kk, sn, sv, sk = class_rows(logits, channels_last)
+    if not 1 <= k <= kk or k > _lib.TOP_MAX_K:
         raise _lib.DevisError("top_logits: k must be in [1, min(K, %d)] = [1, %d], got %d" % (_lib.TOP_MAX_K, min(kk, _lib.TOP_MAX_K), k))
     _check_temperature(temperature)
     dev = _same_device("top_logits", x)
-    shape = tuple(x.shape[:-1]) if channels_last else (x.shape[0],) + tuple(x.shape[2:])
-    oshape = shape + (k,) if channels_last else (x.shape[0], k) + tuple(x.shape[2:])
-    idt = torch.uint8 if kk <= 256 else torch.int32
+    if channels_last:
+        shape = x.shape[:-1]
+        oshape, on, ov, ok = shape + (k,), v * k, k, 1
+    else:
+        shape = x.shape[:1] + x.shape[2:]
+        oshape, on, ov, ok = x.shape[:1] + (k,) + x.shape[2:], v * k, 1, v
+    small = kk <= 256
     with _on_device(dev):
         values = torch.empty(oshape, dtype=x.dtype, device=dev)
-        indices = torch.empty(oshape, dtype=idt, device=dev)
+        indices = torch.empty(oshape, dtype=torch.uint8 if small else torch.int32, device=dev)
         rest = torch.empty(shape, dtype=torch.float32, device=dev) if want_rest else None
         if n * v:
-            on, ov, ok = class_rows(values, channels_last)[4:]
-            check(_lib.load().devis_top_logits(_p(x), sn, sv, sk, code, n, v, kk, k, temperature, _p(values), _p(indices),
-                                               _label_code(indices), on, ov, ok, _p(rest), _stream()), "top_logits")
+            rc = _lib.load().devis_top_logits(x.data_ptr(), sn, sv, sk, code, n, v, kk, k, temperature, values.data_ptr(),
+                                              indices.data_ptr(), _lib.LABEL_U8 if small else _lib.LABEL_I32, on, ov, ok,
+                                              rest.data_ptr() if want_rest else None, _stream())
+            if rc:
+                check(rc, "top_logits")
     return dict(values=values, indices=indices, rest=rest)
 
 
@@ -1128,39 +1131,44 @@ def verify_drafts(tokens: Tensor, target_probs: Tensor, draft_probs: Optional[Te
     if tokens.dim() != 2 or target_probs.dim() != 3:
         raise _lib.DevisError("verify_drafts: tokens must be (B, T) and target_probs (B, T or T + 1, K)")
     b, t = tokens.shape
-    tp, k = target_probs.shape[1:]
+    pb, tp, k = target_probs.shape
     if tokens.dtype not in (torch.int64, torch.int32):
         raise _lib.DevisError("verify_drafts: tokens must be int64 or int32")
-    if target_probs.shape[0] != b or tp not in (t, t + 1) or tp < 1 or k < 1:
+    if pb != b or not t <= tp <= t + 1 or tp < 1 or k < 1:
         raise _lib.DevisError("verify_drafts: target_probs %s do not go with tokens %s" % (tuple(target_probs.shape), (b, t)))
-    if draft_probs is not None and (tuple(draft_probs.shape) != (b, t, k) or draft_probs.dtype != target_probs.dtype):
+    if draft_probs is not None and (draft_probs.shape != (b, t, k) or draft_probs.dtype != target_probs.dtype):
         raise _lib.DevisError("verify_drafts: draft_probs must be %s %s, got %s %s" %
                               ((b, t, k), target_probs.dtype, tuple(draft_probs.shape), draft_probs.dtype))
-    for name, u, shape in (("accept_u", accept_u, (b, t)), ("sample_u", sample_u, (b,))):
-        if u.dtype != torch.float32 or tuple(u.shape) != shape:
-            raise _lib.DevisError("verify_drafts: %s must be float32 %s, got %s %s" % (name, shape, u.dtype, tuple(u.shape)))
-    if lengths is not None:
-        if lengths.dtype not in (torch.int64, torch.int32) or tuple(lengths.shape) != (b,):
-            raise _lib.DevisError("verify_drafts: lengths must be int64 or int32 (B,)")
+    if accept_u.dtype != torch.float32 or accept_u.shape != (b, t):
+        raise _lib.DevisError("verify_drafts: accept_u must be float32 %s, got %s %s" % ((b, t), accept_u.dtype, tuple(accept_u.shape)))
+    if sample_u.dtype != torch.float32 or sample_u.shape != (b,):
+        raise _lib.DevisError("verify_drafts: sample_u must be float32 %s, got %s %s" % ((b,), sample_u.dtype, tuple(sample_u.shape)))
+    if lengths is not None and (lengths.dtype not in (torch.int64, torch.int32) or lengths.shape != (b,)):
+        raise _lib.DevisError("verify_drafts: lengths must be int64 or int32 (B,)")
     code = dt_code(target_probs.dtype)
     dev = _same_device("verify_drafts", tokens, target_probs, draft_probs, accept_u, sample_u, lengths)
-    if lengths is not None:
-        lengths = lengths.to(tokens.dtype).contiguous()
-    tokens, accept_u, sample_u = tokens.contiguous(), accept_u.contiguous(), sample_u.contiguous()
-
-    def regular(x):
-        x = x.detach()
-        return x if k == 1 or x.stride(2) > 0 else x.contiguous()
-    target = regular(target_probs)
-    draft = regular(draft_probs) if draft_probs is not None and t > 0 else None
-    ps = target.stride()
-    qs = draft.stride() if draft is not None else (0, 0, 1)
     with _on_device(dev):
+        if lengths is not None:
+            lengths = lengths.to(tokens.dtype).contiguous()
+        tokens, accept_u, sample_u = tokens.contiguous(), accept_u.contiguous(), sample_u.contiguous()
+        target, draft = target_probs, draft_probs if t > 0 else None
+        ps = target.stride()
+        if k > 1 and ps[2] <= 0:
+            target = target.contiguous()
+            ps = target.stride()
+        qs = (0, 0, 1)
+        if draft is not None:
+            qs = draft.stride()
+            if k > 1 and qs[2] <= 0:
+                draft = draft.contiguous()
+                qs = draft.stride()
         out = torch.empty((b, tp), dtype=tokens.dtype, device=dev)
         accepted = torch.empty((b,), dtype=tokens.dtype, device=dev)
         if b:
-            p = _lib.VerifyParams(b, t, tp, k, ps[0], ps[1], ps[2], qs[0], qs[1], qs[2], _p(tokens), _p(accept_u), _p(sample_u),
-                                  _p(lengths), code, _label_code(tokens))
-            check(_lib.load().devis_verify_drafts(C.byref(p), _p(target), _p(draft), _p(out), _p(accepted), _stream()),
-                  "verify_drafts")
+            p = _lib.VerifyParams(b, t, tp, k, *ps, *qs, tokens.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(),
+                                  None if lengths is None else lengths.data_ptr(), code, _label_code(tokens))
+            rc = _lib.load().devis_verify_drafts(C.byref(p), target.data_ptr(), None if draft is None else draft.data_ptr(),
+                                                 out.data_ptr(), accepted.data_ptr(), _stream())
+            if rc:
+                check(rc, "verify_drafts")
     return dict(tokens=out, accepted=accepted)

@@ -93,6 +93,8 @@ class TMSU(nn.Module):
                 loss = loss + weight * distill_top_loss(logits, top["values"], top["indices"], top["rest"],
                                                         channels_last=True, temperature=temperature)
             return evidence, loss
+        if distill is not None:
+            raise ValueError("TMSU.forward: distill belongs to mode 'train', got mode %r" % (mode,))
         if dataset == 'BraTS':
             out = tailor_and_concat(X, self.backbone)
         else:
@@ -103,12 +105,14 @@ class TMSU(nn.Module):
         """This model as a teacher: the k largest logits of every voxel of X and the mass of the others
         (`ops.top_logits`), channels last.  Runs in eval mode without gradients."""
         training = self.training
-        self.eval()
+        if training:
+            self.eval()
         try:
             with torch.no_grad():
                 return ops.top_logits(self.backbone.forward_channels_last(X), k, channels_last=True, temperature=temperature)
         finally:
-            self.train(training)
+            if training:
+                self.train()
 
     def infer(self, input):
         """softplus evidence of NC(D)HW logits (TrustworthySeg.py:160-166)."""

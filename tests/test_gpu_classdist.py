@@ -525,6 +525,15 @@ def test_verify_borders(K):
             check_verify(tok, p, x, u, r, lengths)
 
 
+def test_verify_random_numbers_that_are_none():
+    for K in (4, 900):
+        tok, p, q, u, r = drafts(6, 2, K, torch.float32, K)
+        u[0], r[1] = math.nan, math.nan                      # never accepted; the last class with weight
+        q[2, 0, ::2] = math.nan
+        check_verify(tok, p, q, u, r)
+        check_verify(tok, p, None, u, r)
+
+
 def test_verify_without_drafts_draws_from_the_target():
     tok, p, q, u, r = drafts(50, 0, 300, torch.float32, 3)
     check_verify(tok, p, q, u, r)
@@ -569,6 +578,51 @@ def test_verify_frequencies():
         out = ops.verify_drafts(tok, pf.expand(n * n, 1, K), qf.expand(n * n, 1, K), uu.reshape(-1, 1).cuda(), rr.reshape(-1).cuda())
         total += q[d] * torch.bincount(out["tokens"][:, 0], minlength=K).cpu().double() / (n * n)
     assert (total - p).abs().max().item() < 2.0 / n
+
+
+# ------------------------------------------------------------------ offsets past 32 bits
+@pytest.mark.parametrize("first", [False, True])
+def test_offsets_past_32_bits(first):
+    """The last rows of arrays of more than 2^31 (volumes, channels first: 2^32) elements."""
+    from devis_amd import criterions, ops
+    if first:
+        rows, K, k = 270_000_000, 8, 2                       # a lane a row
+        z = torch.zeros((2, K, rows), dtype=torch.bfloat16, device="cuda")
+        tail = lambda x: x[1, :, -5:].t() if x.dim() == 3 else x[1, -5:]
+    else:
+        rows, K, k = 34_000, 65_536, 9                       # a block a row
+        z = torch.zeros((rows, K), dtype=torch.bfloat16, device="cuda")
+        tail = lambda x: x[-5:]
+    assert z.numel() > 2 ** 31
+    want = logits(5, K, torch.bfloat16, 3)
+    tail(z).copy_(want)
+    out = ops.top_logits(z, k, channels_last=not first)
+    v, i, r = teacher_of(want, k, 1.0)
+    assert torch.equal(tail(out["indices"]).long().cpu(), i.long()) and torch.equal(tail(out["values"]).cpu(), v)
+    assert (tail(out["rest"]).cpu().double() - r.double()).abs().max().item() < 2 * sum_error(want.double().numpy(), 1.0) + 32 * E
+    z.requires_grad_(True)
+    out["values"].mul_(0.5)
+    per_row = criterions.distill_top_loss(z, out["values"], out["indices"], out["rest"], channels_last=not first, reduction="none")
+    (dz,) = torch.autograd.grad(per_row, z, torch.ones_like(per_row))
+    loss, grad, _, scale, err = oracle_rows(want, (v.float() * 0.5).to(v.dtype), i, tail(out["rest"]).cpu(), None, 1.0)
+    assert np.all(np.abs(tail(per_row).detach().cpu().double().numpy() - loss) <= err)
+    have = tail(dz).cpu().double().numpy()
+    for a, b, c, row in zip(have, grad, scale, want):
+        assert np.all(np.abs(a - b) <= c * (2 * sum_error(row.double().numpy(), 1.0) + 16 * E) + HALF[torch.bfloat16] * np.abs(b) + 1e-37)
+
+
+def test_verify_offsets_past_32_bits():
+    from devis_amd import ops
+    B, K = 34_000, 65_536
+    p = torch.zeros((B, 1, K), dtype=torch.bfloat16, device="cuda")
+    tok, pw, q, u, r = drafts(4, 1, K, torch.bfloat16, 5, bonus=False)
+    p[-4:] = pw.cuda()
+    full = lambda x, n: torch.cat([torch.zeros((n,) + tuple(x.shape[1:]), dtype=x.dtype), x]).cuda()
+    out = ops.verify_drafts(full(tok, B - 4), p, None, full(u, B - 4), full(r, B - 4))
+    for j in range(4):
+        want, a = O.verify_row(tok[j].numpy(), pw[j].double().numpy(), None, u[j].double().numpy(), float(r[j]), 1)
+        assert out["accepted"][B - 4 + j].item() == a and np.array_equal(out["tokens"][B - 4 + j].cpu().numpy(), want)
+    assert out["tokens"][0, 0].item() == -1                  # no class has weight
 
 
 # ------------------------------------------------------------------ together, streams, graphs

@@ -112,6 +112,13 @@ def test_training_command_refuses(flags, tmp_path):
         T.load_teacher(args)
 
 
+def test_the_term_belongs_to_training():
+    student, teacher = models()
+    x, y = batch(1)
+    with pytest.raises(ValueError, match="train"):
+        student(x, y, 5, 'val', 'LiTS', distill=(teacher.top_logits(x, 2), 1.0, 1.0))
+
+
 def test_no_teacher_without_the_flag():
     from devis_amd import train as T
     assert T.load_teacher(T.getArgs(['--dataset', 'BraTS'])) is None
