@@ -9,7 +9,8 @@
 // Without rest, p_rest = 0 and the top is renormalised.  Both passes are bound by memory: the forward reads the row
 // once with a running maximum and sum per thread, keeping the classes in no slot apart (a bit per class in LDS tells
 // them); the backward reads it once more and writes the gradient: for a class in no slot it is one exponential times a
-// factor of the row, W = 1/s - p_rest/s_rest; the k listed classes are put right afterwards.
+// factor of the row, W = 1/s - p_rest/s_rest; the k listed classes are put right afterwards.  4096 x 131072 bf16, 64 slots
+// and rest: forward 194 us (5.5 TB/s), backward 403 us (5.3 TB/s; a copy moves 5.0), together 614.
 #include "rows.h"
 
 #include <type_traits>
@@ -393,7 +394,8 @@ k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
 // ---- few classes: one thread a row, everything in registers, nothing kept for the backward.  Exponentials and logarithms
 // are fp32 here (fp64 ones would cost more than the memory at this many rows); a row's loss is put together from
 //   T (log p_j - log q_j) = (t_j - t_max) - (z_j - z_max) + T log(S_student / S_teacher),
-// where the large parts have cancelled before anything is rounded.  Sums over rows are fp64.
+// where the large parts have cancelled before anything is rounded.  Sums over rows are fp64.  2 x 128^3 x 4 bf16, two slots
+// and rest: 30 us forward, 29 backward (75 and 109 MB; VALU issue is 84 and 92 % busy: ~190 instructions a row).
 __device__ __forceinline__ float log2_f(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ float rcp_f(float x) { return __builtin_amdgcn_rcpf(x); }
 

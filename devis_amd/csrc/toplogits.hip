@@ -4,11 +4,10 @@
 //   order the classes by (value descending, class ascending); values / indices = the first k;
 //   rest = log sum over the classes not among them of exp(z_c / T).
 //
-// Selection in two passes over the row.  A class is its 64-bit key (value as an ordered integer, class counted
-// downwards), so keys differ and every tie falls to the lowest class.  Pass 1: each thread's largest key; the k-th
-// largest of these BS keys, tau, has at least k keys at or above it, and rarely many more (73 expected for k = 64 of
-// 256 threads).  Pass 2: keys >= tau go to a list in LDS, everything else into the sum of exponentials; the list is
-// ranked by counting.  Memory is read once from HBM; pass 2 finds the row in L2 / Infinity Cache.
+// A class is its 64-bit key (value as an ordered integer, class counted downwards), so keys differ and every tie falls to
+// the lowest class.  Bound by memory: one read of the row.  Long rows (k_top_wide): 2048 x 131072 bf16, 64 kept, in 112 us =
+// 4.8 TB/s (two reads of the row, as k_top_rows does it: 196 us).  Few classes (k_top_few): 2 x 128^3 x 4 fp32 in 22 us,
+// 126 MB.  Dozens of classes (k_top_lane): 2 x 104 x 64^3 bf16 in 89 us (a wave a row: 727 us).
 #include "rows.h"
 
 namespace devis {
@@ -103,7 +102,9 @@ __device__ __forceinline__ void top_finish(const T* __restrict__ p, const RowSha
   }
 }
 
-// One row, any strides and any contents, by one block.
+// One row, any strides and any contents, by one block, in two passes.  Pass 1: each thread's largest key; the k-th largest
+// of these BS keys, tau, has at least k keys at or above it, and rarely many more (73 expected for k = 64 of 256 threads).
+// Pass 2: keys >= tau go to a list in LDS, everything else into the sum of exponentials; the list is ranked by counting.
 template <typename T, typename I, bool UNIT, int BS, int U>
 __device__ __forceinline__ void top_row_general(const T* __restrict__ p, const RowShape& s, int64_t r, int k, float scale, double inv_t,
                                 T* __restrict__ values, I* __restrict__ indices, const RowShape& o, float* __restrict__ rest,
