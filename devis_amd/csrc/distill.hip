@@ -18,13 +18,15 @@
 namespace devis {
 
 constexpr int DIS_MAX_K = DEVIS_TOP_MAX_K;
-constexpr int DIS_SEG = 131072;               // classes whose slot bits are in LDS at a time (16 KB)
+// classes whose slot bits are in LDS at a time (16 KB; of a short row all of them, so that LDS does not limit its waves)
+template <int BS> constexpr int dis_seg() { return BS == 64 ? 1024 : 131072; }
 constexpr int DIS_SHORT = 1024;               // classes up to which a wave takes a row, and the block several
 // A gradient as large as the 256 MB Infinity Cache cannot stay there for its reader: written past the caches it leaves the
 // logits in them, which the backward reads from the last row on.  Loss and gradient of 4096 x 131072 bf16 rows: 658 us with
 // ordinary stores, 613 past the caches; 2048 x 65536 (256 MB) 198 and 175; below, the gradient is better kept.
 constexpr double DIS_PAST_BYTES = 256. * 1024 * 1024;
 constexpr int DIS_MAX_BLOCKS = 2048;          // 8 blocks of 256 threads on each of 256 CUs
+constexpr int DIS_MAX_WAVES = 8192;           // or as many blocks of a wave
 
 // what the backward needs of a row
 struct RowStats { float ref, w, m, inv_s; };  // gradient of a class in no slot: exp((z - ref)/T) w;  q = exp((z - m)/T) inv_s
@@ -135,7 +137,8 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
               float* __restrict__ per_row, double* __restrict__ partial) {
   constexpr bool LONG = BS > 64;
   __shared__ SlotShared sh;
-  __shared__ uint32_t s_bits[REST ? DIS_SEG / 32 : 1];
+  constexpr int SEG = dis_seg<BS>();
+  __shared__ uint32_t s_bits[REST ? SEG / 32 : 1];
   __shared__ double s_red[BS / 64];
   __shared__ float s_max[BS / 64];
   const int K = s.K;
@@ -170,8 +173,8 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
       for (int i = 0; i < N; ++i) x[i] = exp2_f((x[i] - ref) * scale);
       acc += sum_of(x);
     };
-    for (int lo = 0; lo < K; lo += DIS_SEG) {
-      const int hi = K - lo < DIS_SEG ? K : lo + DIS_SEG;
+    for (int lo = 0; lo < K; lo += SEG) {
+      const int hi = K - lo < SEG ? K : lo + SEG;
       if constexpr (REST) {
         for (int i = tid; i < (hi - lo + 31) / 32; i += BS) s_bits[i] = 0;
         __syncthreads();
@@ -801,9 +804,9 @@ static bool long_rows(const devis_distill_params* a) { return a->K > DIS_SHORT; 
 static bool few_rows(const devis_distill_params* a) { return a->K >= 8192 && a->N * a->V < 256; }
 static dim3 distill_grid(const devis_distill_params* a) {
   const int64_t NV = a->N * a->V;
-  return long_rows(a) ? row_grid(NV) : dim3((unsigned)(NV < DIS_MAX_BLOCKS ? NV : DIS_MAX_BLOCKS));
+  return long_rows(a) ? row_grid(NV) : dim3((unsigned)(NV < DIS_MAX_WAVES ? NV : DIS_MAX_WAVES));
 }
-static int64_t distill_partials(const devis_distill_params* a) { return long_rows(a) ? a->N * a->V : DIS_MAX_BLOCKS; }
+static int64_t distill_partials(const devis_distill_params* a) { return long_rows(a) ? a->N * a->V : DIS_MAX_WAVES; }
 
 static bool distill_args_ok(const devis_distill_params* a, const void* logits) {
   if (!a || !logits || !a->values || !a->indices) return false;

@@ -297,6 +297,61 @@ k_verify_few(const T* __restrict__ p, const T* __restrict__ q, VerifyArgs a) {
   }
 }
 
+// dozens of classes and many sequences (rows.h): one thread a sequence, the weights added up and then walked, 8 at a time
+template <typename T, bool UNIT, bool DRAFTER>
+__global__ void __launch_bounds__(256)
+k_verify_lane(const T* __restrict__ p, const T* __restrict__ q, VerifyArgs a) {
+  for (int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x; b < a.B; b += (int64_t)gridDim.x * 256) {
+    const int len = draft_length(a, b);
+    int n = 0, drawn = -1;
+    while (n < len && draft_ok(a, p, q, b, n)) {
+      put_int(a.out_tokens, a.token_kind, b * a.Tp + n, int_at(a.tokens, a.token_kind, b * a.T + n));
+      ++n;
+    }
+    if (n < a.Tp) {
+      Draw<T> d = {p + b * a.pB + n * a.pT, nullptr, a.pK, a.qK, -1};
+      if (n < len) {
+        if (DRAFTER) d.q = q + b * a.qB + n * a.qT;
+        else {
+          const int64_t c = int_at(a.tokens, a.token_kind, b * a.T + n);
+          d.skip = c < 0 || c >= a.K ? -1 : (int)c;
+        }
+      }
+      const auto weights = [&](int c, double (&w)[8]) {
+        float x[8], y[8] = {};
+        load8<T, UNIT>(d.p, a.pK, c, a.K, x);                  // -inf behind the last class: no weight
+        if (DRAFTER && d.q) load8<T, UNIT>(d.q, a.qK, c, a.K, y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = c + i < a.K ? weight_of(x[i], y[i], c + i != d.skip) : 0.;
+      };
+      double w[8], total = 0.;
+      for (int c = 0; c < a.K; c += 8) { weights(c, w); total += sum_of(w); }
+      if (!(total > 0.) && (d.q || d.skip >= 0)) {             // nothing is left over: the target's row itself
+        d.q = nullptr;
+        d.skip = -1;
+        total = 0.;
+        for (int c = 0; c < a.K; c += 8) { weights(c, w); total += sum_of(w); }
+      }
+      if (total > 0.) {
+        const double goal = (double)a.sample_u[b] * total;
+        double run = 0.;
+        bool open = true;
+        for (int c = 0; c < a.K && open; c += 8) {
+          weights(c, w);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            run += w[i];
+            drawn = open && w[i] > 0. ? c + i : drawn;         // the last with weight so far
+            open = open && !(w[i] > 0. && run > goal);
+          }
+        }
+      }
+    }
+    for (int t = n; t < a.Tp; ++t) put_int(a.out_tokens, a.token_kind, b * a.Tp + t, t == n ? drawn : -1);
+    put_int(a.out_accepted, a.token_kind, b, n);
+  }
+}
+
 }  // namespace devis
 
 using namespace devis;
@@ -322,6 +377,17 @@ extern "C" int devis_verify_drafts(const devis_verify_params* v, const void* tar
 #undef LAUNCH_FEW_ALONE
 #undef LAUNCH_FEW_DRAFTER
 #undef LAUNCH_FEW
+    return launch_status();
+  }
+  if (lane_rows(v->B, v->K, 1)) {
+    const dim3 grid = few_grid(1, v->B, 8192);
+    const bool unit = v->pK == 1 && (!draft || v->qK == 1);
+#define LAUNCH_LANE(UNIT, DRAFTER) hipLaunchKernelGGL((k_verify_lane<T, UNIT, DRAFTER>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)target, (const T*)draft, a)
+    DEVIS_DISPATCH_DTYPE(v->dtype, {
+      if (draft) { if (unit) LAUNCH_LANE(true, true); else LAUNCH_LANE(false, true); }
+      else { if (unit) LAUNCH_LANE(true, false); else LAUNCH_LANE(false, false); }
+    });
+#undef LAUNCH_LANE
     return launch_status();
   }
   const unsigned blocks = (unsigned)(v->B < (1 << 20) ? v->B : (1 << 20));

@@ -507,6 +507,30 @@ def test_verify_sizes(B, T, K, dtype, bonus):
         check_verify(tok, p, None, u * 0.01, r, lengths.to(torch.int32))
 
 
+def many(x, times):
+    return None if x is None else torch.cat([x] * times)
+
+
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K", [4, 17, 40, 100, 256])
+def test_verify_many_sequences(K, dtype, strided):
+    """The same sequences many times over: a thread each; every copy as the first ones, and those as the oracle says."""
+    from devis_amd import ops
+    times = 200
+    put = (lambda x: x.cuda().movedim(2, 0).contiguous().movedim(0, 2)) if strided else (lambda x: x.cuda())
+    for bonus in (True, False):
+        tok, p, q, u, r = drafts(41, 3, K, dtype, K, bonus, torch.int32)
+        p[5] = 0.0
+        p[8], q[8] = q[8, :1].expand(p.shape[1:]), p[8, :3]
+        lengths = torch.arange(41) % 4
+        for x, n in ((q, None), (q, lengths), (None, lengths)):
+            one = check_verify(tok, p, x, u, r, n)
+            out = ops.verify_drafts(many(tok, times).cuda(), put(many(p, times)), None if x is None else put(many(x, times)),
+                                    many(u, times).cuda(), many(r, times).cuda(), None if n is None else many(n, times).cuda())
+            assert torch.equal(out["tokens"], many(one["tokens"], times)) and torch.equal(out["accepted"], many(one["accepted"], times))
+
+
 @pytest.mark.parametrize("K", [4, 40, 5000])
 def test_verify_borders(K):
     tok, p, q, u, r = drafts(12, 2, K, torch.float32, K)
