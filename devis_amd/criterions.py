@@ -166,12 +166,12 @@ def dce_evidence_u_loss(p, alpha, c, current_step, lamda_step, total_step, eps, 
 
 # --------------------------------------------------------------------------- distillation (no counterpart in the reference)
 class _DistillFn(torch.autograd.Function):
-    """logits -> loss (scalar, or one per row), given the teacher's top logits.  `how` = (channels_last, temperature,
-    reduction, grad mode of the caller)."""
+    """logits -> loss (scalar, or one per row).  `call` = (values, indices, rest, row_mask, channels_last, temperature,
+    reduction, grad mode of the caller): one argument, because autograd looks at every one it is given."""
 
     @staticmethod
-    def forward(ctx, logits, values, indices, rest, row_mask, how):
-        channels_last, temperature, reduction, grad_on = how
+    def forward(ctx, logits, call):
+        values, indices, rest, row_mask, channels_last, temperature, reduction, grad_on = call
         rows = reduction == "none"
         params, dev, shape, ts = ops.distill_params(logits, values, indices, rest, row_mask, channels_last, temperature,
                                                     reduction == "mean")
@@ -183,19 +183,18 @@ class _DistillFn(torch.autograd.Function):
         loss, scratch = ops.distill_fwd(params, dev, shape, ts[0], rows, need)
         if need:
             ctx.save_for_backward(*ts, scratch)
-            ctx.params, ctx.channels_last, ctx.rows = params, channels_last, rows
-            ctx.at = _places(ts)
+            ctx.call = params, channels_last, rows, dev, _places(ts)
         return loss
 
     @staticmethod
     def backward(ctx, g):
         if not torch.is_grad_enabled():
-            return (_distill_backward(ctx, g),) + (None,) * 5
+            return _distill_backward(ctx, g), None
         # under create_graph: a second derivative has to be refused, not taken as zero
         logits = ctx.saved_tensors[0] if not ctx.empty else g
         with torch.no_grad():
             dz = _distill_backward(ctx, g)
-        return (_NoSecondDerivative.apply(dz, logits, g),) + (None,) * 5
+        return _NoSecondDerivative.apply(dz, logits, g), None
 
 
 class _NoSecondDerivative(torch.autograd.Function):
@@ -219,13 +218,12 @@ def _distill_backward(ctx, g):
         shape, dtype, dev = ctx.like
         return torch.zeros(shape, dtype=dtype, device=dev)
     *ts, scratch = ctx.saved_tensors
-    params = ctx.params
-    if _places(ts) != ctx.at:                     # moved by saved-tensor hooks
-        params, _, _, ts = ops.distill_params(*ts, ctx.channels_last, params.temperature, params.mean)
+    params, channels_last, rows, dev, places = ctx.call
+    if _places(ts) != places:                     # moved by saved-tensor hooks
+        params, dev, _, ts = ops.distill_params(*ts, channels_last, params.temperature, params.mean)
     if g.dtype != torch.float32 or not g.is_contiguous():
         g = g.contiguous().float()
-    x = ts[0]
-    return ops.distill_bwd(params, x.device, x, ctx.channels_last, scratch, g, ctx.rows)
+    return ops.distill_bwd(params, dev, ts[0], channels_last, scratch, g, rows)
 
 
 def distill_top_loss(logits: Tensor, values: Tensor, indices: Tensor, rest: Optional[Tensor] = None, channels_last: bool = True,
@@ -245,8 +243,8 @@ def distill_top_loss(logits: Tensor, values: Tensor, indices: Tensor, rest: Opti
         raise ValueError("reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
     if values.requires_grad or (rest is not None and rest.requires_grad):
         raise ValueError("distill_top_loss does not differentiate in the teacher: detach values and rest")
-    return _DistillFn.apply(logits, values, indices, rest, row_mask,
-                            (bool(channels_last), float(temperature), reduction, torch.is_grad_enabled()))
+    return _DistillFn.apply(logits, (values, indices, rest, row_mask, bool(channels_last), float(temperature), reduction,
+                                     torch.is_grad_enabled()))
 
 
 # --------------------------------------------------------------------------- API-compat shims (torch ops)

@@ -1057,8 +1057,8 @@ def distill_params(logits: Tensor, values: Tensor, indices: Tensor, rest: Option
         raise _lib.DevisError("distill: values %s and indices %s differ in shape" % (tuple(values.shape), tuple(indices.shape)))
     if not 1 <= k <= min(kk, _lib.TOP_MAX_K):
         raise _lib.DevisError("distill: 1 to min(K, %d) = %d slots a row, got %d" % (_lib.TOP_MAX_K, min(kk, _lib.TOP_MAX_K), k))
-    i, _, _, _, *io = class_rows(indices, channels_last)
-    if tuple(io) != (on, ov, ok):
+    i = indices
+    if i.stride() != t.stride():
         t, i = t.contiguous(), i.contiguous()
         on, ov, ok = class_rows(t, channels_last)[4:]
     _check_temperature(temperature)
