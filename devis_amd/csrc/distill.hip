@@ -31,8 +31,8 @@ constexpr int DIS_MAX_WAVES = 8192;           // or as many blocks of a wave
 // what the backward needs of a row
 struct RowStats { float ref, w, m, inv_s; };  // gradient of a class in no slot: exp((z - ref)/T) w;  q = exp((z - m)/T) inv_s
 
-// The ends of a row: fp64 for long rows; for the short ones of a wave each, fp32 (there are many, and fp64 logarithms,
-// exponentials and quotients would cost more than the row).
+// The ends of a row: fp64 for long rows.  Of the short ones of a wave each there are many, and the library's fp64 functions
+// would cost more than the row: logarithms by a Newton step, exponentials and quotients in fp32.
 template <bool LONG> __device__ __forceinline__ double end_log(double x) { return LONG || !(x > 0.) ? log(x) : 0.6931471805599453 * log2_newton(x); }
 template <bool LONG> __device__ __forceinline__ double end_exp2(double x) { return LONG ? exp2(x) : (double)exp2_f((float)x); }
 template <bool LONG> __device__ __forceinline__ double end_div(double a, double b) { return LONG ? a / b : a * (double)(1.f / (float)b); }
@@ -394,8 +394,8 @@ k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
   }
 }
 
-// ---- few classes: one thread a row, everything in registers, nothing kept for the backward.  Exponentials and logarithms
-// are fp32 here (fp64 ones would cost more than the memory at this many rows); a row's loss is put together from
+// ---- few classes: one thread a row, everything in registers, nothing kept for the backward.  For a mean and for
+// the gradient exponentials and logarithms are fp32 (FEW_ROW_LOSS below: fp64); a row's loss is put together from
 //   T (log p_j - log q_j) = (t_j - t_max) - (z_j - z_max) + T log(S_student / S_teacher),
 // where the large parts have cancelled before anything is rounded.  Sums over rows are fp64.  2 x 128^3 x 4 bf16, two slots
 // and rest: 30 us forward, 29 backward (75 and 109 MB; VALU issue is 84 and 92 % busy: ~190 instructions a row).
@@ -783,6 +783,7 @@ k_distill_lane_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, 
       each_slot(t, at, K, [&](int, float v, int) { sum += exp2_f(fmaf(v - hi, scale, -shift)); });
       const float inv_sum = rcp_f(sum);
       each_slot(t, at, K, [&](int, float, int c) {
+        if (c < 0 || c >= K) return;           // the forward would have seen it: the slots have been rewritten since
         float share = 0.f;
         each_slot(t, at, K, [&](int, float v, int c2) { share += c2 == c ? exp2_f(fmaf(v - hi, scale, -shift)) : 0.f; });
         const float x = (float)p[(int64_t)c * s.sK];

@@ -63,7 +63,8 @@ __device__ __forceinline__ void top_finish(const T* __restrict__ p, const RowSha
       indices[at_o] = (I)c;
       if (rank == k - 1) sh.kth = key;
     } else {
-      sum += (double)exp2_f((key_value(key) - base) * scale);
+      // far above `base` where large classes lie side by side and one thread held them all: past what fp32 holds
+      sum += exp2_series(((double)key_value(key) - (double)base) * inv_t * 1.4426950408889634);
     }
   }
   if (rest) {
@@ -71,8 +72,8 @@ __device__ __forceinline__ void top_finish(const T* __restrict__ p, const RowSha
     __syncthreads();
     const int tid = lane_id();
     float ref = base;
-    // the rest lies far below the listed classes (or they are infinite): take its own largest value as reference
-    if (!(sum > 0x1p-60) || !(ref < __builtin_inff())) {
+    // the rest lies far below `base` or too far above it, or is infinite: take its own largest value as reference
+    if (!(sum > 0x1p-60) || !(sum < 0x1p900) || !(ref < __builtin_inff())) {
       const uint64_t kth = sh.kth;
       float m = neg_inf();
       each_class<T, UNIT, BS, 1>(tid, p, s.sK, 0, K, [&](auto& x, int c) {

@@ -1149,7 +1149,9 @@ def verify_drafts(tokens: Tensor, target_probs: Tensor, draft_probs: Optional[Te
     dev = _same_device("verify_drafts", tokens, target_probs, draft_probs, accept_u, sample_u, lengths)
     with _on_device(dev):
         if lengths is not None:
-            lengths = lengths.to(tokens.dtype).contiguous()
+            if lengths.dtype != tokens.dtype:
+                lengths = lengths.clamp(0, t).to(tokens.dtype)       # an int64 length past int32 stays long
+            lengths = lengths.contiguous()
         tokens, accept_u, sample_u = tokens.contiguous(), accept_u.contiguous(), sample_u.contiguous()
         target, draft = target_probs, draft_probs if t > 0 else None
         ps = target.stride()

@@ -200,8 +200,9 @@ def load_teacher(args):
 
 def train(args, model, optimizer, epoch, train_loader, reducer=None, log=print, teacher=None):
     """One epoch; same order of operations as trainUMIS.py:239-263.  `reducer` (devis_amd.parallel)
-    averages gradients across ranks; `teacher` (`load_teacher`) adds the distillation term of `--distill_*`.  The per-iteration loss lines are kept, in order, but are printed
-    through LossMeter: the launch thread never waits for the GPU inside the loop."""
+    averages gradients across ranks; `teacher` (`load_teacher`) adds the distillation term of `--distill_*`.
+    The per-iteration loss lines are kept, in order, but are printed through LossMeter: the launch thread
+    never waits for the GPU inside the loop."""
     model.train()
     meter = LossMeter(log)
     step = 0
@@ -530,11 +531,11 @@ def run(args, loaders=None, log=print):
         get = lambda a, salt=0: loaders
     train_loader, valid_loader, test_loader = get(args)
     model, optimizer, reducer = build(args, rank)
-    teacher = load_teacher(args)
     out = dict(loss_list=[], dice_list=[], best_dice=0, test=None)
     best_dice = 0
     if mode in ('train&test', 'train'):
         first = args.start_epoch if mode == 'train&test' else 1
+        teacher = load_teacher(args)
         for epoch in range(first, args.end_epochs + 1):
             say('===========Train begining!===========')
             say('Epoch {}/{}'.format(epoch, args.end_epochs - 1))
