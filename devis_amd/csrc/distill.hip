@@ -73,32 +73,34 @@ template <bool LONG>
 __device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int K, double inv_t, int lane, SlotShared& sh) {
   const int k = t.o.K;
   const int64_t at = row_offset(t.o, r);
-  double y[2];
+  float v[2];
   int cls[2];
   bool bad = false, any = false;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int j = lane + 64 * u;
-    y[u] = -__builtin_inf();
+    v[u] = neg_inf();
     cls[u] = 0;
     if (j < k) {
       const int64_t i = at + j * t.o.sK;
-      const float v = slot_value(t, i);
-      if (v != neg_inf()) {
+      v[u] = slot_value(t, i);
+      if (v[u] != neg_inf()) {
         any = true;
-        y[u] = (double)v * inv_t;
         cls[u] = class_at(t.indices, t.index_kind, i);
         if (cls[u] < 0 || cls[u] >= K) { bad = true; cls[u] = 0; }
       }
     }
   }
   const int state = !__any(any) ? 0 : __any(bad) ? 2 : 1;
-  const double yr = t.rest ? (double)t.rest[r] : -__builtin_inf();
-  double hi = fmax(fmax(y[0], y[1]), yr);
+  // The largest value is taken off before anything is scaled, and off the rest in one rounding (a fused multiply-add): of a
+  // teacher whose values are all the type's lowest the small differences stay.
+  const float hi = wave_max(fmaxf(v[0], v[1]));
+  const double yr = t.rest ? fma(-(double)hi, inv_t, (double)t.rest[r]) : -__builtin_inf(), shift = fmax(yr, 0.);
+  double y[2];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) hi = fmax(hi, __shfl_xor(hi, o, 64));
-  const double e0 = exp2_series((y[0] - hi) * 1.4426950408889634), e1 = exp2_series((y[1] - hi) * 1.4426950408889634);
-  const double er = exp2_series((yr - hi) * 1.4426950408889634);
+  for (int u = 0; u < 2; ++u) y[u] = v[u] == neg_inf() ? -__builtin_inf() : ((double)v[u] - (double)hi) * inv_t;
+  const double e0 = exp2_series((y[0] - shift) * 1.4426950408889634), e1 = exp2_series((y[1] - shift) * 1.4426950408889634);
+  const double er = exp2_series((yr - shift) * 1.4426950408889634);
   const double sum = wave_sum(e0 + e1) + er;
   const double ls = end_log<LONG>(sum);
   const double inv = end_div<LONG>(1., sum);
@@ -107,14 +109,14 @@ __device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int K, 
     const int j = lane + 64 * u;
     if (j < k) {
       sh.p[j] = (float)((u ? e1 : e0) * inv);
-      sh.logp[j] = y[u] - hi - ls;
+      sh.logp[j] = y[u] - shift - ls;
       // an empty slot takes part in nothing
       sh.c[j] = y[u] == -__builtin_inf() ? -1 : cls[u];
     }
   }
   if (lane == 0) {
     sh.p_rest = er * inv;
-    sh.log_p_rest = yr - hi - ls;
+    sh.log_p_rest = yr - shift - ls;
     sh.state = state;
   }
 }
@@ -503,7 +505,7 @@ __device__ __forceinline__ void few_row(const T* __restrict__ z, const RowShape&
   double a_rest = -__builtin_inf();
   S shift = 0;
   if constexpr (REST) {
-    a_rest = (double)rest * 1.4426950408889634 - (double)hi * scale_d;
+    a_rest = fma(-(double)hi, inv_t, (double)rest) * 1.4426950408889634;     // one rounding before the large parts cancel
     shift = (S)fmax(a_rest, 0.);
   }
   w.p_rest = REST ? few_exp((S)a_rest, shift, 1.f, 1.) : (S)0;
@@ -700,7 +702,7 @@ k_distill_lane_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, 
       const double sum = left.s * to_m + (in.m == neg_inf() ? in.s : in.s * exp2_series(((double)in.m - (double)m) * scale_d));
       double a_rest = -__builtin_inf(), shift = 0.;
       if constexpr (REST) {
-        a_rest = (double)t.rest[r] * 1.4426950408889634 - (double)hi * scale_d;
+        a_rest = fma(-(double)hi, inv_t, (double)t.rest[r]) * 1.4426950408889634;
         shift = fmax(a_rest, 0.);
       }
       const double e_rest = REST ? exp2_series(a_rest - shift) : 0.;
@@ -776,7 +778,7 @@ k_distill_lane_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, 
       float hi = neg_inf(), shift = 0.f, sum = 0.f;
       each_slot(t, at, K, [&](int, float v, int) { hi = fmaxf(hi, v); });
       if (t.rest) {
-        const float a_rest = (float)(((double)t.rest[r] - (double)hi * inv_t) * 1.4426950408889634);
+        const float a_rest = (float)(fma(-(double)hi, inv_t, (double)t.rest[r]) * 1.4426950408889634);
         shift = fmaxf(a_rest, 0.f);
         sum = exp2_f(a_rest - shift);
       }

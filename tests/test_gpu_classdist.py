@@ -375,6 +375,23 @@ def test_distill_makes_bad_rows_nan(K):
         assert torch.isnan(out[4]) and torch.isfinite(out[5])
 
 
+@pytest.mark.parametrize("T", [0.25, 1.0, 8.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K, times", [(2, 1), (6, 1), (16, 700), (40, 1), (40, 2100), (1001, 1), (3001, 1), (20000, 1)])
+def test_distill_teacher_of_lowest_values(K, times, dtype, T):
+    """A teacher's row that its mask left at the type's lowest value: the listed classes and the rest share alike, as what
+    the call is given says (rest is fp32: ln K is lost in it)."""
+    z = logits(4, K, dtype, K, 2.0)
+    t = torch.full((4, K), torch.finfo(dtype).min / 16).to(dtype)      # its quotient by 1/4 is still a fp32 number
+    t[2, :1] = 1.0
+    t[3] = -1e30
+    for k in {1, 2, min(K, 6)}:
+        v, i, rest = teacher_of(t, k, T)
+        for reduction in ("mean", "none"):
+            check_distill(z, v, i, rest, None, T, reduction, times=times)
+            check_distill(z, v, i, None, None, T, reduction, times=times)
+
+
 @pytest.mark.parametrize("rows, K", [(50, 6), (9000, 40), (50, 40), (5, 3000)])
 @pytest.mark.parametrize("itype", [torch.int32, torch.int64])
 def test_distill_slots_rewritten_before_the_backward(rows, K, itype):
