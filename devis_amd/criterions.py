@@ -220,6 +220,8 @@ def _distill_backward(ctx, g):
     *ts, scratch = ctx.saved_tensors
     params, channels_last, rows, dev, places = ctx.call
     if _places(ts) != places:                     # moved by saved-tensor hooks
+        if not ops.distill_keeps_stats(params):   # nor may the backward want any: adjacent rows do not
+            ts = [None if t is None else t.contiguous() for t in ts]
         params, dev, _, ts = ops.distill_params(*ts, channels_last, params.temperature, params.mean)
     if g.dtype != torch.float32 or not g.is_contiguous():
         g = g.contiguous().float()

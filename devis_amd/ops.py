@@ -1096,6 +1096,10 @@ def distill_fwd(params, dev: torch.device, shape, x: Tensor, rows: bool, want_st
     return loss, scratch
 
 
+def distill_keeps_stats(params) -> bool:
+    return _lib.load().devis_distill_stats_bytes(C.byref(params)) > 0
+
+
 def distill_bwd(params, dev: torch.device, x: Tensor, channels_last: bool, scratch: Tensor, grad: Tensor,
                 grad_rows: bool) -> Tensor:
     with _on_device(dev):

@@ -498,6 +498,29 @@ def test_distill_saved_tensors_moved_to_the_host_and_back():
             assert torch.equal(want, zd.grad)
 
 
+def test_distill_saved_tensors_come_back_far_apart():
+    """Rows of few classes keep nothing for the backward; where hooks return them further apart than the kernels of few
+    classes reach, they are brought together."""
+    from devis_amd import criterions
+    z, v, i, r = pair(5, 4, 2, 1.0, torch.float32, 11)
+    dev = [x.cuda() for x in (z, v, i, r)]
+
+    def back(t):
+        if t.shape != z.shape:
+            return t
+        far = torch.zeros(5 * ((1 << 20) + 8), device="cuda", dtype=t.dtype).as_strided(t.shape, ((1 << 20) + 8, 1))
+        return far.copy_(t)
+
+    got = []
+    for unpack in (lambda t: t, back):
+        x = dev[0].clone().requires_grad_(True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), unpack):
+            loss = criterions.distill_top_loss(x, dev[1], dev[2], dev[3])
+        loss.backward()
+        got.append(x.grad)
+    assert torch.equal(*got)
+
+
 def test_distill_refuses_a_second_derivative():
     from devis_amd import criterions
     z, v, i, r = pair(3, 20, 2, 1.0, torch.float32, 8)
