@@ -397,33 +397,51 @@ k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
 }
 
 // ---- few classes: one thread a row, everything in registers, nothing kept for the backward.  For a mean and for
-// the gradient exponentials and logarithms are fp32 (FEW_ROW_LOSS below: fp64); a row's loss is put together from
-//   T (log p_j - log q_j) = (t_j - t_max) - (z_j - z_max) + T log(S_student / S_teacher),
-// where the large parts have cancelled before anything is rounded.  Sums over rows are fp64.  2 x 128^3 x 4 bf16, two slots
-// and rest: 30 us forward, 29 backward (75 and 109 MB; VALU issue is 84 and 92 % busy: ~190 instructions a row).
+// the gradient exponentials and logarithms are fp32 (FEW_ROW_LOSS below: fp64).  Sums over rows are fp64.
 __device__ __forceinline__ float log2_f(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ float rcp_f(float x) { return __builtin_amdgcn_rcpf(x); }
 
 // a sum of shares of numbers in range stays in range where rounding alone would carry it past the largest (a student's mask
 // of the type's lowest value on a listed class); NaN stays
 __device__ __forceinline__ float in_range(float x) { return x > 3.4028235e38f ? 3.4028235e38f : x; }
-__device__ __forceinline__ double in_range(double x) { return x; }
 
-template <int KT>
-__device__ __forceinline__ float pick_class(const float (&x)[KT], int c) {
-  float v = 0.f;
+// x[c], and ec = e[c]; -inf and 0 of an empty slot
+template <int KT, typename S>
+__device__ __forceinline__ float pick_class(const float (&x)[KT], int c, const S (&e)[KT], S& ec) {
+  float v = neg_inf();
+  ec = 0;
 #pragma unroll
   for (int i = 0; i < KT; ++i) {
     const float xi = x[i];
-    if (c == i) v = xi;
+    const S ei = e[i];
+    if (c == i) { v = xi; ec = ei; }
   }
   return v;
 }
 
+// p (r - 1 - log r) times T, of a finite d = T log(p / q): by its series where q and p are near (what is left out is 4e-8 of
+// it), otherwise as it stands
+__device__ __forceinline__ float kl_part(float p, float q, float d, float temperature, float inv_t) {
+  const float l = d * inv_t, pd = p * d;
+  float s = -1.f / 362880.f;
+  s = fmaf(s, l, 1.f / 40320.f);
+  s = fmaf(s, l, -1.f / 5040.f);
+  s = fmaf(s, l, 1.f / 720.f);
+  s = fmaf(s, l, -1.f / 120.f);
+  s = fmaf(s, l, 1.f / 24.f);
+  s = fmaf(s, l, -1.f / 6.f);
+  s = fmaf(s, l, 0.5f);
+  return fabsf(l) <= 0.5f ? pd * (l * s) : fmaf(temperature, q - p, pd);
+}
+
 // What few_row works out.  A row's own loss is what is left when logarithms cancel (a student near its teacher at a high
-// temperature: 0.02 of numbers near 1), so for it everything is fp64; in a mean over many rows the roundings of fp32
-// average out, and in the gradient they stay at the shares' own size.  8 x 64^3 voxels of 9 classes at temperature 4: the
-// rows' losses are off by 2.4e-6 relative in fp32.
+// temperature: 0.02 of numbers near 1), so for it everything is fp64.  Of many rows that would be half of the step, and fp32
+// differences of logarithms would not do: what rounds alike in every row - a constant, a sum - is a bias of their mean (9
+// classes, temperature 4, losses of 2e-5: 4e-3 of it).  A mean is fp32 and adds up, for each of the row's classes (the
+// rest is one),
+//   p (r - 1 - log r),  r = q / p,   instead of   -p log r:
+// the same total, because the p and the q each sum to one, of terms that are never negative and do not cancel; and an error e
+// that all log r of a row share, as that of a logarithm of a sum, changes the total by sum p (r - 1) e = 0 and e^2 / 2.
 enum { FEW_GRADIENT, FEW_MEAN_LOSS, FEW_ROW_LOSS };
 
 // KS bounds the slots as KT bounds the classes; S is the type of shares and sums.
@@ -439,6 +457,7 @@ template <int KT, int KS, typename S> struct FewRow {
   S p_rest;
   S off;                       // with a loss: log2(S_student / S_teacher), both against their own maxima
   S off_rest;                  // with a loss: log2(p_rest / q_rest)
+  unsigned twice;              // classes in two slots
 };
 
 __device__ __forceinline__ float few_exp(float x, float ref, float scale, double) { return exp2_f((x - ref) * scale); }
@@ -459,7 +478,7 @@ __device__ __forceinline__ void few_row(const T* __restrict__ z, const RowShape&
   const uint32_t slot = lane * (uint32_t)t.o.sV;
   // every load first, raw: nothing is looked at before all of them are on their way.  Slots behind the last read the last.
   lane_load_row<T, KT, FULL>(z + n * s.sN + v0 * s.sV, lane * (uint32_t)s.sV, s.sK, K, w.x);
-  const float rest = REST ? lane_load(t.rest + r0, lane) : neg_inf();
+  const float rest = REST && t.rest ? lane_load(t.rest + r0, lane) : neg_inf();
   const unsigned keep = t.mask ? lane_load(t.mask + r0, lane) : 1u;
   const bool wide = t.value_kind == DEVIS_F32;
   uint32_t raw[KS];
@@ -488,7 +507,7 @@ __device__ __forceinline__ void few_row(const T* __restrict__ z, const RowShape&
   }
   float hi = neg_inf();
   bool bad = false;
-  w.listed = 0;
+  w.listed = w.twice = 0;
 #pragma unroll
   for (int j = 0; j < KS; ++j) {
     w.a[j] = __builtin_bit_cast(float, raw[j] << (wide ? 0 : 16));
@@ -496,10 +515,12 @@ __device__ __forceinline__ void few_row(const T* __restrict__ z, const RowShape&
     const bool filled = w.a[j] != neg_inf();
     bad = bad || (filled && (unsigned)w.c[j] >= (unsigned)K);
     w.c[j] = filled ? w.c[j] & (FEW_CLASSES - 1) : FEW_CLASSES;
+    if constexpr (WANT == FEW_MEAN_LOSS) w.twice |= w.listed & (1u << w.c[j]);
     w.listed |= 1u << w.c[j];
     hi = fmaxf(hi, w.a[j]);
   }
   w.listed &= (1u << FEW_CLASSES) - 1;
+  w.twice &= (1u << FEW_CLASSES) - 1;
   w.state = w.listed == 0 || keep == 0 ? 0 : bad ? 2 : 1;
   // teacher, in base 2 against its largest logarithm
   double a_rest = -__builtin_inf();
@@ -553,7 +574,8 @@ __device__ __forceinline__ void few_row(const T* __restrict__ z, const RowShape&
   }
 }
 
-template <typename T, int KT, int KS, bool FULL, bool REST, bool ROWS>
+// (without rest its share of the teacher is zero, and what the student gives those classes still counts)
+template <typename T, int KT, int KS, bool FULL, bool ROWS>
 __global__ void __launch_bounds__(256)
 k_distill_few_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
                   float* __restrict__ per_row, double* __restrict__ partial) {
@@ -569,20 +591,45 @@ k_distill_few_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
       const uint32_t lane = lane_id();
       if (v0 + lane >= s.V) continue;
       FewRow<KT, KS, S> w;
-      few_row<T, KT, KS, FULL, REST, ROWS ? FEW_ROW_LOSS : FEW_MEAN_LOSS>(z, s, t, n, v0, lane, scale, inv_t, w);
+      few_row<T, KT, KS, FULL, true, ROWS ? FEW_ROW_LOSS : FEW_MEAN_LOSS>(z, s, t, n, v0, lane, scale, inv_t, w);
       S sum = 0;
       bool barred = false;                     // a listed class has probability zero
+      if constexpr (ROWS) {
 #pragma unroll
-      for (int j = 0; j < KS; ++j) {
-        const float x = pick_class(w.x, w.c[j]);
-        const S d = x == neg_inf() ? (S)__builtin_inff() : w.off * unit + ((S)w.a[j] - ((S)x - (S)w.m));
-        barred = barred || (d == (S)__builtin_inff() && w.p[j] != (S)0);
-        sum += w.p[j] == (S)0 ? (S)0 : w.p[j] * d;
-      }
-      sum = barred ? +sum : in_range(sum);
-      if constexpr (REST) {
+        for (int j = 0; j < KS; ++j) {
+          S e;
+          const float x = pick_class(w.x, w.c[j], w.e, e);
+          const S d = x == neg_inf() ? (S)__builtin_inff() : w.off * unit + ((S)w.a[j] - ((S)x - (S)w.m));
+          barred = barred || (d == (S)__builtin_inff() && w.p[j] != (S)0);
+          sum += w.p[j] == (S)0 ? (S)0 : w.p[j] * d;
+        }
         const S d = w.sum_rest == (S)0 ? (S)__builtin_inff() : w.off_rest * unit;
         sum += w.p_rest == (S)0 ? (S)0 : w.p_rest * d;
+      } else {
+        const float inv = w.sum == 0.f ? 0.f : rcp_f(w.sum);
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          float e;
+          const float x = pick_class(w.x, w.c[j], w.e, e);
+          const bool none = x == neg_inf();
+          barred = barred || (none && w.p[j] != 0.f);
+          sum += kl_part(w.p[j], e * inv, none ? 0.f : fmaf(w.off, unit, w.a[j] - (x - w.m)), temperature, (float)inv_t);
+        }
+        if (w.twice) {                         // the q of a class in two slots has been added twice
+#pragma unroll
+          for (int j = 1; j < KS; ++j) {
+            float e;
+            bool again = false;
+#pragma unroll
+            for (int i = 0; i < j; ++i) again = again || w.c[i] == w.c[j];
+            pick_class(w.x, w.c[j], w.e, e);
+            sum -= again && w.c[j] != FEW_CLASSES ? temperature * (e * inv) : 0.f;
+          }
+        }
+        sum = barred ? sum + __builtin_inff() : in_range(sum);
+        const float q = w.sum_rest * w.to_m * inv;
+        const float part = kl_part(w.p_rest, q, w.off_rest * unit, temperature, (float)inv_t);
+        sum += w.p_rest == 0.f ? temperature * q : w.sum_rest == 0.f ? __builtin_inff() : part;
       }
       float loss = (float)(sum * (S)temperature);              // the terms are T (log p - log q)
       loss = w.state == 1 ? loss : w.state ? __builtin_nanf("") : 0.f;
@@ -824,18 +871,16 @@ static bool distill_args_ok(const devis_distill_params* a, const void* logits) {
 
 using namespace devis;
 
-// KERNEL(KT, KS, FULL, REST); the slots are bounded at 2, 4 or the classes, because they are half of the work of a row
-#define DISTILL_FEW_FULL(KERNEL, KT, KS, REST) do { if (unit && a->K == KT) KERNEL(KT, KS, true, REST); else KERNEL(KT, KS, false, REST); } while (0)
-#define DISTILL_FEW_KS(KERNEL, KT, REST) do { if (a->k <= 2) DISTILL_FEW_FULL(KERNEL, KT, 2, REST); else if (a->k <= 4) DISTILL_FEW_FULL(KERNEL, KT, 4, REST); else DISTILL_FEW_FULL(KERNEL, KT, KT, REST); } while (0)
-#define DISTILL_FEW_KT(KERNEL, REST)                                                                              \
+// KERNEL(KT, KS, FULL, FLAG); the slots are bounded at 2, 4 or the classes, because they are half of the work of a row
+#define DISTILL_FEW_FULL(KERNEL, KT, KS, FLAG) do { if (unit && a->K == KT) KERNEL(KT, KS, true, FLAG); else KERNEL(KT, KS, false, FLAG); } while (0)
+#define DISTILL_FEW_KS(KERNEL, KT, FLAG) do { if (a->k <= 2) DISTILL_FEW_FULL(KERNEL, KT, 2, FLAG); else if (a->k <= 4) DISTILL_FEW_FULL(KERNEL, KT, 4, FLAG); else DISTILL_FEW_FULL(KERNEL, KT, KT, FLAG); } while (0)
+#define DISTILL_FEW_KT(KERNEL, FLAG)                                                                              \
   do {                                                                                                            \
-    if (a->K <= 2) DISTILL_FEW_FULL(KERNEL, 2, 2, REST);                                                          \
-    else if (a->K <= 4) DISTILL_FEW_KS(KERNEL, 4, REST);                                                          \
-    else if (a->K <= 8) DISTILL_FEW_KS(KERNEL, 8, REST);                                                          \
-    else DISTILL_FEW_KS(KERNEL, 16, REST);                                                                        \
+    if (a->K <= 2) DISTILL_FEW_FULL(KERNEL, 2, 2, FLAG);                                                          \
+    else if (a->K <= 4) DISTILL_FEW_KS(KERNEL, 4, FLAG);                                                          \
+    else if (a->K <= 8) DISTILL_FEW_KS(KERNEL, 8, FLAG);                                                          \
+    else DISTILL_FEW_KS(KERNEL, 16, FLAG);                                                                        \
   } while (0)
-#define DISTILL_DISPATCH_FEW(KERNEL) \
-  DEVIS_DISPATCH_DTYPE(a->dtype, { if (a->rest) DISTILL_FEW_KT(KERNEL, true); else DISTILL_FEW_KT(KERNEL, false); })
 
 #define DISTILL_DISPATCH(KERNEL, ...)                                                                             \
   DEVIS_DISPATCH_DTYPE(a->dtype, {                                                                                \
@@ -876,10 +921,8 @@ int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* 
     if (one_stride(s) && one_stride(t.o)) { merge_rows(s); merge_rows(t.o); }
     const dim3 grid = few_grid(s.N, s.V, DIS_MAX_BLOCKS);
     parts = (int64_t)grid.x * grid.y;
-#define LAUNCH_FEW_R(KT, KS, FULL, REST, ROWS) hipLaunchKernelGGL((k_distill_few_fwd<T, KT, KS, FULL, REST, ROWS>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, per_row, part)
-#define LAUNCH_FEW(KT, KS, FULL, REST) do { if (per_row) LAUNCH_FEW_R(KT, KS, FULL, REST, true); else LAUNCH_FEW_R(KT, KS, FULL, REST, false); } while (0)
-    DISTILL_DISPATCH_FEW(LAUNCH_FEW);
-#undef LAUNCH_FEW
+#define LAUNCH_FEW_R(KT, KS, FULL, ROWS) hipLaunchKernelGGL((k_distill_few_fwd<T, KT, KS, FULL, ROWS>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, per_row, part)
+    DEVIS_DISPATCH_DTYPE(a->dtype, { if (per_row) DISTILL_FEW_KT(LAUNCH_FEW_R, true); else DISTILL_FEW_KT(LAUNCH_FEW_R, false); });
 #undef LAUNCH_FEW_R
   } else if (lane_rows(a->N * a->V, a->K, a->k)) {
     const int64_t blocks = cdiv(a->N * a->V, 256);
@@ -919,7 +962,7 @@ int devis_distill_bwd(const devis_distill_params* a, const void* logits, const v
     if (one_stride(s) && one_stride(t.o) && one_stride(d)) { merge_rows(s); merge_rows(t.o); merge_rows(d); }
     const dim3 grid = few_grid(s.N, s.V, 8192);
 #define LAUNCH_FEW(KT, KS, FULL, REST) hipLaunchKernelGGL((k_distill_few_bwd<T, KT, KS, FULL, REST>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, scal, grad, grad_rows, (T*)dlogits, d)
-    DISTILL_DISPATCH_FEW(LAUNCH_FEW);
+    DEVIS_DISPATCH_DTYPE(a->dtype, { if (a->rest) DISTILL_FEW_KT(LAUNCH_FEW, true); else DISTILL_FEW_KT(LAUNCH_FEW, false); });
 #undef LAUNCH_FEW
     return launch_status();
   }
