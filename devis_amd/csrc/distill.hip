@@ -765,7 +765,8 @@ k_distill_lane_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, 
       const double sum_t = e_all + e_rest, inv_sum_t = 1. / sum_t, off = log2_newton(sum) - log2_newton(sum_t) - shift;
       const double p_rest = e_rest * inv_sum_t;
       // infinite where a listed class has probability zero, whatever else is added
-      double kl = inv_sum_t * (terms == __builtin_inf() ? terms : fma(e_all * off, unit, terms));
+      // (shares that are all zero add nothing, though a student that may use no class has no logarithm)
+      double kl = e_all == 0. ? 0. : inv_sum_t * (terms == __builtin_inf() ? terms : fma(e_all * off, unit, terms));
       if constexpr (REST) {
         const double d = left.s == 0. ? __builtin_inf() : unit * ((a_rest - d_rest) + (off - log2_newton(left.s)));
         kl += p_rest == 0. ? 0. : p_rest * d;
