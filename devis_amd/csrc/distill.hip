@@ -33,9 +33,32 @@ struct RowStats { float ref, w, m, inv_s; };  // gradient of a class in no slot:
 
 // The ends of a row: fp64 for long rows.  Of the short ones of a wave each there are many, and the library's fp64 functions
 // would cost more than the row: logarithms by a Newton step, exponentials and quotients in fp32.
-template <bool LONG> __device__ __forceinline__ double end_log(double x) { return LONG || !(x > 0.) ? log(x) : 0.6931471805599453 * log2_newton(x); }
+template <bool LONG> __device__ __forceinline__ double end_log2(double x) { return LONG || !(x > 0.) ? log2(x) : log2_newton(x); }
 template <bool LONG> __device__ __forceinline__ double end_exp2(double x) { return LONG ? exp2(x) : (double)exp2_f((float)x); }
 template <bool LONG> __device__ __forceinline__ double end_div(double a, double b) { return LONG ? a / b : a * (double)(1.f / (float)b); }
+
+// What a class adds to a row's divergence, from the logarithms (base 2) of its shares p and q:  p (r - 1 - log r),  r = q / p.
+// The listed classes and the rest have shares that sum to one on both sides, so these add up to sum p log(p / q); but they are
+// never negative, nothing cancels among them, and an error e that every log q of the row has in common - its sum of fp32
+// exponentials, whose constant log2(e) / T rounds the same way in every row - changes the total by sum (q - p) e = 0 and
+// e^2 / 2 instead of e.  The series is for |log r| <= 1/2; what it leaves out is 2e-9 of it.
+__device__ __forceinline__ double kl_part(double log2_p, double log2_q) {
+  const double p = exp2_series(log2_p), l = (log2_q - log2_p) * 0.6931471805599453;
+  if (p != 0. && fabs(l) <= 0.5) {
+    double s = 1. / 3628800.;
+    s = fma(s, l, 1. / 362880.);
+    s = fma(s, l, 1. / 40320.);
+    s = fma(s, l, 1. / 5040.);
+    s = fma(s, l, 1. / 720.);
+    s = fma(s, l, 1. / 120.);
+    s = fma(s, l, 1. / 24.);
+    s = fma(s, l, 1. / 6.);
+    s = fma(s, l, 0.5);
+    return p * (l * l * s);
+  }
+  const double q = exp2_series(log2_q);
+  return p == 0. ? q : q - fma(p, l, p);
+}
 
 struct Teacher {
   const void* values; const void* indices; const float* rest; const uint8_t* mask;
@@ -58,10 +81,9 @@ __device__ __forceinline__ float slot_value(const Teacher& t, int64_t i) {
 __device__ __forceinline__ RowStats not_counted() { return RowStats{__builtin_inff(), 0.f, 0.f, 0.f}; }
 
 struct SlotShared {
-  double logp[DIS_MAX_K];      // logarithm of each slot's share
+  double logp[DIS_MAX_K];      // logarithm (base 2) of each slot's share
   float p[DIS_MAX_K];          // its share
   int c[DIS_MAX_K];            // its class, -1 for an empty slot
-  int at[DIS_MAX_K];           // the same, before the shares are known (slot_classes)
   double p_rest, log_p_rest;
   int state;                   // 0 row not counted (masked, or every slot empty), 1 counted, 2 a slot names no class
 };
@@ -99,48 +121,47 @@ __device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int K, 
   double y[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) y[u] = v[u] == neg_inf() ? -__builtin_inf() : ((double)v[u] - (double)hi) * inv_t;
-  const double e0 = exp2_series((y[0] - shift) * 1.4426950408889634), e1 = exp2_series((y[1] - shift) * 1.4426950408889634);
-  const double er = exp2_series((yr - shift) * 1.4426950408889634);
+  y[0] = (y[0] - shift) * 1.4426950408889634;
+  y[1] = (y[1] - shift) * 1.4426950408889634;
+  const double e0 = exp2_series(y[0]), e1 = exp2_series(y[1]), y_rest = (yr - shift) * 1.4426950408889634, er = exp2_series(y_rest);
   const double sum = wave_sum(e0 + e1) + er;
-  const double ls = end_log<LONG>(sum);
+  const double ls = end_log2<LONG>(sum);
   const double inv = end_div<LONG>(1., sum);
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int j = lane + 64 * u;
     if (j < k) {
       sh.p[j] = (float)((u ? e1 : e0) * inv);
-      sh.logp[j] = y[u] - shift - ls;
+      sh.logp[j] = y[u] - ls;
       // an empty slot takes part in nothing
       sh.c[j] = y[u] == -__builtin_inf() ? -1 : cls[u];
     }
   }
   if (lane == 0) {
     sh.p_rest = er * inv;
-    sh.log_p_rest = yr - shift - ls;
+    sh.log_p_rest = y_rest - ls;
     sh.state = state;
   }
 }
 
-// the classes of the filled slots, by the whole block
-template <int BS> __device__ __forceinline__ void slot_classes(const Teacher& t, int64_t r, int K, int tid, SlotShared& sh) {
-  const int64_t at = row_offset(t.o, r);
-  for (int j = tid; j < t.o.K; j += BS) {
-    const int64_t i = at + j * t.o.sK;
-    const int c = class_at(t.indices, t.index_kind, i);
-    sh.at[j] = slot_value(t, i) == neg_inf() || c >= K ? -1 : c;
-  }
+// the class of slot j, -1 for an empty one
+__device__ __forceinline__ int slot_class(const Teacher& t, int64_t at, int j, int K) {
+  const int64_t i = at + j * t.o.sK;
+  const int c = class_at(t.indices, t.index_kind, i);
+  return slot_value(t, i) == neg_inf() || c >= K ? -1 : c;
 }
 
 __device__ __forceinline__ bool row_masked(const Teacher& t, int64_t r) { return t.mask && t.mask[r] == 0; }
 
-template <typename T, bool UNIT, bool REST, int BS>
+// (without rest its share of the teacher is zero, and the student's share of those classes is summed apart all the same)
+template <typename T, bool UNIT, int BS>
 __global__ void __launch_bounds__(BS, BS == 256 ? 8 : BS == 1024 ? 4 : 1)
 k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, double t2, RowStats* __restrict__ stats,
               float* __restrict__ per_row, double* __restrict__ partial) {
   constexpr bool LONG = BS > 64;
   __shared__ SlotShared sh;
   constexpr int SEG = dis_seg<BS>();
-  __shared__ uint32_t s_bits[REST ? SEG / 32 : 1];
+  __shared__ uint32_t s_bits[SEG / 32];
   __shared__ double s_red[BS / 64];
   __shared__ float s_max[BS / 64];
   const int K = s.K;
@@ -152,6 +173,12 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
   for (int64_t r = first_row; r < NV; r += gridDim.x) {
     const int tid = lane_id();
     const T* p = z + row_offset(s, r);
+    // the slots' classes, wanted first of all for their bits, and the mask come in together
+    constexpr int OWN = BS < DIS_MAX_K ? DIS_MAX_K / BS : 1;
+    const int64_t slots = row_offset(t.o, r);
+    int own[OWN];
+#pragma unroll
+    for (int u = 0; u < OWN; ++u) own[u] = tid + u * BS < t.o.K ? slot_class(t, slots, tid + u * BS, K) : -1;
     if (row_masked(t, r)) {
       if (tid == 0) {
         if (per_row) per_row[r] = 0.f;
@@ -160,11 +187,8 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
       if (LONG) break;
       continue;
     }
-    // The first wave works out the teacher's shares, which nobody needs before the end, while the others begin; only
-    // the slots' classes are wanted first, for their bits.
-    if constexpr (REST) slot_classes<BS>(t, r, K, tid, sh);
     if (tid < 64) teacher_row<LONG>(t, r, K, inv_t, tid, sh);
-    // running maximum and sum of the classes in no slot (all classes without REST)
+    // running maximum and sum of the classes in no slot
     float m = neg_inf(), acc = 0.f;
     const auto absorb = [&](auto& x) {
       constexpr int N = sizeof(x) / sizeof(float);
@@ -177,23 +201,19 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
     };
     for (int lo = 0; lo < K; lo += SEG) {
       const int hi = K - lo < SEG ? K : lo + SEG;
-      if constexpr (REST) {
-        for (int i = tid; i < (hi - lo + 31) / 32; i += BS) s_bits[i] = 0;
-        __syncthreads();
-        for (int j = tid; j < t.o.K; j += BS) {
-          const int c = sh.at[j];
-          if (c >= lo && c < hi) atomicOr(&s_bits[(c - lo) >> 5], 1u << ((c - lo) & 31));
-        }
-        __syncthreads();
-      }
+      for (int i = tid; i < (hi - lo + 31) / 32; i += BS) s_bits[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < OWN; ++u)
+        if (own[u] >= lo && own[u] < hi) atomicOr(&s_bits[(own[u] - lo) >> 5], 1u << ((own[u] - lo) & 31));
+      __syncthreads();
       if constexpr (UNIT) {
         constexpr int VEC = vec_of<T>();
         const T* q = p + lo;
         const int full = (hi - lo) / VEC;
         // the slot bits of vector v: a byte, or half of one
         const auto bits = [&](int v) -> uint32_t {
-          if constexpr (!REST) return 0;
-          else if constexpr (VEC == 8) return ((const uint8_t*)s_bits)[v];
+          if constexpr (VEC == 8) return ((const uint8_t*)s_bits)[v];
           else return (((const uint8_t*)s_bits)[v >> 1] >> ((v & 1) * 4)) & 15u;
         };
         int v = tid;
@@ -203,13 +223,11 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
           uint32_t b = 0;
 #pragma unroll
           for (int u = 0; u < 4; ++u) raw[u] = load16(q + (int64_t)(v + u * BS) * VEC);
-          if constexpr (REST) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) b |= bits(v + u * BS) << (u * VEC);
-          }
+          for (int u = 0; u < 4; ++u) b |= bits(v + u * BS) << (u * VEC);
 #pragma unroll
           for (int u = 0; u < 4; ++u) unpack(raw[u], *(float(*)[VEC])(x + u * VEC));
-          if (REST && b) {
+          if (b) {
 #pragma unroll
             for (int i = 0; i < 4 * VEC; ++i) x[i] = (b >> i) & 1u ? neg_inf() : +x[i];
           }
@@ -219,35 +237,34 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
           float x[VEC];
           unpack(load16(q + (int64_t)v * VEC), x);
           const uint32_t b = bits(v);
-          if (REST && b) {
+          if (b) {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) x[i] = (b >> i) & 1u ? neg_inf() : +x[i];
           }
           absorb(x);
         }
         const int c = full * VEC + tid;
-        if (c < hi - lo && !(REST && (s_bits[c >> 5] >> (c & 31)) & 1u)) {
+        if (c < hi - lo && !((s_bits[c >> 5] >> (c & 31)) & 1u)) {
           float x[1] = {(float)q[c]};
           absorb(x);
         }
       } else {
         for (int c = lo + tid; c < hi; c += BS) {
           float x[1] = {(float)p[(int64_t)c * s.sK]};
-          if (REST && (s_bits[(c - lo) >> 5] >> ((c - lo) & 31)) & 1u) continue;
+          if ((s_bits[(c - lo) >> 5] >> ((c - lo) & 31)) & 1u) continue;
           absorb(x);
         }
       }
-      if constexpr (REST) __syncthreads();
+      __syncthreads();
     }
     const float m_rest = block_max<BS>(m, s_max);              // (its barrier also ends the wait for the teacher's shares)
     const float ref = m_rest == neg_inf() ? 0.f : m_rest;
-    double sum_rest = block_sum<BS>(m == neg_inf() ? (double)acc : (double)acc * (double)exp2_f((m - ref) * scale), s_red);
+    const double sum_rest = block_sum<BS>(m == neg_inf() ? (double)acc : (double)acc * (double)exp2_f((m - ref) * scale), s_red);
     if (threadIdx.x < 64) {
       const int tid = lane_id();
       // the listed classes' logits; a class in two slots counts once in the student's sum (its first slot)
       float x[2];
       bool first[2];
-      float m_all = m_rest;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int j = tid + 64 * u;
@@ -255,33 +272,28 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
         first[u] = false;
         if (j < t.o.K && sh.c[j] >= 0) {
           x[u] = (float)p[(int64_t)sh.c[j] * s.sK];
-          if constexpr (REST) {
-            bool again = false;
+          bool again = false;
 #pragma unroll 8
-            for (int i = 0; i < j; ++i) again |= sh.c[i] == sh.c[j];
-            first[u] = !again;
-          }
+          for (int i = 0; i < j; ++i) again |= sh.c[i] == sh.c[j];
+          first[u] = !again;
         }
       }
-      double sum = sum_rest;
-      if constexpr (REST) {
-        m_all = fmaxf(m_rest, wave_max(fmaxf(x[0], x[1])));
-        const float ra = m_all == neg_inf() ? 0.f : m_all;
-        double mine = 0.;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) if (first[u]) mine += (double)exp2_f((x[u] - ra) * scale);
-        sum = wave_sum(mine) + (m_rest == neg_inf() ? sum_rest : sum_rest * end_exp2<LONG>(((double)m_rest - (double)ra) * inv_t * 1.4426950408889634));
-      }
+      const float m_all = fmaxf(m_rest, wave_max(fmaxf(x[0], x[1])));
       const double m_d = m_all == neg_inf() ? 0. : (double)m_all;
-      const double ls = end_log<LONG>(sum);   // log q = (x - m)/T - ls: the large part cancels first
+      double mine = 0.;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) if (first[u]) mine += (double)exp2_f((x[u] - (float)m_d) * scale);
+      const double to_m = m_rest == neg_inf() ? 0. : end_exp2<LONG>(((double)m_rest - m_d) * inv_t * 1.4426950408889634);
+      const double sum = wave_sum(mine) + (m_rest == neg_inf() ? sum_rest : sum_rest * to_m);
+      const double ls = end_log2<LONG>(sum);  // log q = (x - m)/T - ls: the large part cancels first
       double kl = 0.;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int j = tid + 64 * u;
         if (j < t.o.K && sh.c[j] >= 0) {
-          const double pj = (double)sh.p[j];
-          const double logq = x[u] == neg_inf() ? -__builtin_inf() : ((double)x[u] - m_d) * inv_t - ls;
-          if (!(pj == 0.)) kl += pj * (sh.logp[j] - logq);
+          const double logq = x[u] == neg_inf() ? -__builtin_inf() : ((double)x[u] - m_d) * inv_t * 1.4426950408889634 - ls;
+          kl += kl_part(sh.logp[j], logq);
+          if (!first[u]) kl -= exp2_series(logq);              // the q of a class in two slots counts once
         }
       }
       kl = wave_sum(kl);
@@ -291,15 +303,11 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
         if (stats) stats[r] = sh.state == 2 ? RowStats{0.f, v, 0.f, v} : not_counted();
         if (sh.state == 2) { loss_sum += (double)v; ++count; }
       } else if (tid == 0) {
-        const double pr = sh.p_rest;
-        double inv = sum > 0. ? end_div<LONG>(1., sum) : sum == 0. ? 0. : sum;
-        double w = inv;
-        if constexpr (REST) {
-          const double log_q_rest = sum_rest == 0. ? -__builtin_inf() : ((double)ref - m_d) * inv_t + end_log<LONG>(sum_rest) - ls;
-          if (!(pr == 0.)) kl += pr * (sh.log_p_rest - log_q_rest);
-          // q = exp((z - m_rest)/T) * w before the teacher's share of the rest is taken off
-          w = m_rest == neg_inf() ? 0. : inv * end_exp2<LONG>(((double)m_rest - m_d) * inv_t * 1.4426950408889634) - end_div<LONG>(pr, sum_rest);
-        }
+        const double log_q_rest = sum_rest == 0. ? -__builtin_inf() : ((double)ref - m_d) * inv_t * 1.4426950408889634 + end_log2<LONG>(sum_rest) - ls;
+        kl += kl_part(sh.log_p_rest, log_q_rest);
+        const double inv = sum > 0. ? end_div<LONG>(1., sum) : sum == 0. ? 0. : sum;
+        // q = exp((z - m_rest)/T) * w before the teacher's share of the rest is taken off
+        const double w = m_rest == neg_inf() ? 0. : inv * to_m - end_div<LONG>(sh.p_rest, sum_rest);
         const double loss = t2 * kl;
         if (per_row) per_row[r] = (float)loss;
         if (stats) stats[r] = RowStats{ref, (float)w, (float)m_d, (float)inv};
@@ -692,15 +700,15 @@ __device__ __forceinline__ void each_slot(const Teacher& t, int64_t at, int K, F
   }
 }
 
-template <typename T, bool UNIT, bool REST>
+template <typename T, bool UNIT>
 __global__ void __launch_bounds__(256)
 k_distill_lane_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature,
                    RowStats* __restrict__ stats, float* __restrict__ per_row, double* __restrict__ partial) {
-  __shared__ uint32_t s_bits[REST ? 256 * (LANE_CLASSES / 32 + 1) : 1];       // a row's words, one apart from the next lane's
+  __shared__ uint32_t s_bits[256 * (LANE_CLASSES / 32 + 1)];       // a row's words, one apart from the next lane's
   __shared__ double s_red[4];
-  const double unit = (double)temperature * 0.6931471805599453, scale_d = inv_t * 1.4426950408889634;
+  const double scale_d = inv_t * 1.4426950408889634;
   const int K = s.K, words = (K + 31) / 32;
-  uint32_t* const bits = s_bits + (REST ? threadIdx.x * (LANE_CLASSES / 32 + 1) : 0);
+  uint32_t* const bits = s_bits + threadIdx.x * (LANE_CLASSES / 32 + 1);
   const int64_t NV = s.N * s.V;
   double loss_sum = 0.;
   int count = 0;
@@ -708,14 +716,17 @@ k_distill_lane_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, 
     const T* p = z + row_offset(s, r);
     const int64_t at = row_offset(t.o, r);
     float hi = neg_inf();
-    bool any = false, bad = false;
-    if constexpr (REST) for (int i = 0; i < words; ++i) bits[i] = 0;
+    bool any = false, bad = false, twice = false;
+    for (int i = 0; i < words; ++i) bits[i] = 0;
     if (!row_masked(t, r)) {
       each_slot(t, at, K, [&](int, float v, int c) {
         any = true;
         hi = fmaxf(hi, v);
         if (c < 0 || c >= K) bad = true;
-        else if constexpr (REST) bits[c >> 5] |= 1u << (c & 31);
+        else {
+          twice = twice || ((bits[c >> 5] >> (c & 31)) & 1u);
+          bits[c >> 5] |= 1u << (c & 31);
+        }
       });
     }
     float loss = 0.f;
@@ -724,20 +735,18 @@ k_distill_lane_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, 
       loss = __builtin_nanf("");
       st = RowStats{0.f, loss, 0.f, loss};
     } else if (any) {
-      LaneSum in = {neg_inf(), 0.}, left = {neg_inf(), 0.};                // listed classes, and all others (all, without REST)
+      LaneSum in = {neg_inf(), 0.}, left = {neg_inf(), 0.};                // listed classes, and all others
       for (int c = 0; c < K; c += 8) {
         float x[8];
         load8<T, UNIT>(p, s.sK, c, K, x);
-        if constexpr (REST) {
-          uint32_t b = (bits[c >> 5] >> (c & 31)) & 255u;
-          if (b) {
+        const uint32_t b = (bits[c >> 5] >> (c & 31)) & 255u;
+        if (b) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if ((b >> i) & 1u) {
-                const float xi = x[i];
-                in.add_one(xi, scale);
-                x[i] = neg_inf();
-              }
+          for (int i = 0; i < 8; ++i) {
+            if ((b >> i) & 1u) {
+              const float xi = x[i];
+              in.add_one(xi, scale);
+              x[i] = neg_inf();
             }
           }
         }
@@ -747,33 +756,25 @@ k_distill_lane_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, 
       const float ref = left.m == neg_inf() ? 0.f : left.m;
       const double d_rest = left.m == neg_inf() ? 0. : ((double)left.m - (double)m) * scale_d, to_m = exp2_series(d_rest);
       const double sum = left.s * to_m + (in.m == neg_inf() ? in.s : in.s * exp2_series(((double)in.m - (double)m) * scale_d));
-      double a_rest = -__builtin_inf(), shift = 0.;
-      if constexpr (REST) {
-        a_rest = fma(-(double)hi, inv_t, (double)t.rest[r]) * 1.4426950408889634;
-        shift = fmax(a_rest, 0.);
-      }
-      const double e_rest = REST ? exp2_series(a_rest - shift) : 0.;
-      // the shares are e / (e_all + e_rest): the terms are gathered before their sum is known
-      double e_all = 0., terms = 0.;
-      each_slot(t, at, K, [&](int, float v, int c) {
-        const double a = (double)v - (double)hi, e = exp2_series(fma(a, scale_d, -shift));
+      const double a_rest = t.rest ? fma(-(double)hi, inv_t, (double)t.rest[r]) * 1.4426950408889634 : -__builtin_inf();
+      const double shift = fmax(a_rest, 0.), e_rest = exp2_series(a_rest - shift);
+      double sum_t = e_rest;
+      each_slot(t, at, K, [&](int, float v, int) { sum_t += exp2_series(fma((double)v - (double)hi, scale_d, -shift)); });
+      const double ls_t = log2_newton(sum_t) + shift, ls = log2_newton(sum), p_rest = e_rest / sum_t;
+      double kl = kl_part(a_rest - ls_t, left.s == 0. ? -__builtin_inf() : d_rest + log2_newton(left.s) - ls);
+      each_slot(t, at, K, [&](int j, float v, int c) {
         const float x = (float)p[(int64_t)c * s.sK];
-        const double d = x == neg_inf() ? __builtin_inf() : a - ((double)x - (double)m);
-        e_all += e;
-        terms += e == 0. ? 0. : e * d;
+        const double logq = x == neg_inf() ? -__builtin_inf() : fma((double)x - (double)m, scale_d, -ls);
+        kl += kl_part(fma((double)v - (double)hi, scale_d, -ls_t), logq);
+        if (twice) {                           // the q of a class in two slots counts once
+          bool again = false;
+          each_slot(t, at, K, [&](int j2, float, int c2) { again = again || (j2 < j && c2 == c); });
+          if (again) kl -= exp2_series(logq);
+        }
       });
-      const double sum_t = e_all + e_rest, inv_sum_t = 1. / sum_t, off = log2_newton(sum) - log2_newton(sum_t) - shift;
-      const double p_rest = e_rest * inv_sum_t;
-      // infinite where a listed class has probability zero, whatever else is added
-      // (shares that are all zero add nothing, though a student that may use no class has no logarithm)
-      double kl = e_all == 0. ? 0. : inv_sum_t * (terms == __builtin_inf() ? terms : fma(e_all * off, unit, terms));
-      if constexpr (REST) {
-        const double d = left.s == 0. ? __builtin_inf() : unit * ((a_rest - d_rest) + (off - log2_newton(left.s)));
-        kl += p_rest == 0. ? 0. : p_rest * d;
-      }
-      loss = (float)(kl * (double)temperature);                // the terms are T (log p - log q)
+      loss = (float)(kl * (double)temperature * (double)temperature);
       const float inv = sum == 0. ? 0.f : rcp_f((float)sum);
-      st = RowStats{ref, left.s == 0. ? 0.f : (float)to_m * inv - (REST ? (float)p_rest * rcp_f((float)left.s) : 0.f), m, inv};
+      st = RowStats{ref, left.s == 0. ? 0.f : (float)to_m * inv - (float)p_rest * rcp_f((float)left.s), m, inv};
     }
     if (per_row) per_row[r] = loss;
     if (stats) stats[r] = st;
@@ -883,17 +884,12 @@ using namespace devis;
     else DISTILL_FEW_KS(KERNEL, 16, FLAG);                                                                        \
   } while (0)
 
-#define DISTILL_DISPATCH(KERNEL, ...)                                                                             \
+#define DISTILL_DISPATCH(KERNEL)                                                                                  \
   DEVIS_DISPATCH_DTYPE(a->dtype, {                                                                                \
-    if (!long_rows(a)) {                                                                                          \
-      if (unit) { if (a->rest) KERNEL(true, true, 64); else KERNEL(true, false, 64); }                            \
-      else { if (a->rest) KERNEL(false, true, 64); else KERNEL(false, false, 64); }                               \
-    } else if (unit && few_rows(a)) {                                                                             \
-      if (a->rest) KERNEL(true, true, 1024); else KERNEL(true, false, 1024);                                      \
-    } else {                                                                                                      \
-      if (unit) { if (a->rest) KERNEL(true, true, 256); else KERNEL(true, false, 256); }                          \
-      else { if (a->rest) KERNEL(false, true, 256); else KERNEL(false, false, 256); }                             \
-    }                                                                                                             \
+    if (!long_rows(a)) { if (unit) KERNEL(true, 64); else KERNEL(false, 64); }                                    \
+    else if (unit && few_rows(a)) KERNEL(true, 1024);                                                             \
+    else if (unit) KERNEL(true, 256);                                                                             \
+    else KERNEL(false, 256);                                                                                      \
   })
 
 extern "C" {
@@ -928,14 +924,11 @@ int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* 
   } else if (lane_rows(a->N * a->V, a->K, a->k)) {
     const int64_t blocks = cdiv(a->N * a->V, 256);
     parts = blocks < DIS_MAX_BLOCKS ? blocks : DIS_MAX_BLOCKS;
-#define LAUNCH_LANE(UNIT, REST) hipLaunchKernelGGL((k_distill_lane_fwd<T, UNIT, REST>), dim3((unsigned)parts), dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, (RowStats*)stats, per_row, part)
-    DEVIS_DISPATCH_DTYPE(a->dtype, {
-      if (unit) { if (a->rest) LAUNCH_LANE(true, true); else LAUNCH_LANE(true, false); }
-      else { if (a->rest) LAUNCH_LANE(false, true); else LAUNCH_LANE(false, false); }
-    });
+#define LAUNCH_LANE(UNIT) hipLaunchKernelGGL((k_distill_lane_fwd<T, UNIT>), dim3((unsigned)parts), dim3(256), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, (RowStats*)stats, per_row, part)
+    DEVIS_DISPATCH_DTYPE(a->dtype, { if (unit) LAUNCH_LANE(true); else LAUNCH_LANE(false); });
 #undef LAUNCH_LANE
   } else {
-#define LAUNCH_DISTILL_FWD(UNIT, REST, BS) hipLaunchKernelGGL((k_distill_fwd<T, UNIT, REST, BS>), rows, dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, t2, (RowStats*)stats, per_row, part)
+#define LAUNCH_DISTILL_FWD(UNIT, BS) hipLaunchKernelGGL((k_distill_fwd<T, UNIT, BS>), rows, dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, t2, (RowStats*)stats, per_row, part)
     DISTILL_DISPATCH(LAUNCH_DISTILL_FWD);
   }
 #undef LAUNCH_DISTILL_FWD

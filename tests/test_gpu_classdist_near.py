@@ -62,7 +62,10 @@ def near_pair(rows, K, k, T, noise, dtype, seed):
     return z, v, i, rest
 
 
-SHAPES = [(1, 4, 2), (1, 9, 3), (1, 16, 16), (300, 2, 1), (64, 9, 3), (20000, 4, 2), (20000, 7, 3), (20000, 9, 3), (20000, 12, 12)]
+# rows of few classes; a lane a row; a wave a row; long rows
+SHAPES = [(1, 4, 2), (1, 9, 3), (1, 16, 16), (300, 2, 1), (64, 9, 3), (20000, 4, 2), (20000, 7, 3), (20000, 9, 3), (20000, 12, 12),
+          (9000, 21, 4), (9000, 40, 40), (9000, 100, 12), (1, 100, 5), (300, 300, 20), (300, 1000, 100), (50, 5003, 20), (8, 33001, 16),
+          (300, 9001, 64), (2, 151936, 64)]
 
 
 @pytest.mark.parametrize("noise", [0.1, 0.01, 0.001, 0.0])
@@ -85,7 +88,7 @@ def test_a_student_near_its_teacher(rows, K, k, T, noise):
         assert abs(total - loss.sum().item()) <= tol.sum().item() + E * loss.sum().item()
 
 
-@pytest.mark.parametrize("rows, K, k", [(20000, 4, 2), (20000, 9, 5)])
+@pytest.mark.parametrize("rows, K, k", [(20000, 4, 2), (20000, 9, 5), (9000, 40, 6), (300, 1000, 20), (50, 9001, 30)])
 def test_the_mean_is_the_mean_of_the_rows(rows, K, k):
     """bf16, classes first: both reductions are within their own bounds of the same 64-bit losses, so of each other."""
     from devis_amd import criterions
@@ -103,7 +106,7 @@ def test_the_mean_is_the_mean_of_the_rows(rows, K, k):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("K", [4, 6, 16])
+@pytest.mark.parametrize("K", [4, 6, 16, 40, 3000])
 def test_odd_rows_one_by_one(K, dtype):
     """Empty and repeated slots, masks of the lowest value, barred classes, nothing left outside the list: each row's sum is
     its own loss, whatever form it takes; a NaN on either side makes it NaN."""
