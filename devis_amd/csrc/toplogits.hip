@@ -37,12 +37,12 @@ template <int BS> struct TopShared {
   };
   union {
     struct { float max[top_groups<BS>() * BS + 1], sum[top_groups<BS>() * BS + 1]; } groups;       // wide, until the list is begun
-    uint64_t list[TOP_CAP];
+    struct { uint64_t list[TOP_CAP], left[BS > 64 ? TOP_CAP : 1]; };          // left: what the first k leave of it, by rank
   };
   uint64_t tau, kth;
   double red[BS / 64];
   float max[BS / 64];
-  int n, items;
+  int wave_items[BS / 64], n;
 };
 
 // what becomes of the list: its first k are the answer, the others join the rest (`sum`, against `base`)
@@ -51,7 +51,12 @@ __device__ __forceinline__ void top_finish(const T* __restrict__ p, const RowSha
                                            T* __restrict__ values, I* __restrict__ indices, const RowShape& o,
                                            float* __restrict__ rest, TopShared<BS>& sh, int n, double sum, float base) {
   const int tid = threadIdx.x, K = s.K;
-  // rank the list; what does not make the first k joins the rest
+  // Rank the list; what does not make the first k joins the rest, in the order of its ranks: the list's own order is that in
+  // which the waves came, and sums that followed it would differ from call to call (one wave comes in one order only).
+  const auto to_rest = [&](uint64_t key) {
+    // far above `base` where large classes lie side by side and one thread held them all: past what fp32 holds
+    sum += exp2_series(((double)key_value(key) - (double)base) * inv_t * 1.4426950408889634);
+  };
   for (int i = tid; i < n; i += BS) {
     const uint64_t key = sh.list[i];
     int rank = 0;
@@ -62,10 +67,15 @@ __device__ __forceinline__ void top_finish(const T* __restrict__ p, const RowSha
       values[at_o] = p[(int64_t)c * s.sK];
       indices[at_o] = (I)c;
       if (rank == k - 1) sh.kth = key;
+    } else if (BS > 64) {
+      sh.left[rank] = key;
     } else {
-      // far above `base` where large classes lie side by side and one thread held them all: past what fp32 holds
-      sum += exp2_series(((double)key_value(key) - (double)base) * inv_t * 1.4426950408889634);
+      to_rest(key);
     }
+  }
+  if (BS > 64 && rest && n > k) {
+    __syncthreads();
+    for (int i = k + tid; i < n; i += BS) to_rest(sh.left[i]);
   }
   if (rest) {
     sum = block_sum<BS>(sum, sh.red);
@@ -272,7 +282,7 @@ k_top_wide(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t
   const float x_tail = tail ? nan_high((float)p[c_tail]) : neg_inf();
   best = fmaxf(best, x_tail);
   sh.thread_max[tid] = holds || tail ? (uint32_t)(top_key(best, 0) >> 32) : 0;
-  if (tid == 0) { sh.n = 0; sh.items = 0; }
+  if (tid == 0) sh.n = 0;
   __syncthreads();
   if (tid < 64) {
     // the largest value that at least k threads reach; a bf16 value is in the upper half of its key
@@ -298,17 +308,28 @@ k_top_wide(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t
   const float floor_v = tau ? key_value(tau) : neg_inf();
   float base = floor_v == neg_inf() ? 0.f : floor_v;
   float acc = 0.f;
+  uint32_t hit = 0;                                            // this thread's groups that are read again
   for (int g = 0; g * each < groups; ++g) {
     const float gm = sh.groups.max[g * BS + tid];
-    if (gm >= floor_v) {
-      const int at = atomicAdd(&sh.items, 1);
-      if (at < TOP_ITEMS) s_item[at] = g * BS + tid;
-    } else {
-      acc += sh.groups.sum[g * BS + tid] * exp2_f((gm - base) * scale);
-    }
+    if (gm >= floor_v) hit |= 1u << g;
+    else acc += sh.groups.sum[g * BS + tid] * exp2_f((gm - base) * scale);
   }
+  // their list in the order of the threads: which thread reads which group, and so every sum, is the same in every call
+  int at = 0, in_wave = 0, items = 0;
+  for (int g = 0; g * each < groups; ++g) {
+    const unsigned long long reach = __ballot((hit >> g) & 1u);
+    at += __popcll(reach & ((1ull << (tid & 63)) - 1));
+    in_wave += __popcll(reach);
+  }
+  if ((tid & 63) == 0) sh.wave_items[tid >> 6] = in_wave;
   __syncthreads();
-  const int items = sh.items;
+#pragma unroll
+  for (int i = 0; i < BS / 64; ++i) {
+    at += i < (tid >> 6) ? sh.wave_items[i] : 0;
+    items += sh.wave_items[i];
+  }
+  for (; hit; hit &= hit - 1, ++at) if (at < TOP_ITEMS) s_item[at] = (__ffs(hit) - 1) * BS + tid;
+  __syncthreads();
   bool stalled = items > TOP_ITEMS || !tau;
   if (!stalled) {
     const auto take = [&](float x, int c) {

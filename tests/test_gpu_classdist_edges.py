@@ -22,3 +22,23 @@ def test_a_barred_student_whose_teacher_holds_everything_outside_the_list(rows, 
     (dz,) = torch.autograd.grad(loss, z, torch.ones_like(loss))
     assert (dz[::2] == 0).all() and torch.isfinite(dz).all()
     assert criterions.distill_top_loss(z, v, i, rest).item() == math.inf
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows, K, k, spread", [(1500, 131072, 64, 2.0), (800, 151936, 128, 2.0), (3000, 40000, 128, 0.01), (100, 262147, 128, 0.5),
+                                                (3000, 1031, 100, 1.0), (1000, 20000, 100, 0.0), (2000, 1000, 100, 2.0)])
+def test_top_logits_are_the_same_every_time(rows, K, k, spread, dtype):
+    """Bit for bit: nothing depends on the order in which waves run, whatever is read again, listed and left over."""
+    from devis_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(7)
+    z = (torch.randn((rows, K), generator=g, device="cuda") * spread).to(dtype)
+    z[::3, 100:200] += 30.0                        # more large classes than are kept, side by side
+    strided = z[:64].t().contiguous().t()          # and classes that are not adjacent
+    first = None
+    for _ in range(12):
+        out = [ops.top_logits(x, k, temperature=0.7) for x in (z, strided)]
+        got = [o[n] for o in out for n in ("values", "indices", "rest")]
+        if first is None:
+            first = got
+        else:
+            assert all(torch.equal(a, b) for a, b in zip(first, got))
