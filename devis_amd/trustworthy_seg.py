@@ -103,16 +103,16 @@ class TMSU(nn.Module):
 
     def top_logits(self, X, k, temperature=1.0):
         """This model as a teacher: the k largest logits of every voxel of X and the mass of the others
-        (`ops.top_logits`), channels last.  Runs in eval mode without gradients."""
-        training = self.training
-        if training:
-            self.eval()
+        (`ops.top_logits`), channels last.  Runs in eval mode without gradients; every module keeps the mode it was in."""
+        training = [m for m in self.modules() if m.training]
+        for m in training:
+            m.training = False
         try:
             with torch.no_grad():
                 return ops.top_logits(self.backbone.forward_channels_last(X), k, channels_last=True, temperature=temperature)
         finally:
-            if training:
-                self.train()
+            for m in training:
+                m.training = True
 
     def infer(self, input):
         """softplus evidence of NC(D)HW logits (TrustworthySeg.py:160-166)."""
