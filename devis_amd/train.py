@@ -69,12 +69,14 @@ def getArgs(argv=None):
     # checkpoint as val() writes it, of a model of --teacher_model (default: --model_name) for the same dataset
     p.add_argument('--teacher', default='', type=str)
     p.add_argument('--teacher_model', default='', type=str)
-    p.add_argument('--distill_top', type=int, default=2, help='logits kept of every voxel')
+    p.add_argument('--distill_top', type=int, default=None, help='logits kept of every voxel (default: of every class)')
     p.add_argument('--distill_temperature', type=float, default=2.0)
     p.add_argument('--distill_weight', type=float, default=1.0)
     args = p.parse_args(argv)
     args.compute_dtype = torch.bfloat16 if args.compute_dtype == 'bf16' else torch.float32
     apply_dataset_overrides(args)
+    if args.distill_top is None:
+        args.distill_top = args.num_classes
     return args
 
 

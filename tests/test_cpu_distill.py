@@ -27,3 +27,11 @@ def test_top_logits_leave_every_module_in_its_mode(outer, inner, monkeypatch):
     with pytest.raises(ZeroDivisionError):
         model.top_logits(torch.zeros(1), 2)
     assert [m.training for m in model.modules()] == before
+
+
+def test_the_command_keeps_every_class_of_a_live_teacher():
+    """Nothing is stored of a teacher that runs beside the student, so by default nothing of it is left out."""
+    from devis_amd import train as T
+    for dataset, classes in (("BraTS", 4), ("LiTS", 3), ("HC", 10)):
+        assert T.getArgs(['--dataset', dataset]).distill_top == classes
+    assert T.getArgs(['--dataset', 'HC', '--distill_top', '2']).distill_top == 2
