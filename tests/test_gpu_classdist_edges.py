@@ -42,3 +42,27 @@ def test_top_logits_are_the_same_every_time(rows, K, k, spread, dtype):
             first = got
         else:
             assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows, K, k, T", [(300, 1000, 20, 1.0), (300, 1031, 3, 2.0), (200, 9001, 128, 1.0), (64, 50257, 64, 1.25), (300, 131072, 64, 1.0),
+                                           (12, 131073, 8, 4.0), (300, 151936, 64, 1.0), (12, 256000, 32, 2.0), (2, 1100003, 64, 1.0)])
+def test_rest_is_as_good_as_its_sums(rows, K, k, T, dtype):
+    """Long vocabularies, with vectors and groups that end inside a tile.  A class d T below the largest has an exponential good
+    to 3 d E + 2 E, twice (against its group, and its group against all); what counts of it is its weight.  A thread adds
+    vectors in turn, 4 classes or more each, as trees.  The logarithm is rounded once."""
+    from devis_amd import ops
+    E = 2.0 ** -24
+    g = torch.Generator(device="cuda").manual_seed(K)
+    z = (torch.randn((rows, K), generator=g, device="cuda") * 2).to(dtype)
+    z.scatter_add_(1, torch.randint(0, K, (rows, 16), generator=g, device="cuda"), (torch.rand((rows, 16), generator=g, device="cuda") * 12).to(dtype))
+    out = ops.top_logits(z, k, temperature=T)
+    order = torch.sort(z, dim=1, descending=True, stable=True)
+    assert torch.equal(out["indices"].long(), order[1][:, :k]) and torch.equal(out["values"], order[0][:, :k])
+    left = order[0][:, k:].double() / T
+    want = torch.logsumexp(left, 1)
+    weight = (left - want[:, None]).exp()
+    far = (weight * (left[:, :1] - left)).sum(1) + (order[0][:, k - 1].double() / T - left[:, 0])
+    adds = 16 + K / ((64 if K <= 1024 else 256) * 4)
+    tol = (6 * far + adds + 16) * E + want.abs() * E
+    assert ((out["rest"].double() - want).abs() <= tol).all(), ((out["rest"].double() - want).abs() / tol).max()
