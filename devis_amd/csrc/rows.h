@@ -205,6 +205,8 @@ template <int BS> __device__ __forceinline__ double block_sum(double v, double* 
 
 // ---- few classes: a thread takes a whole row into registers.  KT = 2, 4, 8 or 16 bounds K; FULL: K = KT adjacent
 // classes, one load of the whole row.
+// (Distillation of 500000 rows, forward + backward, against a lane a row that streams its classes, below: 4 classes 17 and
+// 38 us, 8 24 and 48, 16 31 and 70; top logits 16 classes 12 and 12.)
 constexpr int FEW_CLASSES = 16;
 
 template <typename T, int KT, bool FULL>
@@ -275,12 +277,21 @@ inline dim3 few_grid(int64_t N, int64_t V, int most) {
 
 // ---- a few dozen classes and many rows: one thread a row, the classes streamed in chunks of 8.  A wave a row would leave
 // most of its lanes without work at the end of each row.  Classes first, the lanes' rows are adjacent and every load is
-// whole lines; classes last, each lane walks its own row 16 bytes at a time.  2 x 21 x 64^3 bf16, classes last, loss and
-// gradient: 2.86 ms a wave a row, 0.12 ms a lane a row.
+// whole lines; classes last, each lane walks its own row 16 bytes at a time, and a wave's load is 64 lines.
+// A lane's time is that of its row until the rows fill the card, a wave's grows with the rows: which is less depends on the
+// classes, and on the slots, every pair of which the lane looks at.  Microseconds a lane a row and a wave a row, bf16 classes
+// last, distillation forward + backward / top logits:
+//   64 classes, 4 slots    8192 rows  36, 34 / 11, 16    32768 rows  33, 98         500000 rows  231, 1379 / 94, 722
+//   64 classes, 16 slots   8192 rows 116, 36             32768 rows 118, 105        500000 rows  963, 1511 / 105, 898
+//   256 classes, 4 slots   8192 rows  66, 34 / 34, 16    32768 rows  67, 103        200000 rows  285,  563 / 78, 301
+//   256 classes, 16 slots 32768 rows 165, 112            200000 rows 524, 616 / 197, 334
 constexpr int LANE_CLASSES = 256;             // classes at most: the slots' bits of 256 rows fill 9 KB of LDS
-constexpr int LANE_SLOTS = 16;                // slots at most: every pair of them is looked at
-constexpr int64_t LANE_ROWS = 8192;           // rows at least: fewer are too few lanes
-inline bool lane_rows(int64_t rows, int64_t K, int64_t k) { return K <= LANE_CLASSES && k <= LANE_SLOTS && rows >= LANE_ROWS; }
+constexpr int LANE_SLOTS = 16;                // slots at most: the list of the largest stays in registers
+constexpr int64_t LANE_ROWS = 8192;           // rows at least (17 classes, 4 slots, 2048 rows: 24 us a lane a row, 18 a wave a row)
+inline bool lane_rows(int64_t rows, int64_t K, int64_t k) {
+  const int64_t least = 96 * K * (k > 4 ? 4 : 1);
+  return K <= LANE_CLASSES && k <= LANE_SLOTS && rows >= (least > LANE_ROWS ? least : LANE_ROWS);
+}
 
 // running maximum and sum of exponentials against it (fp64: one lane adds up the whole row)
 struct LaneSum {

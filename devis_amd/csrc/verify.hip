@@ -379,7 +379,9 @@ extern "C" int devis_verify_drafts(const devis_verify_params* v, const void* tar
 #undef LAUNCH_FEW
     return launch_status();
   }
-  if (lane_rows(v->B, v->K, 1)) {
+  // the row is walked two or three times, as if for many slots (3 drafts of 64 classes, 8192 sequences: 15.7 us a lane a sequence,
+  // 11.5 a block; 256 classes, 32768: 53 and 36; 1 draft, 500000 of 64: 95 and 334, 200000 of 256: 84 and 139)
+  if (lane_rows(v->B, v->K, LANE_SLOTS)) {
     const dim3 grid = few_grid(1, v->B, 8192);
     const bool unit = v->pK == 1 && (!draft || v->qK == 1);
 #define LAUNCH_LANE(UNIT, DRAFTER) hipLaunchKernelGGL((k_verify_lane<T, UNIT, DRAFTER>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)target, (const T*)draft, a)

@@ -66,3 +66,61 @@ def test_rest_is_as_good_as_its_sums(rows, K, k, T, dtype):
     adds = 16 + K / ((64 if K <= 1024 else 256) * 4)
     tol = (6 * far + adds + 16) * E + want.abs() * E
     assert ((out["rest"].double() - want).abs() <= tol).all(), ((out["rest"].double() - want).abs() / tol).max()
+
+
+@pytest.mark.parametrize("first", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows, K, k", [(8192, 17, 4), (8192, 40, 4), (24576, 256, 4), (24574, 256, 4), (38400, 100, 16), (38398, 100, 16), (98304, 256, 16)])
+def test_both_sides_of_the_rule_for_dozens_of_classes(rows, K, k, dtype, first):
+    """A lane a row from here on, a wave a row below: the same lists, losses and gradients, as the formulas in 64 bits give them."""
+    from devis_amd import criterions, ops
+    from tests.test_gpu_classdist_near import exact
+    E, T = 2.0 ** -24, 2.0
+    g = torch.Generator(device="cuda").manual_seed(K + k)
+    t = (torch.randn((rows, K), generator=g, device="cuda") * 2).to(dtype)
+    z = (t.float() + torch.randn((rows, K), generator=g, device="cuda")).to(dtype)
+    t[5:9] = 0.5                                   # ties: the lowest classes
+    z[7:11, K // 2:] = torch.finfo(dtype).min
+    put = (lambda x: x.view(2, rows // 2, -1).movedim(-1, 1).contiguous()) if first else lambda x: x
+    back = (lambda x: x.movedim(1, -1).reshape(rows, -1)) if first else lambda x: x
+    top = ops.top_logits(put(t), k, channels_last=not first, temperature=T)
+    order = torch.sort(t, dim=1, descending=True, stable=True)
+    v, i, rest = back(top["values"]), back(top["indices"]).long(), top["rest"].reshape(rows)
+    assert torch.equal(i, order[1][:, :k]) and torch.equal(v, order[0][:, :k])
+    want = torch.logsumexp(order[0][:, k:].double() / T, 1)
+    assert ((rest.double() - want).abs() <= (3 * 10 + K / 64 + 16) * E + want.abs() * E).all()
+    student = put(z).requires_grad_(True)
+    loss = criterions.distill_top_loss(student, top["values"], top["indices"], top["rest"], channels_last=not first, temperature=T, reduction="none")
+    (dz,) = torch.autograd.grad(loss, student, torch.ones_like(loss))
+    want, tol = (x.to("cuda") for x in exact(z, v, i, rest, T))
+    assert ((loss.reshape(rows).double() - want).abs() <= tol).all()
+    zd = z.double().requires_grad_(True)
+    log_p = torch.log_softmax(torch.cat([v.double() / T, rest.double()[:, None]], 1), 1)
+    log_q = torch.log_softmax(zd / T, 1)
+    out = torch.logsumexp(log_q.scatter(1, i, -math.inf), 1, keepdim=True)
+    kl = (log_p.exp() * (log_p - torch.cat([log_q.gather(1, i), out], 1))).sum() * T * T
+    (grad,) = torch.autograd.grad(kl, zd)
+    # shares q, p and p_rest of a class are good to their exponents' roundings and their sums', and the type rounds once
+    q = log_q.detach().exp()
+    scale = q.scatter_add(1, i, log_p[:, :k].exp()) + (q / out.detach().exp()).scatter(1, i, 0.0) * log_p[:, k:].exp()
+    half = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8
+    bound = T * scale * (2 * (3 * 20 + K / 64 + 12) + 16) * E + half * grad.abs() + 1e-37
+    assert ((back(dz).double() - grad).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K, times", [(40, 376), (40, 374), (256, 2400)])
+def test_verification_of_many_sequences_of_dozens_of_classes(K, times, dtype):
+    """A lane a sequence from here on, a block each below: every copy as the first ones, and those as the oracle says."""
+    from devis_amd import ops
+    from tests.test_gpu_classdist import check_verify, drafts, many
+    tok, p, q, u, r = drafts(41, 3, K, dtype, K, True, torch.int32)
+    p[5] = 0.0
+    p[8], q[8] = q[8, :1].expand(p.shape[1:]), p[8, :3]
+    u[9:20] *= 0.01
+    lengths = torch.arange(41) % 4
+    for x, n in ((q, None), (q, lengths), (None, lengths)):
+        one = check_verify(tok, p, x, u, r, n)
+        out = ops.verify_drafts(many(tok, times).cuda(), many(p.cuda(), times), None if x is None else many(x.cuda(), times),
+                                many(u, times).cuda(), many(r, times).cuda(), None if n is None else many(n, times).cuda())
+        assert torch.equal(out["tokens"], many(one["tokens"], times)) and torch.equal(out["accepted"], many(one["accepted"], times))

@@ -65,7 +65,7 @@ def near_pair(rows, K, k, T, noise, dtype, seed):
 # rows of few classes; a lane a row; a wave a row; long rows
 SHAPES = [(1, 4, 2), (1, 9, 3), (1, 16, 16), (300, 2, 1), (64, 9, 3), (20000, 4, 2), (20000, 7, 3), (20000, 9, 3), (20000, 12, 12),
           (9000, 21, 4), (9000, 40, 40), (9000, 100, 12), (1, 100, 5), (300, 300, 20), (300, 1000, 100), (50, 5003, 20), (8, 33001, 16),
-          (300, 9001, 64), (2, 151936, 64)]
+          (300, 9001, 64), (2, 151936, 64), (9700, 100, 4), (25000, 256, 4), (38500, 100, 16), (98400, 256, 9)]
 
 
 @pytest.mark.parametrize("noise", [0.1, 0.01, 0.001, 0.0])
