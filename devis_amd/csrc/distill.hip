@@ -18,9 +18,14 @@
 namespace devis {
 
 constexpr int DIS_MAX_K = DEVIS_TOP_MAX_K;
-// classes whose slot bits are in LDS at a time (16 KB; of a short row all of them, so that LDS does not limit its waves)
-template <int BS> constexpr int dis_seg() { return BS == 64 ? 1024 : 131072; }
-constexpr int DIS_SHORT = 1024;               // classes up to which a wave takes a row, and the block several
+// classes whose slot bits are in LDS at a time (16 KB; 512 bytes for a wave's row, all it has)
+template <int BS> constexpr int dis_seg() { return BS == 64 ? 4096 : 131072; }
+// Rows that a wave takes, many to a block; longer ones take a block each.  Many rows are better off with waves up to 8 KB.
+// Forward + backward, us, a wave and a block a row, 20 slots (16 of the lesser counts):
+//   20000 rows of 1000 bf16   85, 131     1100  95, 135     2000  109, 136     3000  121, 145     4000  158, 181    fp32 4000  245, 230
+//    6000 rows of 1100        36,  49     2000  42,  52     4000   54,  60     2000 rows of 600  20, 21    1100  22, 22    4000  29, 27
+constexpr int DIS_SHORT = 1024;               // classes of any number of rows
+constexpr int64_t DIS_SHORT_BYTES = 8192, DIS_SHORT_ROWS = 4096;
 // A gradient as large as the 256 MB Infinity Cache cannot stay there for its reader: written past the caches it leaves the
 // logits in them, which the backward reads from the last row on.  Loss and gradient of 4096 x 131072 bf16 rows: 658 us with
 // ordinary stores, 613 past the caches; 2048 x 65536 (256 MB) 198 and 175; below, the gradient is better kept.
@@ -851,9 +856,12 @@ static bool few_classes(const devis_distill_params* a) {
 }
 
 // one block a row, or for short rows as many blocks as run at once
-static bool long_rows(const devis_distill_params* a) { return a->K > DIS_SHORT; }
-// fewer rows than CUs: a block four times as large takes each
-static bool few_rows(const devis_distill_params* a) { return a->K >= 8192 && a->N * a->V < 256; }
+static bool long_rows(const devis_distill_params* a) {
+  return a->K > DIS_SHORT && !(a->N * a->V >= DIS_SHORT_ROWS && a->K * (a->dtype == DEVIS_F32 ? 4 : 2) <= DIS_SHORT_BYTES);
+}
+// fewer rows than CUs: a block four times as large takes each (forward + backward, us, 1024 and 256 threads: 16 fp32 rows of
+// 8192 17, 17, of 16384 18, 19, of 32768 19, 22; 200 rows of 32768 25, 29, of 131072 bf16 41, 47; 300 rows of 32768 36, 34)
+static bool few_rows(const devis_distill_params* a) { return a->K >= 16384 && a->N * a->V < 256; }
 static dim3 distill_grid(const devis_distill_params* a) {
   const int64_t NV = a->N * a->V;
   return long_rows(a) ? row_grid(NV) : dim3((unsigned)(NV < DIS_MAX_WAVES ? NV : DIS_MAX_WAVES));

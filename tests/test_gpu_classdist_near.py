@@ -27,7 +27,7 @@ E = 2.0 ** -24
 
 def additions(K):
     """Additions that one thread makes in turn: vectors of 4 classes dealt to 64, 256 or 1024 threads (at least), summed as trees."""
-    return 8 + K / ((64 if K <= 1024 else 256) * 4)
+    return 8 + K / ((64 if K <= 4096 else 256) * 4)
 
 
 def exact(z, v, i, rest, T):
