@@ -29,6 +29,12 @@ __device__ __forceinline__ float key_value(uint64_t key) {
   return __builtin_bit_cast(float, b);
 }
 
+// Fewer rows than CUs: 1024 threads each, where the reading is longer than bringing four times as many threads together (us, 256
+// and 1024 threads: one bf16 row of 32768 8.5, 10.8, of 65536 11.1, 12.5, of 131072 16.6, 15.8, of 262144 26.5, 22.4; 64 rows of
+// 65536 15.6, 15.0, of 131072 21.1, 18.3; 200 rows of 32768 9.6, 12.3, of 65536 16.5, 15.5; 300 rows of 131072 29, 38).  Rows of up
+// to TOP_CAP classes take a wave each (20000 rows of 1000: 49, and 73 with 256 threads).
+constexpr int TOP_WIDE_K = 65536;
+constexpr int64_t TOP_WIDE_ROWS = 256;
 template <int BS> constexpr int top_groups() { return BS == 256 ? 8 : BS == 1024 ? 4 : 0; }     // k_top_wide: groups a thread
 template <int BS> struct TopShared {
   union {
@@ -515,7 +521,7 @@ extern "C" int devis_top_logits(const void* logits, int64_t sN, int64_t sV, int6
   do {                                                                                                            \
     if (K <= TOP_CAP) LAUNCH_TOP_U(I, 64);                                                                        \
     else if (sK != 1) LAUNCH_TOP(I, false, 256);                                                                  \
-    else if (K >= 16384 && NV < 256) LAUNCH_WIDE(I, 1024);                                                        \
+    else if (K >= TOP_WIDE_K && NV < TOP_WIDE_ROWS) LAUNCH_WIDE(I, 1024);                                         \
     else LAUNCH_WIDE(I, 256);                                                                                     \
   } while (0)
   DEVIS_DISPATCH_DTYPE(dtype, { if (index_dtype == DEVIS_LABEL_U8) LAUNCH_TOP_B(uint8_t); else LAUNCH_TOP_B(int32_t); });
