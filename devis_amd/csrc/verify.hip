@@ -102,10 +102,9 @@ __device__ __forceinline__ void each_weight(const Draw<T>& d, int lo, int hi, in
   }
 }
 
-// One block a sequence: 64 threads up to 1024 classes, 256 up to 8192, else 1024 (a row's read is then as short as one CU
-// can make it: 200 sequences of 7 drafts over 131072 bf16 classes in 20 us, 105 MB; one sequence over 32768 fp32 classes in
-// 8 us; with 256 threads, scalar loads and a serial search they took 320 and 51).  Each wave sums the weights of one stretch of the row; the stretch in which the goal lies is read
-// once more, a vector a thread, and the class found by a prefix sum over the block.
+// One block a sequence, of 64, 256 or 1024 threads (verify_threads).  Each wave sums the weights of one stretch of the row; the
+// stretch in which the goal lies is read once more, a vector a thread, and the class found by a prefix sum over the block.
+// 200 sequences of 7 drafts over 131072 bf16 classes: 22.5 us, 105 MB; one sequence of 4 over 32768 fp32: 8.1 us.
 template <typename T, bool UNIT, bool DRAFTER, int BS>
 __global__ void __launch_bounds__(BS)
 k_verify(const T* __restrict__ p, const T* __restrict__ q, VerifyArgs a) {
@@ -352,6 +351,14 @@ k_verify_lane(const T* __restrict__ p, const T* __restrict__ q, VerifyArgs a) {
   }
 }
 
+// Few sequences want a row's read as short as one CU can make it, many the fewest threads that wait for each other.  us, bf16, 5
+// drafts, 64 / 256 threads: 4000 sequences of 1000 classes 10, 21; 2000 of 2000 11, 12; 200 of 2000 9, 6; 2000 of 4000 18, 15.
+// 256 / 1024 threads: 200 sequences of 4000 6, 8; 200 of 16000 9, 10; 200 of 32000 12, 11; 200 of 64000 22, 15; 64 of 64000 18, 12;
+// 500 of 16000 12, 18; 500 of 32000 18, 23; 500 of 64000 31, 31; 1000 of 64000 52, 58; 2000 of 16000 30, 66; 500 of 131072 61, 52.
+static int verify_threads(int64_t B, int64_t K) {
+  return K <= 1024 ? 64 : K <= 16384 || (K <= 65536 && B >= 256) ? 256 : 1024;
+}
+
 }  // namespace devis
 
 using namespace devis;
@@ -392,11 +399,12 @@ extern "C" int devis_verify_drafts(const devis_verify_params* v, const void* tar
 #undef LAUNCH_LANE
     return launch_status();
   }
+  const int threads = verify_threads(v->B, v->K);
   const unsigned blocks = (unsigned)(v->B < (1 << 20) ? v->B : (1 << 20));
   const bool unit = v->pK == 1 && (!draft || v->qK == 1);
 #define LAUNCH_VERIFY(UNIT, DRAFTER, BS) hipLaunchKernelGGL((k_verify<T, UNIT, DRAFTER, BS>), dim3(blocks), dim3(BS), 0, (hipStream_t)stream, (const T*)target, (const T*)draft, a)
 #define LAUNCH_VERIFY_U(DRAFTER, BS) do { if (unit) LAUNCH_VERIFY(true, DRAFTER, BS); else LAUNCH_VERIFY(false, DRAFTER, BS); } while (0)
-#define LAUNCH_VERIFY_B(DRAFTER) do { if (v->K <= 1024) LAUNCH_VERIFY_U(DRAFTER, 64); else if (v->K <= 8192) LAUNCH_VERIFY_U(DRAFTER, 256); else LAUNCH_VERIFY_U(DRAFTER, 1024); } while (0)
+#define LAUNCH_VERIFY_B(DRAFTER) do { if (threads == 64) LAUNCH_VERIFY_U(DRAFTER, 64); else if (threads == 256) LAUNCH_VERIFY_U(DRAFTER, 256); else LAUNCH_VERIFY_U(DRAFTER, 1024); } while (0)
   DEVIS_DISPATCH_DTYPE(v->dtype, { if (draft) LAUNCH_VERIFY_B(true); else LAUNCH_VERIFY_B(false); });
 #undef LAUNCH_VERIFY_B
 #undef LAUNCH_VERIFY_U

@@ -125,3 +125,12 @@ def test_verification_of_many_sequences_of_dozens_of_classes(K, times, dtype):
         out = ops.verify_drafts(many(tok, times).cuda(), many(p.cuda(), times), None if x is None else many(x.cuda(), times),
                                 many(u, times).cuda(), many(r, times).cuda(), None if n is None else many(n, times).cuda())
         assert torch.equal(out["tokens"], many(one["tokens"], times)) and torch.equal(out["accepted"], many(one["accepted"], times))
+
+
+@pytest.mark.parametrize("B, K", [(255, 16385), (256, 16385), (2, 16384), (2, 16385), (256, 65537)])
+def test_verification_on_both_sides_of_the_rule_for_long_rows(B, K):
+    from tests.test_gpu_classdist import check_verify, drafts
+    for dtype in (torch.float32, torch.bfloat16):
+        tok, p, q, u, r = drafts(B, 2, K, dtype, K)
+        check_verify(tok, p, q, u, r)
+        check_verify(tok, p, None, u, r, torch.arange(B) % 3)
