@@ -220,8 +220,9 @@ def _distill_backward(ctx, g):
     *ts, scratch = ctx.saved_tensors
     params, channels_last, rows, dev, places = ctx.call
     if _places(ts) != places:                     # moved by saved-tensor hooks
-        if not ops.distill_keeps_stats(params):   # nor may the backward want any: adjacent rows do not
-            ts = [None if t is None else t.contiguous() for t in ts]
+        if not ops.distill_keeps_stats(params):   # nor may the backward want any: rows of adjacent classes, one behind the other, do not
+            rows_of = (lambda t: t.contiguous()) if channels_last else (lambda t: t.movedim(1, -1).contiguous().movedim(-1, 1))
+            ts = [rows_of(t) for t in ts[:3]] + [None if t is None else t.contiguous() for t in ts[3:]]
         params, dev, _, ts = ops.distill_params(*ts, channels_last, params.temperature, params.mean)
     if g.dtype != torch.float32 or not g.is_contiguous():
         g = g.contiguous().float()

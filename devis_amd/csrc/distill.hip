@@ -850,9 +850,12 @@ k_distill_lane_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, 
   }
 }
 
+static RowShape student_rows(const devis_distill_params* a) { return {a->sN, a->sV, a->sK, a->N, a->V, (int)a->K}; }
+static RowShape slot_rows(const devis_distill_params* a) { return {a->oN, a->oV, a->oK, a->N, a->V, (int)a->k}; }
 // few classes, and rows that a 32-bit offset reaches from the block's first
 static bool few_classes(const devis_distill_params* a) {
-  return a->K <= FEW_CLASSES && (a->V == 1 ? a->sN : a->sV) <= FEW_STRIDE && (a->V == 1 ? a->oN : a->oV) <= FEW_STRIDE;
+  return a->K <= FEW_CLASSES && (a->V == 1 ? a->sN : a->sV) <= FEW_STRIDE && (a->V == 1 ? a->oN : a->oV) <= FEW_STRIDE &&
+         side_by_side(student_rows(a), slot_rows(a));
 }
 
 // one block a row, or for short rows as many blocks as run at once
@@ -914,8 +917,8 @@ int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* 
                       void* ws, size_t ws_bytes, void* stream) {
   if (!distill_args_ok(a, logits) || (!per_row && !loss) || (loss && (!ws || !scal))) return DEVIS_ERR_BAD_ARG;
   if (loss && ws_bytes < devis_distill_workspace_bytes(a)) return DEVIS_ERR_WORKSPACE;
-  RowShape s = {a->sN, a->sV, a->sK, a->N, a->V, (int)a->K};
-  Teacher t = {a->values, a->indices, a->rest, a->row_mask, {a->oN, a->oV, a->oK, a->N, a->V, (int)a->k}, a->values_dtype, a->index_dtype};
+  RowShape s = student_rows(a);
+  Teacher t = {a->values, a->indices, a->rest, a->row_mask, slot_rows(a), a->values_dtype, a->index_dtype};
   const double inv_t = 1.0 / (double)a->temperature, t2 = (double)a->temperature * (double)a->temperature;
   const float scale = (float)(1.4426950408889634 * inv_t);
   const bool unit = a->sK == 1;
@@ -955,8 +958,8 @@ int devis_distill_bwd(const devis_distill_params* a, const void* logits, const v
                       int grad_rows, void* dlogits, int64_t dN, int64_t dV, int64_t dK, void* stream) {
   if (!distill_args_ok(a, logits) || (!stats && !few_classes(a)) || !grad || !dlogits || (!grad_rows && !scal)) return DEVIS_ERR_BAD_ARG;
   if (!rows_ok(dN, dV, dK, a->N, a->V, a->K)) return DEVIS_ERR_BAD_ARG;
-  RowShape s = {a->sN, a->sV, a->sK, a->N, a->V, (int)a->K}, d = {dN, dV, dK, a->N, a->V, (int)a->K};
-  Teacher t = {a->values, a->indices, a->rest, a->row_mask, {a->oN, a->oV, a->oK, a->N, a->V, (int)a->k}, a->values_dtype, a->index_dtype};
+  RowShape s = student_rows(a), d = {dN, dV, dK, a->N, a->V, (int)a->K};
+  Teacher t = {a->values, a->indices, a->rest, a->row_mask, slot_rows(a), a->values_dtype, a->index_dtype};
   const double inv_t = 1.0 / (double)a->temperature;
   const float scale = (float)(1.4426950408889634 * inv_t);
   const bool unit = a->sK == 1 && dK == 1;

@@ -265,6 +265,12 @@ inline void merge_rows(RowShape& s) {
   s.N = 1;
   s.sN = 0;
 }
+// The kernels of few classes take 256 rows v at a time, for each n: rows that do not come as one long v, few of them side by side
+// (small images, channels first), would leave most lanes idle and go the way of more classes instead.  us, top logits +
+// distillation forward + backward, 4 fp32 classes channels first, 256 v at a time and any row a lane: 10^6 x 2 2633, 144;
+// 10^5 x 16 299, 113; 30000 x 64 106, 127; 8000 x 200 59, 116.
+constexpr int64_t FEW_V = 32;
+inline bool side_by_side(const RowShape& a, const RowShape& b) { return a.V >= FEW_V || (one_stride(a) && one_stride(b)); }
 inline dim3 few_grid(int64_t N, int64_t V, int most) {
   int64_t bx = cdiv(V, 256), by = N;
   if (bx > most) bx = most;

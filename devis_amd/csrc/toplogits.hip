@@ -490,7 +490,7 @@ extern "C" int devis_top_logits(const void* logits, int64_t sN, int64_t sV, int6
   const double inv_t = 1.0 / (double)temperature;
   const float scale = (float)(1.4426950408889634 * inv_t);
   const hipStream_t st = (hipStream_t)stream;
-  if (K <= FEW_CLASSES) {
+  if (K <= FEW_CLASSES && side_by_side(s, o)) {
     if (one_stride(s) && one_stride(o)) { merge_rows(s); merge_rows(o); }
     const dim3 grid = few_grid(s.N, s.V, 8192);
 #define LAUNCH_FEW(KT, FULL) hipLaunchKernelGGL((k_top_few<T, I, KT, FULL>), grid, dim3(256), 0, st, (const T*)logits, s, (int)k, scale, inv_t, (T*)values, (I*)indices, o, rest)

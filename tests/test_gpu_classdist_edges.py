@@ -134,3 +134,51 @@ def test_verification_on_both_sides_of_the_rule_for_long_rows(B, K):
         tok, p, q, u, r = drafts(B, 2, K, dtype, K)
         check_verify(tok, p, q, u, r)
         check_verify(tok, p, None, u, r, torch.arange(B) % 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N, K, V, k", [(5, 4, 2, 2), (5000, 4, 2, 2), (4097, 7, 3, 3), (300, 16, 31, 16), (300, 16, 32, 16), (9000, 2, 1, 1), (33, 3, 5, 1)])
+def test_many_small_images_channels_first(N, K, V, k, dtype):
+    """Classes first, few rows side by side: as the same rows one behind the other give it, near enough."""
+    from devis_amd import criterions, ops
+    from tests.test_gpu_classdist_near import exact
+    g = torch.Generator(device="cuda").manual_seed(N)
+    t = (torch.randn((N, K, V), generator=g, device="cuda") * 3).to(dtype)
+    z = (t.float() + torch.randn((N, K, V), generator=g, device="cuda")).to(dtype).requires_grad_(True)
+    mask = torch.rand((N, V), generator=g, device="cuda") < 0.8
+    top = ops.top_logits(t, k, channels_last=False, temperature=2.0)
+    last = ops.top_logits(t.movedim(1, -1).contiguous(), k, temperature=2.0)
+    assert torch.equal(top["values"].movedim(1, -1), last["values"]) and torch.equal(top["indices"].movedim(1, -1), last["indices"])
+    assert torch.allclose(top["rest"], last["rest"], rtol=2.0 ** -22, atol=2.0 ** -20)
+    rows = lambda x: x.movedim(1, -1).reshape(N * V, -1)
+    want, tol = (x.cuda() for x in exact(rows(z.detach()), rows(top["values"]), rows(top["indices"]), top["rest"].reshape(-1), 2.0))
+    want, tol = torch.where(mask.view(-1), want, 0.0), torch.where(mask.view(-1), tol, 0.0)
+    call = lambda x, **kw: criterions.distill_top_loss(x, top["values"], top["indices"], top["rest"], channels_last=False, temperature=2.0, row_mask=mask, **kw)
+    assert ((call(z, reduction="none").reshape(-1).double() - want).abs() <= tol).all()
+    loss = call(z, reduction="sum")
+    assert abs(loss.item() - want.sum().item()) <= tol.sum().item() + 2.0 ** -23 * want.sum().item()
+    (dz,) = torch.autograd.grad(loss, z)
+    flat = rows(z.detach()).requires_grad_(True)
+    one = criterions.distill_top_loss(flat, rows(top["values"]), rows(top["indices"]), top["rest"].reshape(-1), temperature=2.0, row_mask=mask.reshape(-1), reduction="sum")
+    (want,) = torch.autograd.grad(one, flat)
+    # each side is within 2 x 12 roundings of its shares (at most 2 in all, times T), and the type's own
+    half = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8
+    assert ((rows(dz).double() - want.double()).abs() <= 2 * (2 * 2 * 2 * (3 * 12 + 24) * 2.0 ** -24 + half * want.double().abs())).all()
+
+
+@pytest.mark.parametrize("N, V", [(6, 2), (6, 40)])
+def test_saved_tensors_that_come_back_in_another_layout(N, V):
+    """Rows of few classes keep nothing for the backward, whichever layout their tensors come back in."""
+    from devis_amd import criterions, ops
+    g = torch.Generator(device="cuda").manual_seed(V)
+    t = torch.randn((N, V, 4), generator=g, device="cuda")
+    z = torch.randn((N, V, 4), generator=g, device="cuda")
+    top = ops.top_logits(t, 2)
+    got = []
+    for unpack in (lambda x: x, lambda x: x.clone(memory_format=torch.contiguous_format) if x.dim() == 3 else x.clone()):
+        x = z.clone().requires_grad_(True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda s: s, unpack):
+            loss = criterions.distill_top_loss(x.movedim(-1, 1), top["values"].movedim(-1, 1), top["indices"].movedim(-1, 1), top["rest"], channels_last=False)
+        loss.backward()
+        got.append(x.grad)
+    assert torch.equal(*got)
