@@ -1131,7 +1131,7 @@ def verify_drafts(tokens: Tensor, target_probs: Tensor, draft_probs: Optional[Te
     its class; one class more is drawn from max(target - draft, 0) at the first refused place, or from the row behind the
     last draft if all were accepted and there is one.
     -> dict(tokens (B, target_probs.shape[1]): accepted, drawn, then -1; accepted (B,)), both of the tokens' type.
-    A label map is B = voxels, T = 1.  Not differentiable."""
+    For programs that draft and decode: no model of this package does.  Not differentiable."""
     if tokens.dim() != 2 or target_probs.dim() != 3:
         raise _lib.DevisError("verify_drafts: tokens must be (B, T) and target_probs (B, T or T + 1, K)")
     b, t = tokens.shape

@@ -4,7 +4,8 @@ Tolerances.  Let e = 2^-24 (fp32) and D = the largest |z - max z| / T that is fi
 exp2((z - m) * c): the difference, c and the product are rounded (3e of an exponent of D nats), the exponential itself is
 good to 2e: 3 D e + 2e relative.  A thread adds its classes in turn, at most K/64 of them, in groups: (K/64 + 8) e.  So
 every sum of exponentials is within S = (3 D + K/64 + 12) e relative, which is also the absolute error of its logarithm.
-Teacher's shares are good to 4e relative (fp32 exponential of an exact difference, one rounding).
+Teacher's shares are good to 4e relative where they count for something (fp64 and rounded once in most paths, fp32 exponentials
+in the gradients of few and of dozens of classes).  Bounds relative to the loss: test_gpu_classdist_near.py.
 """
 import math
 
