@@ -193,7 +193,8 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
       continue;
     }
     if (tid < 64) teacher_row<LONG>(t, r, K, inv_t, tid, sh);
-    // running maximum and sum of the classes in no slot
+    // running maximum and sum of the classes in no slot: fp32, in which a thread adds trees of 16 or 32 classes in turn; what that
+    // and the exponentials leave over is in every logarithm of the row and drops out of its loss (kl_part)
     float m = neg_inf(), acc = 0.f;
     const auto absorb = [&](auto& x) {
       constexpr int N = sizeof(x) / sizeof(float);
@@ -479,7 +480,7 @@ __device__ __forceinline__ float few_exp(float x, float ref, float scale, double
 __device__ __forceinline__ double few_exp(double x, double ref, float, double scale) { return exp2_series((x - ref) * scale); }
 __device__ __forceinline__ float few_log(float x) { return log2_f(x); }
 __device__ __forceinline__ double few_log(double x) { return log2_newton(x); }
-__device__ __forceinline__ float few_rcp(float x) { return rcp_f(x); }
+__device__ __forceinline__ float few_rcp(float x) { return rcp_f(x); }       // within 2^-23: a share's own exponential is no better
 __device__ __forceinline__ double few_rcp(double x) { return 1. / x; }
 
 // Row (n, v0 + lane) with n and v0 the block's.  Straight-line: a row that is not counted is worked out all the same and
@@ -830,6 +831,7 @@ k_distill_lane_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, 
       }
     }
     if (live && !(st.w != st.w && st.inv_s != st.inv_s)) {           // a NaN row is NaN as it stands
+      // (shares in fp32 with the hardware's reciprocal: the class's own exponential, from which they are taken off, is no better)
       const int64_t at = row_offset(t.o, r);
       float hi = neg_inf(), shift = 0.f, sum = 0.f;
       each_slot(t, at, K, [&](int, float v, int) { hi = fmaxf(hi, v); });

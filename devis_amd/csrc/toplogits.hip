@@ -222,7 +222,8 @@ k_top_rows(const T* __restrict__ z, RowShape s, int k, float scale, double inv_t
 // maximum and sum of exponentials against it kept in LDS (16 KB a block: eight blocks of 256 threads stay on a CU).  The
 // k-th largest of the threads' maxima, found bit by bit by one wave, is a floor under the first k; only the groups that
 // reach it (about k of them) are read again, vector by vector over the whole block, and every other group's sum goes
-// into the rest as it is.  Rows on which this stalls - most groups reach the floor, because classes are equal or masked -
+// into the rest as it is.  (Groups and threads add in fp32, the block in fp64; rest is one fp32 number, which the sum's few 2^-24
+// move by no more than its own rounding does.)  Rows on which this stalls - most groups reach the floor, because classes are equal or masked -
 // go the general way.
 constexpr int TOP_GROUP = 8;                  // vectors of a group
 constexpr int TOP_ITEMS = 440;                // groups read again (with the rest of the LDS: 1/8 of a CU)
