@@ -474,7 +474,11 @@ template <int KT, int KS, typename S> struct FewRow {
   S off;                       // with a loss: log2(S_student / S_teacher), both against their own maxima
   S off_rest;                  // with a loss: log2(p_rest / q_rest)
   unsigned twice;              // classes in two slots
+  bool alive[KS], rest_alive;  // a slot, the rest has a share, be it too small for S
 };
+
+// exponents (base 2) from which on a share is none, here as in exp2_series
+constexpr float NO_SHARE = -1050.f;
 
 __device__ __forceinline__ float few_exp(float x, float ref, float scale, double) { return exp2_f((x - ref) * scale); }
 __device__ __forceinline__ double few_exp(double x, double ref, float, double scale) { return exp2_series((x - ref) * scale); }
@@ -545,12 +549,14 @@ __device__ __forceinline__ void few_row(const T* __restrict__ z, const RowShape&
     a_rest = fma(-(double)hi, inv_t, (double)rest) * 1.4426950408889634;     // one rounding before the large parts cancel
     shift = (S)fmax(a_rest, 0.);
   }
+  w.rest_alive = REST && !(a_rest - (double)shift < NO_SHARE);
   w.p_rest = REST ? few_exp((S)a_rest, shift, 1.f, 1.) : (S)0;
   S sum_t = w.p_rest;
 #pragma unroll
   for (int j = 0; j < KS; ++j) {
     w.a[j] -= hi;
     w.p[j] = REST ? few_exp((S)w.a[j] * (S)scale_d, shift, 1.f, 1.) : few_exp((S)w.a[j], (S)0, scale, scale_d);
+    if constexpr (WANT == FEW_MEAN_LOSS) w.alive[j] = !(w.a[j] * scale - shift < NO_SHARE);      // (an empty slot's is -inf)
     w.p[j] = w.c[j] == FEW_CLASSES ? (S)0 : +w.p[j];
     sum_t += w.p[j];
   }
@@ -628,7 +634,7 @@ k_distill_few_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
           float e;
           const float x = pick_class(w.x, w.c[j], w.e, e);
           const bool none = x == neg_inf();
-          barred = barred || (none && w.p[j] != 0.f);
+          barred |= none & w.alive[j];
           sum += kl_part(w.p[j], e * inv, none ? 0.f : fmaf(w.off, unit, w.a[j] - (x - w.m)), temperature, (float)inv_t);
         }
         if (w.twice) {                         // the q of a class in two slots has been added twice
@@ -645,7 +651,7 @@ k_distill_few_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
         sum = barred ? sum + __builtin_inff() : in_range(sum);
         const float q = w.sum_rest * w.to_m * inv;
         const float part = kl_part(w.p_rest, q, w.off_rest * unit, temperature, (float)inv_t);
-        sum += w.p_rest == 0.f ? temperature * q : w.sum_rest == 0.f ? __builtin_inff() : part;
+        sum += w.sum_rest == 0.f && w.rest_alive ? __builtin_inff() : w.p_rest == 0.f ? temperature * q : part;
       }
       float loss = (float)(sum * (S)temperature);              // the terms are T (log p - log q)
       loss = w.state == 1 ? loss : w.state ? __builtin_nanf("") : 0.f;

@@ -182,3 +182,22 @@ def test_saved_tensors_that_come_back_in_another_layout(N, V):
         loss.backward()
         got.append(x.grad)
     assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("rows, K", [(20, 4), (9000, 12), (9000, 40), (20, 300), (20, 3000)])
+def test_a_closed_class_that_the_teacher_hardly_gives(rows, K):
+    """A class that is closed to the student makes the loss infinite however little the teacher gives it (e^-120 here, too little for
+    fp32), listed or not: in the mean, the sum and row by row."""
+    from devis_amd import criterions
+    v, i = torch.tensor([0.0, -120.0], device="cuda").expand(rows, 2).contiguous(), torch.tensor([1, 2], dtype=torch.uint8, device="cuda").expand(rows, 2).contiguous()
+    z = torch.zeros((rows, K), device="cuda")
+    z[:, 2] = -math.inf
+    rest = torch.full((rows,), -64.0, device="cuda")
+    for reduction in ("mean", "sum", "none"):
+        for r in (rest, None):
+            assert (criterions.distill_top_loss(z, v, i, r, reduction=reduction) == math.inf).all()
+    z[:] = -math.inf
+    z[:, 1:3] = 0.0
+    for reduction in ("mean", "sum", "none"):
+        assert (criterions.distill_top_loss(z, v, i, rest - 60.0, reduction=reduction) == math.inf).all()
+        assert torch.isfinite(criterions.distill_top_loss(z, v, i, rest * math.inf, reduction=reduction)).all()
