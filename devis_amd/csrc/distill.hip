@@ -435,10 +435,9 @@ __device__ __forceinline__ float pick_class(const float (&x)[KT], int c, const S
   return v;
 }
 
-// p (r - 1 - log r) times T, of a finite d = T log(p / q): by its series where q and p are near (what is left out is 4e-8 of
-// it), otherwise as it stands
-__device__ __forceinline__ float kl_part(float p, float q, float d, float temperature, float inv_t) {
-  const float l = d * inv_t, pd = p * d;
+// p (r - 1 - log r) times T, of a finite l = -log r and pd = p T l: by its series where q and p are near (what is left out is 4e-8
+// of it), otherwise as it stands
+__device__ __forceinline__ float kl_part(float p, float q, float l, float pd, float temperature) {
   float s = -1.f / 362880.f;
   s = fmaf(s, l, 1.f / 40320.f);
   s = fmaf(s, l, -1.f / 5040.f);
@@ -472,7 +471,7 @@ template <int KT, int KS, typename S> struct FewRow {
   S sum_rest, to_m;            // classes in no slot: sum against m_rest, exp((m_rest - m)/T)
   S p_rest;
   S off;                       // with a loss: log2(S_student / S_teacher), both against their own maxima
-  S off_rest;                  // with a loss: log2(p_rest / q_rest)
+  double off_rest;             // with a loss: log2(p_rest / q_rest)
   unsigned twice;              // classes in two slots
   bool alive[KS], rest_alive;  // a slot, the rest has a share, be it too small for S
 };
@@ -592,7 +591,7 @@ __device__ __forceinline__ void few_row(const T* __restrict__ z, const RowShape&
   } else {
     if constexpr (WANT == FEW_ROW_LOSS) w.off = few_log(w.sum) - few_log(sum_t) - shift;
     else w.off = few_log(w.sum * inv_sum_t) - shift;
-    if constexpr (REST) w.off_rest = (S)(a_rest - ((double)m_rest - (double)w.m) * scale_d) + (w.off - few_log(w.sum_rest));
+    if constexpr (REST) w.off_rest = (a_rest - ((double)m_rest - (double)w.m) * scale_d) + (double)(w.off - few_log(w.sum_rest));
   }
 }
 
@@ -635,7 +634,8 @@ k_distill_few_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
           const float x = pick_class(w.x, w.c[j], w.e, e);
           const bool none = x == neg_inf();
           barred |= none & w.alive[j];
-          sum += kl_part(w.p[j], e * inv, none ? 0.f : fmaf(w.off, unit, w.a[j] - (x - w.m)), temperature, (float)inv_t);
+          const float d = none ? 0.f : fmaf(w.off, unit, w.a[j] - (x - w.m));       // T log(p / q)
+          sum += kl_part(w.p[j], e * inv, d * (float)inv_t, w.p[j] * d, temperature);
         }
         if (w.twice) {                         // the q of a class in two slots has been added twice
 #pragma unroll
@@ -650,7 +650,9 @@ k_distill_few_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
         }
         sum = barred ? sum + __builtin_inff() : in_range(sum);
         const float q = w.sum_rest * w.to_m * inv;
-        const float part = kl_part(w.p_rest, q, w.off_rest * unit, temperature, (float)inv_t);
+        // (a small share of a student's lowest values is a number where their distance is past the largest one)
+        const double l = w.off_rest * 0.6931471805599453;
+        const float part = kl_part(w.p_rest, q, (float)l, (float)((double)w.p_rest * (l * (double)temperature)), temperature);
         sum += w.sum_rest == 0.f && w.rest_alive ? __builtin_inff() : w.p_rest == 0.f ? temperature * q : part;
       }
       float loss = (float)(sum * (S)temperature);              // the terms are T (log p - log q)

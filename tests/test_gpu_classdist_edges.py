@@ -201,3 +201,20 @@ def test_a_closed_class_that_the_teacher_hardly_gives(rows, K):
     for reduction in ("mean", "sum", "none"):
         assert (criterions.distill_top_loss(z, v, i, rest - 60.0, reduction=reduction) == math.inf).all()
         assert torch.isfinite(criterions.distill_top_loss(z, v, i, rest * math.inf, reduction=reduction)).all()
+
+
+@pytest.mark.parametrize("T", [1.0, 2.0])
+@pytest.mark.parametrize("rows, K", [(20, 4), (9000, 12), (9000, 40), (20, 300), (20, 3000)])
+def test_a_rest_that_the_student_holds_at_the_lowest_value(rows, K, T):
+    """One part in 1e28 of the teacher lies outside the list, where the student's mask left the type's lowest value: that adds T times
+    the distance times the share, a number, in the mean and the sum as row by row."""
+    from devis_amd import criterions
+    low = torch.finfo(torch.float32).min
+    v, i = torch.tensor([0.0, -120.0], device="cuda").expand(rows, 2).contiguous(), torch.tensor([1, 2], dtype=torch.uint8, device="cuda").expand(rows, 2).contiguous()
+    z = torch.full((rows, K), low, device="cuda")
+    z[:, 1], z[:, 2] = 0.0, -120.0
+    want = T * math.exp(-64.0) * -float(low)       # and terms of order one, far below its last digit
+    for reduction, n in (("mean", 1), ("sum", rows), ("none", 1)):
+        loss = criterions.distill_top_loss(z, v, i, torch.full((rows,), -64.0, device="cuda"), temperature=T, reduction=reduction).double()
+        # the share is an fp32 exponential of 64 nats (192 E + 3 E); a sum of rows in fp64
+        assert ((loss / n - want).abs() <= 200 * 2.0 ** -24 * want).all()
