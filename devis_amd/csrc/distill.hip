@@ -628,24 +628,25 @@ k_distill_few_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
         sum += w.p_rest == (S)0 ? (S)0 : w.p_rest * d;
       } else {
         const float inv = w.sum == 0.f ? 0.f : rcp_f(w.sum);
-#pragma unroll
-        for (int j = 0; j < KS; ++j) {
+        // slot j; the q of a class that an earlier slot names counts there
+        const auto part_of = [&](int j, bool again) {
           float e;
           const float x = pick_class(w.x, w.c[j], w.e, e);
           const bool none = x == neg_inf();
           barred |= none & w.alive[j];
-          const float d = none ? 0.f : fmaf(w.off, unit, w.a[j] - (x - w.m));       // T log(p / q)
-          sum += kl_part(w.p[j], e * inv, d * (float)inv_t, w.p[j] * d, temperature);
-        }
-        if (w.twice) {                         // the q of a class in two slots has been added twice
+          const float d = none ? 0.f : fmaf(w.off, unit, w.a[j] - (x - w.m)), pd = w.p[j] * d;       // d = T log(p / q)
+          return again ? fmaf(-temperature, w.p[j], pd) : kl_part(w.p[j], e * inv, d * (float)inv_t, pd, temperature);
+        };
 #pragma unroll
-          for (int j = 1; j < KS; ++j) {
-            float e;
+        for (int j = 0; j < KS; ++j) sum += part_of(j, false);
+        if (w.twice) {                         // rarely: once more
+          sum = 0;
+#pragma unroll
+          for (int j = 0; j < KS; ++j) {
             bool again = false;
 #pragma unroll
-            for (int i = 0; i < j; ++i) again = again || w.c[i] == w.c[j];
-            pick_class(w.x, w.c[j], w.e, e);
-            sum -= again && w.c[j] != FEW_CLASSES ? temperature * (e * inv) : 0.f;
+            for (int i = 0; i < j; ++i) again |= w.c[i] == w.c[j];
+            sum += part_of(j, again);
           }
         }
         sum = barred ? sum + __builtin_inff() : in_range(sum);

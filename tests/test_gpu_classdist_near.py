@@ -128,3 +128,40 @@ def test_odd_rows_one_by_one(K, dtype):
         one = slice(n, n + 1)
         for rest in (None, r[one].cuda()):
             assert math.isnan(criterions.distill_top_loss(z[one].cuda(), v[one].cuda(), i[one].cuda(), rest).item())
+
+
+@pytest.mark.parametrize("T", [1.0, 0.25])
+@pytest.mark.parametrize("rows, K, k", [(4000, 3, 3), (4000, 5, 2), (4000, 9, 6), (9000, 40, 5), (300, 300, 20), (50, 5003, 20)])
+def test_a_class_in_two_slots_of_a_student_near_its_teacher(rows, K, k, T):
+    """Two slots p1 > p2 of one class whose share is q: their terms are p1 (r - 1 - log r), r = q / p1, and -p2 - p2 log(q / p2).  Where p2
+    is small nothing of it is lost beside q: the error is a few E of each term and second order in what is common."""
+    from devis_amd import criterions
+    z, v, i, rest = near_pair(rows, K, k, T, 0.0, torch.float32, K)
+    i[:, k - 1] = i[:, 0]                          # the last slot, the least share, names the first's class
+    v[:, k - 1] = v[:, 0] - T * torch.linspace(0.0, 18.0, rows)
+    zt, t = z.double() / T, v.double() / T
+    log_p = torch.log_softmax(torch.cat([t, rest.double()[:, None]], 1), 1)
+    log_q = torch.log_softmax(zt, 1)
+    out = torch.logsumexp(log_q.scatter(1, i.long(), -math.inf), 1, keepdim=True)
+    log_q = torch.cat([log_q.gather(1, i.long()), out], 1)
+    p, q = log_p.exp(), log_q.exp()
+    term = torch.where(p > 0, p * (log_p - log_q), torch.zeros_like(p)) + q - p
+    term[:, k - 1] -= q[:, 0]
+    want = T * T * term.sum(1)
+    top = zt.max(1)[0][:, None]
+    near = torch.where(zt > top - 110, top - zt, torch.zeros_like(zt)).max(1)[0]
+    sums = (3 * near + additions(K) + 12) * E      # as in exact()
+    each = torch.cat([(t[:, :1] - t) + (top - zt.gather(1, i.long())) + 4, torch.full_like(out, 4.0) + sums[:, None] / E + (rest.double()[:, None] - t[:, :1]).abs().nan_to_num(0, 0, 0)], 1) * E
+    change = q - p
+    change[:, k - 1] = -p[:, k - 1]
+    tol = T * T * ((change.abs() * each).sum(1) + (2 * sums + 8 * E) ** 2 + 3e-11 + 24 * E * term.abs().sum(1)) + E * want.abs()
+    args = z.cuda(), v.cuda(), i.cuda(), rest.cuda()
+    for reduction in ("none", "rows"):
+        if reduction == "none":
+            have = criterions.distill_top_loss(*args, temperature=T, reduction="none").cpu().double()
+        else:                                      # the form of the mean, row by row
+            some = range(0, rows, max(1, rows // 200))
+            have = want.clone()
+            for n in some:
+                have[n] = criterions.distill_top_loss(*(x[n:n + 1] for x in args), temperature=T, reduction="sum").item()
+        assert ((have - want).abs() <= tol).all(), (reduction, ((have - want).abs() / tol).max())
