@@ -82,6 +82,13 @@ __device__ __forceinline__ float slot_value(const Teacher& t, int64_t i) {
   return t.value_kind == DEVIS_F32 ? ((const float*)t.values)[i] : (float)((const bf16*)t.values)[i];
 }
 
+// rest - hi / T.  Of a masked row both are near the type's lowest value and their difference is what counts: the quotient is
+// rounded correctly (by its remainder; hi times a rounded 1 / T would be off by 1e22), and what it is taken off from is exact.
+__device__ __forceinline__ double rest_gap(float rest, float hi, double inv_t, float temperature) {
+  const double q = (double)hi * inv_t;
+  return (double)rest - fma(fma(-q, (double)temperature, (double)hi), inv_t, q);
+}
+
 // a row that takes no part; no counted row has this reference with a factor of zero
 __device__ __forceinline__ RowStats not_counted() { return RowStats{__builtin_inff(), 0.f, 0.f, 0.f}; }
 
@@ -97,7 +104,7 @@ struct SlotShared {
 // fp64 and the shares rounded once: the loss is the difference of near-equal logarithms once the student is near the
 // teacher (104 rows of 1231 classes at temperature 4: fp32 exponentials here cost 1.4e-6 of it, 3e-7 in the student's sums).
 template <bool LONG>
-__device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int K, double inv_t, int lane, SlotShared& sh) {
+__device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int K, double inv_t, float temperature, int lane, SlotShared& sh) {
   const int k = t.o.K;
   const int64_t at = row_offset(t.o, r);
   float v[2];
@@ -119,10 +126,10 @@ __device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int K, 
     }
   }
   const int state = !__any(any) ? 0 : __any(bad) ? 2 : 1;
-  // The largest value is taken off before anything is scaled, and off the rest in one rounding (a fused multiply-add): of a
-  // teacher whose values are all the type's lowest the small differences stay.
+  // The largest value is taken off before anything is scaled: of a teacher whose values are all the type's lowest the small
+  // differences stay.
   const float hi = wave_max(fmaxf(v[0], v[1]));
-  const double yr = t.rest ? fma(-(double)hi, inv_t, (double)t.rest[r]) : -__builtin_inf(), shift = fmax(yr, 0.);
+  const double yr = t.rest ? rest_gap(t.rest[r], hi, inv_t, temperature) : -__builtin_inf(), shift = fmax(yr, 0.);
   double y[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) y[u] = v[u] == neg_inf() ? -__builtin_inf() : ((double)v[u] - (double)hi) * inv_t;
@@ -161,7 +168,7 @@ __device__ __forceinline__ bool row_masked(const Teacher& t, int64_t r) { return
 // (without rest its share of the teacher is zero, and the student's share of those classes is summed apart all the same)
 template <typename T, bool UNIT, int BS>
 __global__ void __launch_bounds__(BS, BS == 256 ? 8 : BS == 1024 ? 4 : 1)
-k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, double t2, RowStats* __restrict__ stats,
+k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, double inv_t, float temperature, RowStats* __restrict__ stats,
               float* __restrict__ per_row, double* __restrict__ partial) {
   constexpr bool LONG = BS > 64;
   __shared__ SlotShared sh;
@@ -192,7 +199,7 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
       if (LONG) break;
       continue;
     }
-    if (tid < 64) teacher_row<LONG>(t, r, K, inv_t, tid, sh);
+    if (tid < 64) teacher_row<LONG>(t, r, K, inv_t, temperature, tid, sh);
     // running maximum and sum of the classes in no slot: fp32, in which a thread adds trees of 16 or 32 classes in turn; what that
     // and the exponentials leave over is in every logarithm of the row and drops out of its loss (kl_part)
     float m = neg_inf(), acc = 0.f;
@@ -314,7 +321,7 @@ k_distill_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
         const double inv = sum > 0. ? end_div<LONG>(1., sum) : sum == 0. ? 0. : sum;
         // q = exp((z - m_rest)/T) * w before the teacher's share of the rest is taken off
         const double w = m_rest == neg_inf() ? 0. : inv * to_m - end_div<LONG>(sh.p_rest, sum_rest);
-        const double loss = t2 * kl;
+        const double loss = (double)temperature * (double)temperature * kl;
         if (per_row) per_row[r] = (float)loss;
         if (stats) stats[r] = RowStats{ref, (float)w, (float)m_d, (float)inv};
         loss_sum += loss;
@@ -378,7 +385,7 @@ k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
     RowStats st = not_counted();
     if (!row_masked(t, r)) st = stats[r];
     const bool live = !(st.ref == __builtin_inff() && st.w == 0.f);
-    if (live && tid < 64) teacher_row<LONG>(t, r, K, inv_t, tid, sh);       // for the listed classes, at the end
+    if (live && tid < 64) teacher_row<LONG>(t, r, K, inv_t, temperature, tid, sh);       // for the listed classes, at the end
     const float g = grad_rows ? grad[r] : grad[0] * scal[0];
     const float f = g * temperature;
     const float w = f * st.w;
@@ -490,7 +497,7 @@ __device__ __forceinline__ double few_rcp(double x) { return 1. / x; }
 // dropped at the end.
 template <typename T, int KT, int KS, bool FULL, bool REST, int WANT, typename S>
 __device__ __forceinline__ void few_row(const T* __restrict__ z, const RowShape& s, const Teacher& t, int64_t n, int64_t v0,
-                                        uint32_t lane, float scale, double inv_t, FewRow<KT, KS, S>& w) {
+                                        uint32_t lane, float scale, double inv_t, float temperature, FewRow<KT, KS, S>& w) {
   const int K = s.K, k = t.o.K;
   const double scale_d = inv_t * 1.4426950408889634;
   const int64_t r0 = n * s.V + v0, at = n * t.o.sN + v0 * t.o.sV;
@@ -545,7 +552,9 @@ __device__ __forceinline__ void few_row(const T* __restrict__ z, const RowShape&
   double a_rest = -__builtin_inf();
   S shift = 0;
   if constexpr (REST) {
-    a_rest = fma(-(double)hi, inv_t, (double)rest) * 1.4426950408889634;     // one rounding before the large parts cancel
+    a_rest = rest_gap(rest, hi, inv_t, temperature) * 1.4426950408889634;
+    // from here on the rest is all of the teacher, and a number that S holds as it is cancels where it has to
+    a_rest = a_rest > 4096. && a_rest < __builtin_inf() ? 4096. : a_rest;
     shift = (S)fmax(a_rest, 0.);
   }
   w.rest_alive = REST && !(a_rest - (double)shift < NO_SHARE);
@@ -612,7 +621,7 @@ k_distill_few_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
       const uint32_t lane = lane_id();
       if (v0 + lane >= s.V) continue;
       FewRow<KT, KS, S> w;
-      few_row<T, KT, KS, FULL, true, ROWS ? FEW_ROW_LOSS : FEW_MEAN_LOSS>(z, s, t, n, v0, lane, scale, inv_t, w);
+      few_row<T, KT, KS, FULL, true, ROWS ? FEW_ROW_LOSS : FEW_MEAN_LOSS>(z, s, t, n, v0, lane, scale, inv_t, temperature, w);
       S sum = 0;
       bool barred = false;                     // a listed class has probability zero
       if constexpr (ROWS) {
@@ -687,7 +696,7 @@ k_distill_few_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, d
       if (v0 + lane >= s.V) continue;
       const float f = temperature * (grad_rows ? lane_load(grad + n * s.V + v0, lane) : g_all);
       FewRow<KT, KS, float> w;
-      few_row<T, KT, KS, FULL, REST, FEW_GRADIENT>(z, s, t, n, v0, lane, scale, inv_t, w);
+      few_row<T, KT, KS, FULL, REST, FEW_GRADIENT>(z, s, t, n, v0, lane, scale, inv_t, temperature, w);
       const float w_rest = REST && w.sum_rest != 0.f ? w.to_m * w.inv - w.p_rest * rcp_f(w.sum_rest) : 0.f;
       const float fill = w.state ? __builtin_nanf("") : 0.f;
       float out[KT];
@@ -773,7 +782,7 @@ k_distill_lane_fwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, 
       const float ref = left.m == neg_inf() ? 0.f : left.m;
       const double d_rest = left.m == neg_inf() ? 0. : ((double)left.m - (double)m) * scale_d, to_m = exp2_series(d_rest);
       const double sum = left.s * to_m + (in.m == neg_inf() ? in.s : in.s * exp2_series(((double)in.m - (double)m) * scale_d));
-      const double a_rest = t.rest ? fma(-(double)hi, inv_t, (double)t.rest[r]) * 1.4426950408889634 : -__builtin_inf();
+      const double a_rest = t.rest ? rest_gap(t.rest[r], hi, inv_t, temperature) * 1.4426950408889634 : -__builtin_inf();
       const double shift = fmax(a_rest, 0.), e_rest = exp2_series(a_rest - shift);
       double sum_t = e_rest;
       each_slot(t, at, K, [&](int, float v, int) { sum_t += exp2_series(fma((double)v - (double)hi, scale_d, -shift)); });
@@ -845,7 +854,7 @@ k_distill_lane_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, 
       float hi = neg_inf(), shift = 0.f, sum = 0.f;
       each_slot(t, at, K, [&](int, float v, int) { hi = fmaxf(hi, v); });
       if (t.rest) {
-        const float a_rest = (float)(fma(-(double)hi, inv_t, (double)t.rest[r]) * 1.4426950408889634);
+        const float a_rest = (float)(rest_gap(t.rest[r], hi, inv_t, temperature) * 1.4426950408889634);
         shift = fmaxf(a_rest, 0.f);
         sum = exp2_f(a_rest - shift);
       }
@@ -932,7 +941,7 @@ int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* 
   if (loss && ws_bytes < devis_distill_workspace_bytes(a)) return DEVIS_ERR_WORKSPACE;
   RowShape s = student_rows(a);
   Teacher t = {a->values, a->indices, a->rest, a->row_mask, slot_rows(a), a->values_dtype, a->index_dtype};
-  const double inv_t = 1.0 / (double)a->temperature, t2 = (double)a->temperature * (double)a->temperature;
+  const double inv_t = 1.0 / (double)a->temperature;
   const float scale = (float)(1.4426950408889634 * inv_t);
   const bool unit = a->sK == 1;
   const dim3 rows = distill_grid(a);
@@ -952,7 +961,7 @@ int devis_distill_fwd(const devis_distill_params* a, const void* logits, float* 
     DEVIS_DISPATCH_DTYPE(a->dtype, { if (unit) LAUNCH_LANE(true); else LAUNCH_LANE(false); });
 #undef LAUNCH_LANE
   } else {
-#define LAUNCH_DISTILL_FWD(UNIT, BS) hipLaunchKernelGGL((k_distill_fwd<T, UNIT, BS>), rows, dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, t2, (RowStats*)stats, per_row, part)
+#define LAUNCH_DISTILL_FWD(UNIT, BS) hipLaunchKernelGGL((k_distill_fwd<T, UNIT, BS>), rows, dim3(BS), 0, (hipStream_t)stream, (const T*)logits, s, t, scale, inv_t, a->temperature, (RowStats*)stats, per_row, part)
     DISTILL_DISPATCH(LAUNCH_DISTILL_FWD);
   }
 #undef LAUNCH_DISTILL_FWD

@@ -165,3 +165,24 @@ def test_a_class_in_two_slots_of_a_student_near_its_teacher(rows, K, k, T):
             for n in some:
                 have[n] = criterions.distill_top_loss(*(x[n:n + 1] for x in args), temperature=T, reduction="sum").item()
         assert ((have - want).abs() <= tol).all(), (reduction, ((have - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("T", [1.5, 3.0, 0.75, 1.3, 48.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K, times", [(6, 1), (16, 700), (40, 2100), (300, 1), (3001, 1)])
+def test_a_teacher_of_lowest_values_at_other_temperatures(K, times, dtype, T):
+    """A masked teacher's row: its rest is the row's value over T, and so is every slot, to the last digit or far from it; a quotient by
+    way of a rounded 1 / T would be 1e22 off and give all to one side."""
+    from tests.test_gpu_classdist import check_distill, logits, teacher_of
+    T = float(np.float32(T))
+    z = logits(4, K, dtype, K, 2.0)
+    t = torch.full((4, K), torch.finfo(dtype).min).to(dtype)
+    t[1] = torch.finfo(dtype).min / 2
+    t[2, :1] = 1.0
+    t[3] = -1e30
+    if T < 1:
+        t[0] /= 16
+    for k in {1, 2, 6}:
+        v, i, rest = teacher_of(t, k, T)
+        for reduction in ("mean", "none"):
+            check_distill(z, v, i, rest, None, T, reduction, times=times)
