@@ -464,6 +464,8 @@ __device__ __forceinline__ float kl_part(float p, float q, float l, float pd, fl
 //   p (r - 1 - log r),  r = q / p,   instead of   -p log r :
 // the same total, because the p and the q each sum to one, of terms that are never negative and do not cancel; and an error e
 // that all log r of a row share, as that of a logarithm of a sum, changes the total by sum p (r - 1) e = 0 and e^2 / 2.
+// (A share below 2^-126 of a class that is open to the student counts as zero in a mean: what it adds is less than 1e-38 of the
+// logits' distance.)
 enum { FEW_GRADIENT, FEW_MEAN_LOSS, FEW_ROW_LOSS };
 
 // KS bounds the slots as KT bounds the classes; S is the type of shares and sums.
