@@ -10,7 +10,7 @@
 // once with a running maximum and sum per thread, keeping the classes in no slot apart (a bit per class in LDS tells
 // them); the backward reads it once more and writes the gradient: for a class in no slot it is one exponential times a
 // factor of the row, W = 1/s - p_rest/s_rest; the k listed classes are put right afterwards.  4096 x 131072 bf16, 64 slots
-// and rest: forward 196 us (5.5 TB/s), backward 403 us (5.3 TB/s; a copy moves 5.0), together 616.
+// and rest: forward 196 us (5.5 TB/s), backward 402 us (5.3 TB/s; a copy moves 5.0), together 614.
 #include "rows.h"
 
 #include <type_traits>
@@ -419,8 +419,8 @@ k_distill_bwd(const T* __restrict__ z, RowShape s, Teacher t, float scale, doubl
 
 // ---- few classes: one thread a row, everything in registers, nothing kept for the backward.  For a mean and for
 // the gradient exponentials and logarithms are fp32 (FEW_ROW_LOSS below: fp64).  Sums over rows are fp64.  2 x 128^3 x 4
-// bf16, two slots and rest: 37 us forward, 31 backward (75 and 109 MB; VALU issue is 91 and 84 % busy: 255 and 187 instructions
-// a row); 71 us for the loss of every row.
+// bf16, two slots and rest: 37 us forward, 32 backward (75 and 109 MB; VALU issue is 91 and 83 % busy: 265 and 199 instructions
+// a row); 70 us for the loss of every row.
 __device__ __forceinline__ float log2_f(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ float rcp_f(float x) { return __builtin_amdgcn_rcpf(x); }
 

@@ -104,7 +104,7 @@ __device__ __forceinline__ void each_weight(const Draw<T>& d, int lo, int hi, in
 
 // One block a sequence, of 64, 256 or 1024 threads (verify_threads).  Each wave sums the weights of one stretch of the row; the
 // stretch in which the goal lies is read once more, a vector a thread, and the class found by a prefix sum over the block.
-// 200 sequences of 7 drafts over 131072 bf16 classes: 22.5 us, 105 MB; one sequence of 4 over 32768 fp32: 8.1 us.
+// 200 sequences of 7 drafts over 131072 bf16 classes: 22 us, 105 MB; one sequence of 4 over 32768 fp32: 8.3 us.
 template <typename T, bool UNIT, bool DRAFTER, int BS>
 __global__ void __launch_bounds__(BS)
 k_verify(const T* __restrict__ p, const T* __restrict__ q, VerifyArgs a) {
